@@ -27,7 +27,8 @@ EXPORTS = (
     "clipvit_gemm_mx8_test", "clipvit_preprocess", "clipvit_resample_plan",
     "clipvit_text_create", "clipvit_text_load_weights", "clipvit_text_load_lora",
     "clipvit_encode_text", "clipvit_text_destroy", "clipvit_residual_x24_test", "clipvit_set_tuning",
-    "clipvit_gemm_log",
+    "clipvit_gemm_log", "clipvit_linear_workspace", "clipvit_linear", "clipvit_linear_dz", "clipvit_dropout",
+    "clipvit_lora_pad", "clipvit_lora_down", "clipvit_lora_grad_workspace", "clipvit_lora_grad",
 )
 
 
@@ -63,6 +64,33 @@ class Lora(ctypes.Structure):
                 ("out_features", ctypes.c_int), ("rank", ctypes.c_int), ("scaling", ctypes.c_float)]
 
 
+class DropoutArgs(ctypes.Structure):
+    _fields_ = [("p", ctypes.c_double), ("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64),
+                ("offset_dev", ctypes.c_void_p)]
+
+
+class LinearArgs(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int), ("activation", ctypes.c_int), ("bias_dtype", ctypes.c_int),
+                ("low_mask", ctypes.c_int), ("M", ctypes.c_int64), ("N", ctypes.c_int64),
+                ("K", ctypes.c_int64), ("R", ctypes.c_int64), ("x", ctypes.c_void_p),
+                ("x_stride", ctypes.c_int64 * 2), ("w", ctypes.c_void_p), ("w_stride", ctypes.c_int64 * 2),
+                ("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("residual_stride", ctypes.c_int64),
+                ("y", ctypes.c_void_p), ("y_stride", ctypes.c_int64), ("slope", ctypes.c_void_p),
+                ("low_u", ctypes.c_void_p), ("low_v", ctypes.c_void_p), ("dropout", DropoutArgs)]
+
+
+class DzArgs(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int), ("db_dtype", ctypes.c_int), ("M", ctypes.c_int64), ("N", ctypes.c_int64),
+                ("dy", ctypes.c_void_p), ("dy_stride", ctypes.c_int64), ("slope", ctypes.c_void_p),
+                ("dz", ctypes.c_void_p), ("dz_stride", ctypes.c_int64), ("db", ctypes.c_void_p),
+                ("dropout", DropoutArgs)]
+
+
+class PadArgs(ctypes.Structure):
+    _fields_ = [("src", ctypes.c_void_p)] + [(n, ctypes.c_int64) for n in (
+        "row_stride", "col_stride", "rows", "cols", "rows_padded", "cols_padded")] + [("dst", ctypes.c_void_p)]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -79,6 +107,7 @@ def lib() -> ctypes.CDLL:
             raise ClipVitError(E_STATE, f"{LIB_PATH} is not built (run __graft_entry__.build())")
         L = ctypes.CDLL(str(LIB_PATH))
         vp, i, p_f = ctypes.c_void_p, ctypes.c_int, ctypes.POINTER(ctypes.c_float)
+        i64, sz = ctypes.c_int64, ctypes.c_size_t
         sig = {
             "clipvit_create": (i, [ctypes.POINTER(Config), i, ctypes.POINTER(vp)]),
             "clipvit_set_tuning": (i, [vp, ctypes.c_char_p]),
@@ -107,6 +136,16 @@ def lib() -> ctypes.CDLL:
             "clipvit_preprocess": (i, [vp, vp, ctypes.POINTER(Image), i, i, i, vp]),
             "clipvit_resample_plan": (i, [i, i, ctypes.POINTER(i), ctypes.POINTER(i),
                                           ctypes.POINTER(ctypes.c_int32), i]),
+            "clipvit_linear_workspace": (i, [ctypes.POINTER(LinearArgs), ctypes.POINTER(sz)]),
+            "clipvit_linear": (i, [vp, ctypes.POINTER(LinearArgs), vp, sz]),
+            "clipvit_linear_dz": (i, [vp, ctypes.POINTER(DzArgs), vp, sz]),
+            "clipvit_dropout": (i, [vp, i, vp, i64, vp, i64, vp, i64, i64, i64, ctypes.POINTER(DropoutArgs)]),
+            "clipvit_lora_pad": (i, [vp, ctypes.POINTER(PadArgs), ctypes.POINTER(PadArgs)]),
+            "clipvit_lora_down": (i, [vp, i, vp, i64, vp, i64, vp, i64, i64, i64, ctypes.c_float,
+                                      ctypes.POINTER(DropoutArgs)]),
+            "clipvit_lora_grad_workspace": (i, [i64, i64, i64, ctypes.POINTER(sz)]),
+            "clipvit_lora_grad": (i, [vp, i, vp, i64, vp, vp, i64, i64, i64, i64, i64, i64,
+                                      ctypes.POINTER(DropoutArgs), vp, sz]),
         }
         for name, (res, args) in sig.items():
             fn = getattr(L, name)

@@ -1,0 +1,230 @@
+// Shared pieces of the fine-tuning operators (matmul.hip, finetune.hip): the counter-based dropout
+// generator, the activations with their derivatives and the epilogue of a matrix product.
+#pragma once
+#include "common.h"
+
+namespace clipvit {
+
+// ---- dropout ----
+// Philox4x32-10 (J. Salmon, M. Moraes, R. Dror, D. Shaw, "Parallel random numbers: as easy as 1, 2, 3",
+// SC 2011): ten rounds of two 32 x 32 -> 64-bit products on a 128-bit counter. The counter of element
+// (row m, column n) is (n / 4, m, offset), its word n % 4, the key is the 64-bit seed, so the mask is a
+// function of the element's place and never stored: the backward pass computes it again. An element is
+// kept when its word exceeds `drop_max` = round(p 2^32) - 1 (so p = 1 keeps nothing).
+struct Dropout {
+    unsigned k0, k1;         // seed
+    unsigned o0, o1;         // offset (when offset_dev is null)
+    const uint2* offset_dev; // offset read on the device: a captured graph draws a new mask per replay
+    unsigned drop_max;
+    float scale;             // 1 / (1 - p), 0 for p = 1
+    int on;                  // 0: no dropout (p rounds to 0)
+};
+
+__device__ __forceinline__ uint4 philox4(unsigned quad, unsigned row, unsigned o0, unsigned o1, unsigned k0, unsigned k1) {
+    unsigned c0 = quad, c1 = row, c2 = o0, c3 = o1;
+#pragma unroll
+    for (int r = 0; r < 10; ++r) {
+        const unsigned long long a = (unsigned long long)c0 * 0xD2511F53u, b = (unsigned long long)c2 * 0xCD9E8D57u;
+        c0 = (unsigned)(b >> 32) ^ c1 ^ k0;
+        c1 = (unsigned)b;
+        c2 = (unsigned)(a >> 32) ^ c3 ^ k1;
+        c3 = (unsigned)a;
+        k0 += 0x9E3779B9u;
+        k1 += 0xBB67AE85u;
+    }
+    return make_uint4(c0, c1, c2, c3);
+}
+__device__ __forceinline__ uint2 drop_offset(const Dropout& d) {
+    return d.offset_dev ? *d.offset_dev : make_uint2(d.o0, d.o1);
+}
+// four consecutive columns (n % 4 == 0) of row m: kept values scaled, dropped ones exactly 0 (whatever
+// they held, NaN included)
+__device__ __forceinline__ void drop4(const Dropout& d, const uint2& o, int m, int n, float scale, float& a, float& b, float& c, float& e) {
+    const uint4 w = philox4((unsigned)n >> 2, (unsigned)m, o.x, o.y, d.k0, d.k1);
+    a = w.x > d.drop_max ? a * scale : 0.f;
+    b = w.y > d.drop_max ? b * scale : 0.f;
+    c = w.z > d.drop_max ? c * scale : 0.f;
+    e = w.w > d.drop_max ? e * scale : 0.f;
+}
+
+// ---- activations ----
+// z Phi-like gates: quick_gelu z s(1.702 z), silu z s(z) (s the logistic function by v_exp_f32 and
+// v_rcp_f32: relative error a few 2^-23), gelu z (1 + erf(z / sqrt 2)) / 2, gelu_tanh with the tanh written
+// as a logistic: (1 + tanh t) / 2 = s(2 t).
+enum Act { ACT_NONE = 0, ACT_QUICK_GELU = 1, ACT_GELU = 2, ACT_GELU_TANH = 3, ACT_SILU = 4, ACT_RELU = 5 };
+
+__device__ __forceinline__ float logistic(float t) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * t));
+}
+// value and derivative; the derivative's z factors are clamped so that it reaches its limit (0 or 1) at
+// +-inf instead of inf * 0 (a NaN z gives NaN through the gate)
+template <bool SLOPE>
+__device__ __forceinline__ float act_apply(int act, float z, float& slope) {
+    const float zc = SLOPE ? fminf(fmaxf(z, -100.f), 100.f) : z;
+    if (act == ACT_QUICK_GELU || act == ACT_SILU) {
+        const float beta = act == ACT_SILU ? 1.0f : 1.702f;
+        const float s = logistic(beta * z);
+        if (SLOPE) slope = s * (1.0f + beta * zc * (1.0f - s));
+        return z * s;
+    }
+    if (act == ACT_GELU) {
+        const float c = 0.5f + 0.5f * erff(0.70710678118654752f * z);
+        if (SLOPE) slope = c + 0.39894228040143268f * zc * __builtin_amdgcn_exp2f(-0.72134752044448170f * zc * zc);
+        return z * c;
+    }
+    if (act == ACT_GELU_TANH) {
+        const float z2 = zc * zc;
+        const float s = logistic(1.5957691216057308f * (z + 0.044715f * z * (z * z)));
+        if (SLOPE) slope = s + zc * s * (1.0f - s) * (1.5957691216057308f * (1.0f + 0.134145f * z2));
+        return z * s;
+    }
+    if (act == ACT_RELU) {
+        if (SLOPE) slope = z != z ? z : (z > 0.f ? 1.f : 0.f);
+        return z != z ? z : fmaxf(z, 0.f);
+    }
+    slope = 1.f;
+    return z;
+}
+// The derivative as the forward saves it: 16-bit fixed point, steps of 2^-14. All of these derivatives
+// lie in (-0.13, 1.13), so the rounding is at most 2^-15 absolute, 16 times below the half step of an fp16
+// value near 1 (2^-12 relative) that dz is rounded to afterwards; the code -32768 stands for NaN.
+__device__ __forceinline__ short slope_encode(float g) {
+    return g != g ? (short)-32768 : (short)__float2int_rn(fminf(fmaxf(g, -1.9f), 1.9f) * 16384.f);
+}
+__device__ __forceinline__ float slope_decode(short q) {
+    return q == -32768 ? __builtin_nanf("") : (float)q * (1.0f / 16384.f);
+}
+
+// ---- epilogue of C = A B^T ----
+//   z = acc + bias + low-rank term;  y = residual + dropout(act(z));  slope = act'(z)
+struct Epilogue {
+    void* y;               // [M, N] 16-bit, row stride ldy
+    const void* bias;      // [N] or null
+    const void* res;       // [M, N] 16-bit or null, row stride ldr
+    short* slope;          // [M, N] contiguous (row stride N) or null
+    int64_t ldy, ldr;
+    int M, N;
+    int bias_f32, act;
+    int vec;               // every 8-column group of y, res and slope rows is 16-byte aligned
+    Dropout drop;
+    // low-rank term u v^T (u [M, R], v [N, R], both zero-padded to R % 32 == 0 columns); low_mask: the
+    // dropout mask (scale 1) is applied to this term instead of the activation's value
+    const u16 *lu, *lv;
+    int R, low_mask;
+};
+
+// C consecutive columns n .. n + C - 1 (n % 4 == 0) of row m: v = acc (+ an unmasked low-rank term), t = the
+// masked low-rank term (LOW) or unused. Columns at or past N are not touched.
+template <typename T, int C, bool LOW>
+__device__ __forceinline__ void epilogue_cols(const Epilogue& e, const uint2& off, int m, int n, float (&v)[C], float (&t)[C]) {
+    const int nc = min(C, e.N - n);
+    if (m >= e.M || nc <= 0) return;
+    const bool whole = nc == C && e.vec;
+    if (e.bias) {
+        if (e.bias_f32) {
+            const float* b = (const float*)e.bias + n;
+#pragma unroll
+            for (int j = 0; j < C; ++j)
+                if (j < nc) v[j] += b[j];
+        } else {
+            const u16* b = (const u16*)e.bias + n;
+#pragma unroll
+            for (int j = 0; j < C; ++j)
+                if (j < nc) v[j] += T::to_f32(b[j]);
+        }
+    }
+    if constexpr (LOW) {
+#pragma unroll
+        for (int j = 0; j < C; j += 4) drop4(e.drop, off, m, n + j, 1.0f, t[j], t[j + 1], t[j + 2], t[j + 3]);
+#pragma unroll
+        for (int j = 0; j < C; ++j) v[j] += t[j];
+    }
+    if (e.act != ACT_NONE) {
+        if (e.slope) {
+            short q[C];
+#pragma unroll
+            for (int j = 0; j < C; ++j) {
+                float g;
+                v[j] = act_apply<true>(e.act, v[j], g);
+                q[j] = slope_encode(g);
+            }
+            short* s = e.slope + (int64_t)m * e.N + n;
+            if (whole) {
+                if constexpr (C % 8 == 0) {
+#pragma unroll
+                    for (int j = 0; j < C; j += 8) {
+                        uint4 w;
+                        __builtin_memcpy(&w, q + j, 16);
+                        *(uint4*)(s + j) = w;
+                    }
+                } else {
+                    uint2 w;
+                    __builtin_memcpy(&w, q, 8);
+                    *(uint2*)s = w;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < C; ++j)
+                    if (j < nc) s[j] = q[j];
+            }
+        } else {
+            float g;
+#pragma unroll
+            for (int j = 0; j < C; ++j) v[j] = act_apply<false>(e.act, v[j], g);
+        }
+    }
+    if (!LOW && e.drop.on) {
+#pragma unroll
+        for (int j = 0; j < C; j += 4) drop4(e.drop, off, m, n + j, e.drop.scale, v[j], v[j + 1], v[j + 2], v[j + 3]);
+    }
+    u16* y = (u16*)e.y + (int64_t)m * e.ldy + n;
+    const u16* r = e.res ? (const u16*)e.res + (int64_t)m * e.ldr + n : nullptr;
+    if (whole) {
+        if (r) {
+            u16 rr[C];
+            if constexpr (C % 8 == 0) {
+#pragma unroll
+                for (int j = 0; j < C; j += 8) {
+                    const uint4 w = *(const uint4*)(r + j);
+                    __builtin_memcpy(rr + j, &w, 16);
+                }
+            } else {
+                const uint2 w = *(const uint2*)r;
+                __builtin_memcpy(rr, &w, 8);
+            }
+#pragma unroll
+            for (int j = 0; j < C; ++j) v[j] += T::to_f32(rr[j]);
+        }
+        if constexpr (C % 8 == 0) {
+#pragma unroll
+            for (int j = 0; j < C; j += 8)
+                *(uint4*)(y + j) = make_uint4(pack2<T>(v[j], v[j + 1]), pack2<T>(v[j + 2], v[j + 3]),
+                                              pack2<T>(v[j + 4], v[j + 5]), pack2<T>(v[j + 6], v[j + 7]));
+        } else {
+            *(uint2*)y = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+            if (j < nc) y[j] = T::from_f32(r ? v[j] + T::to_f32(r[j]) : v[j]);
+    }
+}
+
+// ---- matrix product C = A B^T (matmul.hip) ----
+// A(m, k) at A + m * lda + k (a_k) or A + k * lda + m; B(n, k) likewise. Any M, N, K >= 0.
+struct Matmul {
+    const u16 *A, *B;
+    int64_t lda, ldb;
+    int a_k, b_k;
+    int M, N, K;
+    Epilogue e;
+};
+// bytes of device workspace that launch_matmul needs for this shape, strides and alignment
+size_t matmul_workspace(const Matmul& a);
+// 0, or -1 when the workspace is too small
+int launch_matmul(hipStream_t s, int dtype, const Matmul& a, void* ws, size_t ws_bytes);
+
+// largest row stride (elements) the tiles' 32-bit in-tile offsets allow
+constexpr int64_t MATMUL_MAX_LD = 1 << 22;
+
+}  // namespace clipvit

@@ -1,0 +1,743 @@
+// Fine-tuning operators: counter-based dropout, a Linear's dz and bias gradient, the low-rank adapter's
+// thin products, and the C entry points of all of them (the matrix product itself is matmul.hip).
+//
+// A Linear with an adapter (main.py:19-59): y = x W^T + b + s (dropout(x) A) B. The reference runs the
+// adapter as a side branch while it trains (train_lora.py) and this library merges it for inference
+// (clipvit_load_lora); these operators are the unmerged form with its gradients.
+#include <cmath>
+#include <string>
+
+#include "clipvit.h"
+#include "finetune.h"
+
+namespace clipvit {
+
+extern thread_local std::string g_err;
+
+namespace {
+
+// ---- element access: 32- or 16-bit storage, fp32 arithmetic ----
+struct F32T {
+    typedef float store;
+    static __device__ __forceinline__ float to_f32(float v) { return v; }
+    static __device__ __forceinline__ float from_f32(float v) { return v; }
+};
+struct BF16T {
+    typedef u16 store;
+    static __device__ __forceinline__ float to_f32(u16 v) { return BF16::to_f32(v); }
+    static __device__ __forceinline__ u16 from_f32(float v) { return BF16::from_f32(v); }
+};
+struct F16T {
+    typedef u16 store;
+    static __device__ __forceinline__ float to_f32(u16 v) { return F16::to_f32(v); }
+    static __device__ __forceinline__ u16 from_f32(float v) { return F16::from_f32(v); }
+};
+// C consecutive elements, nc of them valid; 16 bytes at a time where `vec` says so and all are valid
+template <class E, int C>
+__device__ __forceinline__ void load_cols(const typename E::store* p, int nc, bool vec, float (&v)[C]) {
+    constexpr int PER = 16 / sizeof(typename E::store);
+    if (vec && nc >= C) {
+#pragma unroll
+        for (int j = 0; j < C; j += PER) {
+            typename E::store t[PER];
+            const uint4 w = *(const uint4*)(p + j);
+            __builtin_memcpy(t, &w, 16);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) v[j + i] = E::to_f32(t[i]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < C; ++j) v[j] = j < nc ? E::to_f32(p[j]) : 0.f;
+    }
+}
+template <class E, int C>
+__device__ __forceinline__ void store_cols(typename E::store* p, int nc, bool vec, const float (&v)[C]) {
+    constexpr int PER = 16 / sizeof(typename E::store);
+    if (vec && nc >= C) {
+#pragma unroll
+        for (int j = 0; j < C; j += PER) {
+            typename E::store t[PER];
+#pragma unroll
+            for (int i = 0; i < PER; ++i) t[i] = E::from_f32(v[j + i]);
+            uint4 w;
+            __builtin_memcpy(&w, t, 16);
+            *(uint4*)(p + j) = w;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+            if (j < nc) p[j] = E::from_f32(v[j]);
+    }
+}
+
+// ---- dropout: y = residual + mask(x) scale; eight columns a thread ----
+struct DropArgs {
+    const void *x, *res;
+    void* y;
+    int64_t ldx, ldr, ldy;
+    int rows, cols, vec, tx;  // tx threads cover tx * 8 columns, 256 / tx rows a step
+    Dropout d;
+};
+template <class E>
+__global__ __launch_bounds__(256) void dropout_kernel(DropArgs a) {
+    typedef typename E::store S;
+    const int c = ((int)blockIdx.x * a.tx + (int)threadIdx.x % a.tx) * 8;
+    const int ty = (int)threadIdx.x / a.tx, ny = 256 / a.tx;
+    if (c >= a.cols) return;
+    const int nc = min(8, a.cols - c);
+    const uint2 off = drop_offset(a.d);
+    for (int64_t m = (int64_t)blockIdx.y * ny + ty; m < a.rows; m += (int64_t)gridDim.y * ny) {
+        float v[8];
+        load_cols<E, 8>((const S*)a.x + m * a.ldx + c, nc, a.vec, v);
+        if (a.d.on) {
+            drop4(a.d, off, (int)m, c, a.d.scale, v[0], v[1], v[2], v[3]);
+            drop4(a.d, off, (int)m, c + 4, a.d.scale, v[4], v[5], v[6], v[7]);
+        }
+        if (a.res) {
+            float r[8];
+            load_cols<E, 8>((const S*)a.res + m * a.ldr + c, nc, a.vec, r);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] += r[j];
+        }
+        store_cols<E, 8>((S*)a.y + m * a.ldy + c, nc, a.vec, v);
+    }
+}
+
+// ---- dz = dropout(dy) * act'(z), and the column sums of the unrounded dz for the bias gradient ----
+struct DzArgs {
+    const void* dy;
+    const short* slope;  // [M, N] or null
+    void* dz;            // [M, lddz] or null
+    float* part;         // [gridDim.y][N] column sums of a block's rows, or null
+    int64_t lddy, lddz;
+    int M, N, rows, vec;  // rows of a block
+    Dropout d;
+};
+template <class E>
+__global__ __launch_bounds__(256) void dz_kernel(DzArgs a) {
+    typedef typename E::store S;
+    __shared__ float sums[8][32][9];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int c = ((int)blockIdx.x * 32 + tx) * 8;
+    const int nc = min(8, a.N - c);
+    float s[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] = 0.f;
+    if (nc > 0) {
+        const uint2 off = drop_offset(a.d);
+        const int64_t m1 = min((int64_t)a.M, ((int64_t)blockIdx.y + 1) * a.rows);
+        for (int64_t m = (int64_t)blockIdx.y * a.rows + ty; m < m1; m += 8) {
+            float v[8];
+            load_cols<E, 8>((const S*)a.dy + m * a.lddy + c, nc, a.vec, v);
+            if (a.d.on) {
+                drop4(a.d, off, (int)m, c, a.d.scale, v[0], v[1], v[2], v[3]);
+                drop4(a.d, off, (int)m, c + 4, a.d.scale, v[4], v[5], v[6], v[7]);
+            }
+            if (a.slope) {
+                const short* q = a.slope + m * a.N + c;
+                short t[8];
+                if (a.vec && nc == 8) {
+                    const uint4 w = *(const uint4*)q;
+                    __builtin_memcpy(t, &w, 16);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) t[j] = j < nc ? q[j] : (short)0;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] *= slope_decode(t[j]);
+            }
+            if (a.dz) store_cols<E, 8>((S*)a.dz + m * a.lddz + c, nc, a.vec, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s[j] += v[j];
+        }
+    }
+    if (!a.part) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sums[ty][tx][j] = s[j];
+    __syncthreads();
+    if (ty == 0 && nc > 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float t = 0.f;
+#pragma unroll
+            for (int y = 0; y < 8; ++y) t += sums[y][tx][j];
+            if (j < nc) a.part[(int64_t)blockIdx.y * a.N + c + j] = t;
+        }
+    }
+}
+// db = the blocks' column sums in a fixed order; 32 columns a block, eight slices of the blocks each
+template <class E>
+__global__ __launch_bounds__(256) void db_kernel(const float* __restrict__ part, int blocks, int N, void* db, int db_f32) {
+    __shared__ float sums[8][33];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int n = blockIdx.x * 32 + tx;
+    float s = 0.f;
+    if (n < N)
+        for (int b = ty; b < blocks; b += 8) s += part[(int64_t)b * N + n];
+    sums[ty][tx] = s;
+    __syncthreads();
+    if (ty || n >= N) return;
+    float t = 0.f;
+#pragma unroll
+    for (int y = 0; y < 8; ++y) t += sums[y][tx];
+    if (db_f32) ((float*)db)[n] = t;
+    else ((typename E::store*)db)[n] = E::from_f32(t);
+}
+
+// ---- low-rank factors, zero padded: dst[i][j] = src(i, j), i < I (zeros past ri), j < J (zeros past rj) ----
+struct PadArgs {
+    const u16* src;
+    int64_t s0, s1;
+    int ri, rj, I, J;
+    u16* dst;
+};
+__global__ __launch_bounds__(256) void pad_kernel(PadArgs a, PadArgs b, int blocks_a) {
+    const bool first = (int)blockIdx.x < blocks_a;
+    const PadArgs& p = first ? a : b;
+    const int64_t i = ((int64_t)blockIdx.x - (first ? 0 : blocks_a)) * 256 + threadIdx.x;
+    const int64_t r = i / p.J;
+    const int c = (int)(i - r * p.J);
+    if (r >= p.I) return;
+    p.dst[i] = r < p.ri && c < p.rj ? p.src[r * p.s0 + c * p.s1] : (u16)0;
+}
+
+// ---- thin product u[m, r] = alpha sum_k mask(x)[m, k] f[r, k], 32 ranks a launch row ----
+// One workgroup: 16 rows of x, its four waves a quarter of k each, so x is read once, by 16-byte loads
+// straight into the MFMA fragment (lane: row lane & 15, eight k at 8 (lane >> 4)); the quarters meet in LDS.
+struct DownArgs {
+    const u16 *x, *f;  // x [M, K] row stride ldx; f [R, K] row stride ldf, rows past r and columns past K zero
+    u16* u;            // [M, R]
+    int64_t ldx, ldf;
+    int M, K, R, vec;
+    float alpha;
+    Dropout d;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void lora_down_kernel(DownArgs a) {
+    typedef typename T::vec8 vec8;
+    __shared__ float red[3][64][9];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int li = lane & 15, g = lane >> 4;
+    const int m = blockIdx.x * 16 + li, r0 = blockIdx.y * 32;
+    const int nk = (a.K + 31) >> 5, k0 = nk * wave / 4, k1 = nk * (wave + 1) / 4;
+    const u16* xr = a.x + (int64_t)m * a.ldx;
+    const u16* f0 = a.f + (int64_t)(r0 + li) * a.ldf;
+    const u16* f1 = f0 + 16 * a.ldf;
+    const uint2 off = drop_offset(a.d);
+    f32x4 c0 = {0.f, 0.f, 0.f, 0.f}, c1 = c0;
+#pragma unroll 4
+    for (int kt = k0; kt < k1; ++kt) {
+        const int k = kt * 32 + 8 * g;
+        u16 v[8];
+        const int n = m < a.M ? min(8, a.K - k) : 0;
+        if (a.vec && n == 8) {
+            const uint4 w = *(const uint4*)(xr + k);
+            __builtin_memcpy(v, &w, 16);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = j < n ? xr[k + j] : (u16)0;
+        }
+        if (a.d.on) {
+            const uint4 p = philox4((unsigned)k >> 2, (unsigned)m, off.x, off.y, a.d.k0, a.d.k1);
+            const uint4 q = philox4(((unsigned)k >> 2) + 1, (unsigned)m, off.x, off.y, a.d.k0, a.d.k1);
+            const unsigned w[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = w[j] > a.d.drop_max ? v[j] : (u16)0;
+        }
+        vec8 xf;
+        __builtin_memcpy(&xf, v, 16);
+        const vec8 p0 = *(const vec8*)(f0 + k), p1 = *(const vec8*)(f1 + k);
+        c0 = T::mfma16(p0, xf, c0);  // lane: row m, ranks 4 g .. 4 g + 3
+        c1 = T::mfma16(p1, xf, c1);
+    }
+    if (wave) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            red[wave - 1][lane][j] = c0[j];
+            red[wave - 1][lane][4 + j] = c1[j];
+        }
+    }
+    __syncthreads();
+    if (wave || m >= a.M) return;
+    for (int w = 0; w < 3; ++w)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            c0[j] += red[w][lane][j];
+            c1[j] += red[w][lane][4 + j];
+        }
+    u16* u = a.u + (int64_t)m * a.R + r0 + 4 * g;
+    c0 *= a.alpha;
+    c1 *= a.alpha;
+    *(uint2*)u = make_uint2(pack2<T>(c0[0], c0[1]), pack2<T>(c0[2], c0[3]));
+    *(uint2*)(u + 16) = make_uint2(pack2<T>(c1[0], c1[1]), pack2<T>(c1[2], c1[3]));
+}
+
+// ---- thin gradient g[c, r] = sum_m mask(x)[m, c] u[m, r]: 128 columns x 32 ranks a workgroup, slices of rows ----
+// x passes through registers once (16-byte loads, masked, eight columns of a row a thread) into an LDS tile of
+// 32 rows, which the four waves read transposed (32 columns each) against u's 32 ranks.
+struct GradArgs {
+    const u16 *x, *u;  // x [M, C] row stride ldx, u [M, R] contiguous
+    float* part;       // [gridDim.z][R][C4]
+    int64_t ldx;
+    int M, C, C4, R, rows, vec;  // rows of a slice, a multiple of 32
+    Dropout d;
+};
+typedef unsigned u32x2f __attribute__((ext_vector_type(2)));
+template <typename T>
+__global__ __launch_bounds__(256) void lora_grad_kernel(GradArgs a) {
+    typedef typename T::vec8 vec8;
+    // rows of 128 columns (256 B) / 32 ranks (64 B), 32-B units swizzled by the row (see matmul.hip)
+    __shared__ __attribute__((aligned(16))) u16 xs[2][32 * 128], us[2][32 * 32];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int li = lane & 15, g = lane >> 4, q = li >> 2, p = li & 3;
+    const int c0 = blockIdx.x * 128, r0 = blockIdx.y * 32;
+    const int64_t ms = (int64_t)blockIdx.z * a.rows;
+    const int steps = (int)((min((int64_t)a.M - ms, (int64_t)a.rows) + 31) >> 5);
+    const uint2 off = drop_offset(a.d);
+    const int xk = threadIdx.x >> 4, xc = threadIdx.x & 15;  // this thread's rows xk, xk + 16, chunk xc
+    const int cc = c0 + xc * 8, nc = min(8, a.C - cc);
+    const int uk = threadIdx.x >> 2, uc = threadIdx.x & 3;   // threads 0 .. 127: row uk of u, chunk uc
+    u16 xv[2][8];
+    uint4 uv;
+    auto fetch = [&](int st) {
+        const int64_t mb = ms + st * 32;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int64_t m = mb + xk + 16 * h;
+            const int n = m < a.M ? nc : 0;
+            const u16* s = a.x + m * a.ldx + cc;
+            if (a.vec && n == 8) {
+                const uint4 w = *(const uint4*)s;
+                __builtin_memcpy(xv[h], &w, 16);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) xv[h][j] = j < n ? s[j] : (u16)0;
+            }
+        }
+        if (threadIdx.x < 128) {
+            const int64_t m = mb + uk;
+            uv = m < a.M ? *(const uint4*)(a.u + m * a.R + r0 + uc * 8) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    auto put = [&](int st) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int k = xk + 16 * h;
+            if (a.d.on && nc > 0) {
+                const unsigned m = (unsigned)(ms + st * 32 + k);
+                const uint4 w0 = philox4((unsigned)cc >> 2, m, off.x, off.y, a.d.k0, a.d.k1);
+                const uint4 w1 = philox4(((unsigned)cc >> 2) + 1, m, off.x, off.y, a.d.k0, a.d.k1);
+                const unsigned w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+                for (int j = 0; j < 8; ++j) xv[h][j] = w[j] > a.d.drop_max ? xv[h][j] : (u16)0;
+            }
+            const int f = (k & 3) | ((k >> 1) & 4);
+            uint4 w;
+            __builtin_memcpy(&w, xv[h], 16);
+            *(uint4*)(&xs[st & 1][k * 128 + ((xc ^ (f << 1)) << 3)]) = w;
+        }
+        if (threadIdx.x < 128) *(uint4*)(&us[st & 1][uk * 32 + uc * 8]) = uv;
+    };
+    f32x4 acc[2][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    fetch(0);
+    for (int st = 0; st < steps; ++st) {
+        put(st);
+        if (st + 1 < steps) fetch(st + 1);
+        __syncthreads();
+        vec8 xf[2], uf[2];
+        {
+            const int k = 8 * g + q, f = (k & 3) | ((k >> 1) & 4);
+            const unsigned xb = (unsigned)(size_t)(LDS_AS u16*)xs[st & 1], ub = (unsigned)(size_t)(LDS_AS u16*)us[st & 1];
+            const unsigned x0 = xb + k * 256 + (((wave * 2) ^ f) << 5) + p * 8, x1 = xb + k * 256 + (((wave * 2 + 1) ^ f) << 5) + p * 8;
+            const unsigned u0 = ub + k * 64 + p * 8;
+            u32x2f r[8];
+            asm volatile(
+                "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:1024\n\t"
+                "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:1024\n\t"
+                "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:256\n\t"
+                "ds_read_b64_tr_b16 %6, %10 offset:32\n\tds_read_b64_tr_b16 %7, %10 offset:288\n\ts_waitcnt lgkmcnt(0)"
+                : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+                : "v"(x0), "v"(x1), "v"(u0)
+                : "memory");
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                xf[i] = __builtin_bit_cast(vec8, (u32x4){r[2 * i].x, r[2 * i].y, r[2 * i + 1].x, r[2 * i + 1].y});
+                uf[i] = __builtin_bit_cast(vec8, (u32x4){r[4 + 2 * i].x, r[4 + 2 * i].y, r[5 + 2 * i].x, r[5 + 2 * i].y});
+            }
+        }
+        // lane: rank r0 + 16 i + li, columns 16 j + 4 g .. + 3 of the wave's 32
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) acc[i][j] = T::mfma16(xf[j], uf[i], acc[i][j]);
+        // two LDS buffers: the next put writes the other one, and a wave passes the next barrier only
+        // after its reads above
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int c = c0 + wave * 32 + 16 * j + 4 * g;
+            if (c < a.C4) *(f32x4*)(a.part + ((int64_t)blockIdx.z * a.R + r0 + 16 * i + li) * a.C4 + c) = acc[i][j];
+        }
+}
+// the slices' sums in order; out[c, r] (or [r, c]) by strides, r < rank
+template <typename T>
+__global__ __launch_bounds__(256) void lora_grad_join_kernel(const float* __restrict__ part, int slices, int R, int C, int C4, int rank,
+                                                             u16* out, int64_t so_c, int64_t so_r) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int r = (int)(i / C), c = (int)(i - (int64_t)r * C);
+    if (r >= rank) return;
+    float s = 0.f;
+    for (int z = 0; z < slices; ++z) s += part[((int64_t)z * R + r) * C4 + c];
+    out[c * so_c + r * so_r] = T::from_f32(s);
+}
+
+// ---- host side ----
+#define FT_FAIL(code, msg) \
+    do {                   \
+        g_err = (msg);     \
+        return (code);     \
+    } while (0)
+#define FT_LAUNCHED()                                                                            \
+    do {                                                                                         \
+        const hipError_t e_ = hipGetLastError();                                                 \
+        if (e_ != hipSuccess) FT_FAIL(CLIPVIT_E_HIP, std::string("launch: ") + hipGetErrorString(e_)); \
+    } while (0)
+
+bool is16(int dtype) { return dtype == CLIPVIT_BF16 || dtype == CLIPVIT_F16; }
+bool aligned16(const void* p) { return ((size_t)p & 15) == 0; }
+int64_t up(int64_t v, int64_t q) { return (v + q - 1) / q * q; }
+constexpr int64_t MAX_DIM = 1 << 30;
+
+bool bad_dropout(const clipvit_dropout_args& d) { return !(d.p >= 0.0 && d.p <= 1.0); }
+Dropout make_dropout(const clipvit_dropout_args& d) {
+    Dropout r{};
+    const double t = std::floor(d.p * 4294967296.0 + 0.5);
+    r.on = t >= 1.0;
+    if (!r.on) return r;
+    r.k0 = (unsigned)d.seed;
+    r.k1 = (unsigned)(d.seed >> 32);
+    r.o0 = (unsigned)d.offset;
+    r.o1 = (unsigned)(d.offset >> 32);
+    r.offset_dev = (const uint2*)d.offset_dev;
+    r.drop_max = (unsigned)(t - 1.0);
+    r.scale = d.p < 1.0 ? (float)(1.0 / (1.0 - d.p)) : 0.f;
+    return r;
+}
+
+// a [rows, cols] view with one unit stride -> (contiguous along columns?, row stride); false: refused
+bool panel_of(const int64_t (&st)[2], int64_t rows, int64_t cols, int& contig, int64_t& ld) {
+    if (st[1] == 1 || cols == 1) {
+        contig = 1;
+        ld = rows <= 1 ? up(cols, 8) : st[0];
+        if (cols == 1 && rows > 1 && st[0] == 1) {  // one column of consecutive elements
+            contig = 0;
+            ld = up(rows, 8);
+            return true;
+        }
+        return rows <= 1 || (ld >= cols && ld < MATMUL_MAX_LD);
+    }
+    if (st[0] == 1 || rows == 1) {
+        contig = 0;
+        ld = cols <= 1 ? up(rows, 8) : st[1];
+        return ld >= rows && ld < MATMUL_MAX_LD;
+    }
+    return false;
+}
+
+int matmul_of(const clipvit_linear_args* a, Matmul& m) {
+    if (!a) FT_FAIL(CLIPVIT_E_INVALID, "null arguments");
+    if (!is16(a->dtype)) FT_FAIL(CLIPVIT_E_INVALID, "linear: dtype must be BF16 or F16");
+    if (a->activation < 0 || a->activation > ACT_RELU) FT_FAIL(CLIPVIT_E_INVALID, "linear: unknown activation");
+    if (a->bias_dtype != CLIPVIT_F32 && a->bias_dtype != a->dtype) FT_FAIL(CLIPVIT_E_INVALID, "linear: bias must be F32 or of the operands' type");
+    if (a->M < 0 || a->N < 0 || a->K < 0 || a->R < 0 || a->M > MAX_DIM || a->N > MAX_DIM || a->K > MAX_DIM)
+        FT_FAIL(CLIPVIT_E_INVALID, "linear: M, N and K must lie in [0, 2^30]");
+    if (a->M && a->N) {
+        if (!a->y || (a->K && (!a->x || !a->w))) FT_FAIL(CLIPVIT_E_INVALID, "linear: null operand");
+        if (a->y_stride < a->N && a->M > 1) FT_FAIL(CLIPVIT_E_INVALID, "linear: y rows overlap");
+        if (a->residual && a->residual_stride < 0) FT_FAIL(CLIPVIT_E_INVALID, "linear: residual stride");
+        if (a->K && (!panel_of(a->x_stride, a->M, a->K, m.a_k, m.lda) || !panel_of(a->w_stride, a->N, a->K, m.b_k, m.ldb)))
+            FT_FAIL(CLIPVIT_E_INVALID, "linear: x and w need one unit stride, rows that do not overlap and a stride below 2^22");
+        if (a->R && (a->R % 32 || !a->low_u || !a->low_v || !aligned16(a->low_u) || !aligned16(a->low_v)))
+            FT_FAIL(CLIPVIT_E_INVALID, "linear: the low-rank factors need 16-byte aligned rows padded to a multiple of 32");
+    }
+    if (bad_dropout(a->dropout)) FT_FAIL(CLIPVIT_E_INVALID, "dropout: p must lie in [0, 1]");
+    if (a->low_mask && (a->activation || a->bias)) FT_FAIL(CLIPVIT_E_INVALID, "linear: a masked low-rank term takes no bias or activation");
+    m.A = (const u16*)a->x;
+    m.B = (const u16*)a->w;
+    m.M = (int)a->M;
+    m.N = (int)a->N;
+    m.K = (int)a->K;
+    Epilogue& e = m.e;
+    e.y = a->y;
+    e.bias = a->bias;
+    e.res = a->residual;
+    e.slope = a->activation ? a->slope : nullptr;
+    e.ldy = a->M > 1 ? a->y_stride : up(a->N, 8);
+    e.ldr = a->M > 1 ? a->residual_stride : up(a->N, 8);
+    e.M = m.M;
+    e.N = m.N;
+    e.bias_f32 = a->bias_dtype == CLIPVIT_F32;
+    e.act = a->activation;
+    e.drop = make_dropout(a->dropout);
+    e.lu = (const u16*)a->low_u;
+    e.lv = (const u16*)a->low_v;
+    e.R = (int)a->R;
+    e.low_mask = a->low_mask && e.drop.on;
+    if (a->low_mask && !e.drop.on) e.low_mask = 0;
+    return CLIPVIT_OK;
+}
+
+int dz_blocks(int64_t M) { return (int)((M + 63) / 64 < 512 ? (M + 63) / 64 : 512); }
+int64_t dz_rows(int64_t M) { return up((M + dz_blocks(M) - 1) / (dz_blocks(M) ? dz_blocks(M) : 1), 8); }
+
+int grad_slices(int64_t M, int64_t C, int64_t R) {
+    const int64_t wg = ((C + 127) / 128) * (R / 32);
+    int64_t s = (1024 + wg - 1) / wg;
+    const int64_t most = (M + 127) / 128;  // at least four 32-row steps a slice
+    if (s > most) s = most;
+    return (int)(s < 1 ? 1 : s);
+}
+
+template <typename F>
+int guarded(F&& f) noexcept {
+    try {
+        g_err.clear();
+        return f();
+    } catch (...) {
+        try {
+            g_err = "host allocation failed";
+        } catch (...) {
+        }
+        return CLIPVIT_E_NOMEM;
+    }
+}
+
+}  // namespace
+}  // namespace clipvit
+
+using namespace clipvit;
+
+extern "C" {
+
+int clipvit_linear_workspace(const clipvit_linear_args* a, size_t* bytes) {
+    return guarded([&]() -> int {
+        Matmul m{};
+        if (!bytes) FT_FAIL(CLIPVIT_E_INVALID, "null argument");
+        const int rc = matmul_of(a, m);
+        if (rc) return rc;
+        *bytes = matmul_workspace(m);
+        return CLIPVIT_OK;
+    });
+}
+
+int clipvit_linear(void* stream, const clipvit_linear_args* a, void* workspace, size_t bytes) {
+    return guarded([&]() -> int {
+        Matmul m{};
+        const int rc = matmul_of(a, m);
+        if (rc) return rc;
+        if (matmul_workspace(m) > bytes || (bytes && !workspace) || ((size_t)workspace & 255))
+            FT_FAIL(CLIPVIT_E_INVALID, "linear: workspace too small or not 256-byte aligned (clipvit_linear_workspace)");
+        if (!m.M || !m.N) return CLIPVIT_OK;
+        if (launch_matmul((hipStream_t)stream, a->dtype, m, workspace, bytes)) FT_FAIL(CLIPVIT_E_INVALID, "linear: workspace");
+        FT_LAUNCHED();
+        return CLIPVIT_OK;
+    });
+}
+
+int clipvit_linear_dz(void* stream, const clipvit_dz_args* a, void* workspace, size_t bytes) {
+    return guarded([&]() -> int {
+        if (!a) FT_FAIL(CLIPVIT_E_INVALID, "null arguments");
+        if (!is16(a->dtype)) FT_FAIL(CLIPVIT_E_INVALID, "linear_dz: dtype must be BF16 or F16");
+        if (a->db_dtype != CLIPVIT_F32 && a->db_dtype != a->dtype) FT_FAIL(CLIPVIT_E_INVALID, "linear_dz: db must be F32 or of dy's type");
+        if (a->M < 0 || a->N < 0 || a->M > MAX_DIM || a->N > MAX_DIM) FT_FAIL(CLIPVIT_E_INVALID, "linear_dz: M and N must lie in [0, 2^30]");
+        if (bad_dropout(a->dropout)) FT_FAIL(CLIPVIT_E_INVALID, "dropout: p must lie in [0, 1]");
+        if (a->N == 0) return CLIPVIT_OK;
+        if (a->M && !a->dy) FT_FAIL(CLIPVIT_E_INVALID, "linear_dz: null dy");
+        if (a->M > 1 && (a->dy_stride < 0 || (a->dz && a->dz_stride < a->N))) FT_FAIL(CLIPVIT_E_INVALID, "linear_dz: row stride");
+        const int blocks = dz_blocks(a->M);
+        const size_t need = a->db ? (size_t)blocks * a->N * 4 : 0;
+        if (bytes < need || (need && !workspace) || ((size_t)workspace & 15))
+            FT_FAIL(CLIPVIT_E_INVALID, "linear_dz: workspace of 4 N ceil(M / 64) bytes (at most 512 blocks), 16-byte aligned");
+        DzArgs d{};
+        d.dy = a->dy;
+        d.slope = a->slope;
+        d.dz = a->dz;
+        d.part = a->db ? (float*)workspace : nullptr;
+        d.lddy = a->M > 1 ? a->dy_stride : up(a->N, 8);
+        d.lddz = a->M > 1 ? a->dz_stride : up(a->N, 8);
+        d.M = (int)a->M;
+        d.N = (int)a->N;
+        d.rows = (int)dz_rows(a->M);
+        d.d = make_dropout(a->dropout);
+        d.vec = aligned16(d.dy) && d.lddy % 8 == 0 && aligned16(d.dz) && d.lddz % 8 == 0 && aligned16(d.slope) && (!d.slope || d.N % 8 == 0);
+        if (!d.dz) d.vec = aligned16(d.dy) && d.lddy % 8 == 0 && aligned16(d.slope) && (!d.slope || d.N % 8 == 0);
+        hipStream_t s = (hipStream_t)stream;
+        const bool bf = a->dtype == CLIPVIT_BF16;
+        if (blocks) {
+            const dim3 grid((d.N + 255) / 256, blocks);
+            if (bf) dz_kernel<BF16T><<<grid, 256, 0, s>>>(d);
+            else dz_kernel<F16T><<<grid, 256, 0, s>>>(d);
+        }
+        if (a->db) {
+            const int g = (d.N + 31) / 32;
+            if (bf) db_kernel<BF16T><<<g, 256, 0, s>>>(d.part, blocks, d.N, a->db, a->db_dtype == CLIPVIT_F32);
+            else db_kernel<F16T><<<g, 256, 0, s>>>(d.part, blocks, d.N, a->db, a->db_dtype == CLIPVIT_F32);
+        }
+        FT_LAUNCHED();
+        return CLIPVIT_OK;
+    });
+}
+
+int clipvit_dropout(void* stream, int dtype, const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, void* y,
+                    int64_t y_stride, int64_t rows, int64_t cols, const clipvit_dropout_args* dropout) {
+    return guarded([&]() -> int {
+        if (!dropout) FT_FAIL(CLIPVIT_E_INVALID, "null arguments");
+        if (dtype != CLIPVIT_F32 && !is16(dtype)) FT_FAIL(CLIPVIT_E_INVALID, "dropout: dtype must be F32, BF16 or F16");
+        if (bad_dropout(*dropout)) FT_FAIL(CLIPVIT_E_INVALID, "dropout: p must lie in [0, 1]");
+        if (rows < 0 || cols < 0 || rows > MAX_DIM || cols > MAX_DIM) FT_FAIL(CLIPVIT_E_INVALID, "dropout: rows and columns must lie in [0, 2^30]");
+        if (!rows || !cols) return CLIPVIT_OK;
+        if (!x || !y) FT_FAIL(CLIPVIT_E_INVALID, "dropout: null argument");
+        if (rows > 1 && (x_stride < 0 || residual_stride < 0 || y_stride < cols)) FT_FAIL(CLIPVIT_E_INVALID, "dropout: row stride");
+        DropArgs d{};
+        d.x = x;
+        d.res = residual;
+        d.y = y;
+        d.ldx = rows > 1 ? x_stride : 0;
+        d.ldr = rows > 1 ? residual_stride : 0;
+        d.ldy = rows > 1 ? y_stride : 0;
+        d.rows = (int)rows;
+        d.cols = (int)cols;
+        d.d = make_dropout(*dropout);
+        const int per = dtype == CLIPVIT_F32 ? 4 : 8;
+        d.vec = aligned16(x) && aligned16(y) && aligned16(residual) && d.ldx % per == 0 && d.ldy % per == 0 && (!residual || d.ldr % per == 0);
+        // thread groups of 8 columns: the widest row of threads that leaves at most an eighth of them idle
+        const int groups = (int)((cols + 7) / 8);
+        d.tx = 64;
+        while (d.tx > 1 && ((groups + d.tx - 1) / d.tx) * (int64_t)d.tx * 8 > (int64_t)groups * 9) d.tx >>= 1;
+        const int ny = 256 / d.tx, gx = (groups + d.tx - 1) / d.tx;
+        int64_t gy = (rows + ny - 1) / ny;
+        const int64_t cap = (16384 + gx - 1) / gx;
+        if (gy > cap) gy = cap;
+        if (gy > 65535) gy = 65535;
+        const dim3 grid(gx, (unsigned)gy);
+        hipStream_t s = (hipStream_t)stream;
+        if (dtype == CLIPVIT_F32) dropout_kernel<F32T><<<grid, 256, 0, s>>>(d);
+        else if (dtype == CLIPVIT_BF16) dropout_kernel<BF16T><<<grid, 256, 0, s>>>(d);
+        else dropout_kernel<F16T><<<grid, 256, 0, s>>>(d);
+        FT_LAUNCHED();
+        return CLIPVIT_OK;
+    });
+}
+
+int clipvit_lora_pad(void* stream, const clipvit_pad_args* a, const clipvit_pad_args* b) {
+    return guarded([&]() -> int {
+        PadArgs p[2]{};
+        unsigned blocks[2] = {0, 0};
+        const clipvit_pad_args* in[2] = {a, b};
+        for (int i = 0; i < 2; ++i) {
+            const clipvit_pad_args* q = in[i];
+            if (!q) continue;
+            if (q->rows < 0 || q->cols < 0 || q->rows_padded < q->rows || q->cols_padded < q->cols || q->rows_padded > MAX_DIM ||
+                q->cols_padded > MAX_DIM)
+                FT_FAIL(CLIPVIT_E_INVALID, "lora_pad: sizes");
+            const int64_t n = q->rows_padded * q->cols_padded;
+            if (!n) continue;
+            if (n > (int64_t)1 << 38) FT_FAIL(CLIPVIT_E_INVALID, "lora_pad: sizes");
+            if ((!q->src && q->rows && q->cols) || !q->dst) FT_FAIL(CLIPVIT_E_INVALID, "lora_pad: null argument");
+            p[i] = PadArgs{(const u16*)q->src, q->row_stride, q->col_stride, (int)q->rows, (int)q->cols, (int)q->rows_padded,
+                           (int)q->cols_padded, (u16*)q->dst};
+            blocks[i] = (unsigned)((n + 255) / 256);
+        }
+        if (blocks[0] + blocks[1] == 0) return CLIPVIT_OK;
+        pad_kernel<<<blocks[0] + blocks[1], 256, 0, (hipStream_t)stream>>>(p[0], p[1], (int)blocks[0]);
+        FT_LAUNCHED();
+        return CLIPVIT_OK;
+    });
+}
+
+int clipvit_lora_down(void* stream, int dtype, const void* x, int64_t x_stride, const void* f, int64_t f_stride, void* u, int64_t M, int64_t K,
+                      int64_t R, float alpha, const clipvit_dropout_args* dropout) {
+    return guarded([&]() -> int {
+        if (!dropout || bad_dropout(*dropout)) FT_FAIL(CLIPVIT_E_INVALID, "dropout: p must lie in [0, 1]");
+        if (!is16(dtype)) FT_FAIL(CLIPVIT_E_INVALID, "lora_down: dtype must be BF16 or F16");
+        if (M < 0 || K < 0 || R < 0 || R % 32 || M > MAX_DIM || K > MAX_DIM || R > 65536) FT_FAIL(CLIPVIT_E_INVALID, "lora_down: sizes");
+        if (!M || !R) return CLIPVIT_OK;
+        if (!u || (K && (!x || !f))) FT_FAIL(CLIPVIT_E_INVALID, "lora_down: null argument");
+        if (!aligned16(f) || f_stride % 8 || f_stride < up(K, 32) || !aligned16(u)) FT_FAIL(CLIPVIT_E_INVALID, "lora_down: factor rows must be 16-byte aligned, zero padded to 32");
+        if (M > 1 && x_stride < 0) FT_FAIL(CLIPVIT_E_INVALID, "lora_down: row stride");
+        DownArgs d{};
+        d.x = (const u16*)x;
+        d.f = (const u16*)f;
+        d.u = (u16*)u;
+        d.ldx = M > 1 ? x_stride : 0;
+        d.ldf = f_stride;
+        d.M = (int)M;
+        d.K = (int)K;
+        d.R = (int)R;
+        d.vec = aligned16(x) && d.ldx % 8 == 0;
+        d.alpha = alpha;
+        d.d = make_dropout(*dropout);
+        const dim3 grid((unsigned)((M + 15) / 16), (unsigned)(R / 32));
+        if (dtype == CLIPVIT_BF16) lora_down_kernel<BF16><<<grid, 256, 0, (hipStream_t)stream>>>(d);
+        else lora_down_kernel<F16><<<grid, 256, 0, (hipStream_t)stream>>>(d);
+        FT_LAUNCHED();
+        return CLIPVIT_OK;
+    });
+}
+
+int clipvit_lora_grad_workspace(int64_t M, int64_t C, int64_t R, size_t* bytes) {
+    return guarded([&]() -> int {
+        if (!bytes || M < 0 || C < 0 || R < 0 || R % 32 || M > MAX_DIM || C > MAX_DIM || R > 65536) FT_FAIL(CLIPVIT_E_INVALID, "lora_grad: sizes");
+        *bytes = C && R ? (size_t)grad_slices(M, C, R) * (size_t)R * (size_t)up(C, 4) * 4 : 0;
+        return CLIPVIT_OK;
+    });
+}
+
+int clipvit_lora_grad(void* stream, int dtype, const void* x, int64_t x_stride, const void* u, void* out, int64_t out_col_stride,
+                      int64_t out_rank_stride, int64_t M, int64_t C, int64_t R, int64_t rank, const clipvit_dropout_args* dropout, void* workspace,
+                      size_t bytes) {
+    return guarded([&]() -> int {
+        if (!dropout || bad_dropout(*dropout)) FT_FAIL(CLIPVIT_E_INVALID, "dropout: p must lie in [0, 1]");
+        if (!is16(dtype)) FT_FAIL(CLIPVIT_E_INVALID, "lora_grad: dtype must be BF16 or F16");
+        size_t need = 0;
+        const int rc = clipvit_lora_grad_workspace(M, C, R, &need);
+        if (rc) return rc;
+        if (rank < 0 || rank > R) FT_FAIL(CLIPVIT_E_INVALID, "lora_grad: rank");
+        if (!C || !rank) return CLIPVIT_OK;
+        if (!out || (M && (!x || !u || !aligned16(u)))) FT_FAIL(CLIPVIT_E_INVALID, "lora_grad: null or misaligned argument");
+        if (M > 1 && x_stride < 0) FT_FAIL(CLIPVIT_E_INVALID, "lora_grad: row stride");
+        if (bytes < need || !workspace || !aligned16(workspace)) FT_FAIL(CLIPVIT_E_INVALID, "lora_grad: workspace too small or misaligned (clipvit_lora_grad_workspace)");
+        GradArgs d{};
+        d.x = (const u16*)x;
+        d.u = (const u16*)u;
+        d.part = (float*)workspace;
+        d.ldx = M > 1 ? x_stride : 0;
+        d.M = (int)M;
+        d.C = (int)C;
+        d.C4 = (int)up(C, 4);
+        d.R = (int)R;
+        d.vec = aligned16(x) && d.ldx % 8 == 0;
+        d.d = make_dropout(*dropout);
+        int slices = grad_slices(M, C, R);
+        d.rows = (int)up((M + slices - 1) / slices, 32);
+        slices = M ? (int)((M + d.rows - 1) / d.rows) : 0;
+        hipStream_t s = (hipStream_t)stream;
+        const bool bf = dtype == CLIPVIT_BF16;
+        if (slices) {
+            const dim3 grid((unsigned)((C + 127) / 128), (unsigned)(R / 32), slices);
+            if (bf) lora_grad_kernel<BF16><<<grid, 256, 0, s>>>(d);
+            else lora_grad_kernel<F16><<<grid, 256, 0, s>>>(d);
+        }
+        const unsigned g = (unsigned)((rank * C + 255) / 256);
+        if (bf) lora_grad_join_kernel<BF16><<<g, 256, 0, s>>>(d.part, slices, d.R, d.C, d.C4, (int)rank, (u16*)out, out_col_stride, out_rank_stride);
+        else lora_grad_join_kernel<F16><<<g, 256, 0, s>>>(d.part, slices, d.R, d.C, d.C4, (int)rank, (u16*)out, out_col_stride, out_rank_stride);
+        FT_LAUNCHED();
+        return CLIPVIT_OK;
+    });
+}
+
+}  // extern "C"

@@ -242,6 +242,110 @@ int clipvit_preprocess(void* stream, const unsigned char* rgb_dev, const clipvit
 int clipvit_resample_plan(int in_size, int out_size, int* ksize, int* bounds, int32_t* kk,
                           int kk_cap);
 
+/* ---- Fine-tuning operators: a Linear with its epilogue, counter-based dropout, the unmerged LoRA Linear ----
+ * The reference trains its adapters on LoRALinear modules (main.py:34-59, train_lora.py:62-100); these are
+ * that Linear's forward and gradients on 16-bit device tensors with fp32 accumulation. No handle: every
+ * call takes the stream and, where it says so, a caller-owned device workspace that no other call in
+ * flight uses. Nothing is allocated, synchronised or cleared by the runtime inside, so all of them can be
+ * captured into a graph. Pointers are device pointers; strides count elements. */
+
+/* Element (row m, column n) is kept when word n % 4 of Philox4x32-10 at counter (n / 4, m, offset) under the
+ * 64-bit key `seed` is at least round(p 2^32), and then scaled by 1 / (1 - p); a dropped element is 0 whatever
+ * it held. The mask is never stored. p = 0: no dropout; p = 1: everything is dropped. */
+typedef struct {
+    double p;
+    uint64_t seed;
+    uint64_t offset;
+    const int64_t* offset_dev; /* NULL, or the offset in device memory (read by the kernels: a replayed
+                                  graph draws the mask of the value it finds there) */
+} clipvit_dropout_args;
+
+typedef enum {
+    CLIPVIT_ACT_NONE = 0,
+    CLIPVIT_ACT_QUICK_GELU = 1, /* z s(1.702 z)                   */
+    CLIPVIT_ACT_GELU = 2,       /* z (1 + erf(z / sqrt 2)) / 2    */
+    CLIPVIT_ACT_GELU_TANH = 3,
+    CLIPVIT_ACT_SILU = 4,
+    CLIPVIT_ACT_RELU = 5,
+} clipvit_activation;
+
+/* y[m, n] = residual[m, n] + dropout(act(z))[m, n],  z = sum_k x[m, k] w[n, k] + bias[n] + sum_r u[m, r] v[n, r].
+ * x [M, K] and w [N, K] are views with two strides, one of them 1 (so a gradient's product takes the forward's
+ * tensors transposed); the other is below 2^22 and at least the row's length. y and residual have unit column
+ * stride. slope (or NULL): act'(z) as [M, N] contiguous 16-bit fixed point, q / 2^14 (-32768 = NaN), what
+ * clipvit_linear_dz takes. R > 0: the low-rank term, u [M, R] and v [N, R] contiguous, R % 32 == 0. low_mask:
+ * the dropout mask, unscaled, applies to the low-rank term instead (no bias and no activation then).
+ * Rows of any length, stride and alignment are taken; those that 16-byte loads cannot address are copied into the
+ * workspace first. y must not overlap an input other than an identical residual. */
+typedef struct {
+    int dtype;      /* CLIPVIT_BF16 or CLIPVIT_F16: x, w, residual, y, u, v */
+    int activation; /* clipvit_activation */
+    int bias_dtype; /* CLIPVIT_F32 or dtype */
+    int low_mask;
+    int64_t M, N, K, R;
+    const void* x;
+    int64_t x_stride[2];
+    const void* w;
+    int64_t w_stride[2];
+    const void* bias;     /* [N] or NULL */
+    const void* residual; /* [M, N] or NULL */
+    int64_t residual_stride;
+    void* y;
+    int64_t y_stride;
+    int16_t* slope;
+    const void* low_u;
+    const void* low_v;
+    clipvit_dropout_args dropout;
+} clipvit_linear_args;
+
+/* Bytes of workspace (256-byte aligned) that clipvit_linear needs for these arguments; may be 0. */
+int clipvit_linear_workspace(const clipvit_linear_args* args, size_t* bytes);
+int clipvit_linear(void* stream, const clipvit_linear_args* args, void* workspace, size_t bytes);
+
+/* dz[m, n] = dropout(dy)[m, n] slope[m, n] (dz, slope may be NULL) and db[n] = sum_m of the unrounded dz (or NULL),
+ * summed in a fixed order. Workspace with db: 4 N min(512, ceil(M / 64)) bytes, 16-byte aligned. */
+typedef struct {
+    int dtype;
+    int db_dtype; /* CLIPVIT_F32 or dtype */
+    int64_t M, N;
+    const void* dy;
+    int64_t dy_stride;
+    const int16_t* slope;
+    void* dz;
+    int64_t dz_stride;
+    void* db;
+    clipvit_dropout_args dropout;
+} clipvit_dz_args;
+int clipvit_linear_dz(void* stream, const clipvit_dz_args* args, void* workspace, size_t bytes);
+
+/* y = residual + dropout(x) on [rows, cols] F32, BF16 or F16 rows of unit column stride (residual may be NULL, y may
+ * be x or residual). The gradient of x is the same call on dy. */
+int clipvit_dropout(void* stream, int dtype, const void* x, int64_t x_stride, const void* residual,
+                    int64_t residual_stride, void* y, int64_t y_stride, int64_t rows, int64_t cols,
+                    const clipvit_dropout_args* dropout);
+
+/* dst[i, j] = src(i, j) for i < rows, j < cols, 0 up to [rows_padded, cols_padded] (contiguous): a 16-bit low-rank
+ * factor in the padded (and, by its strides, transposed) form the calls below and clipvit_linear take. Two
+ * factors a launch; either may be NULL. */
+typedef struct {
+    const void* src;
+    int64_t row_stride, col_stride, rows, cols, rows_padded, cols_padded;
+    void* dst;
+} clipvit_pad_args;
+int clipvit_lora_pad(void* stream, const clipvit_pad_args* a, const clipvit_pad_args* b);
+
+/* u[m, r] = alpha sum_k mask(x)[m, k] f[r, k]: the adapter's thin product. x [M, K] of row stride x_stride;
+ * f [R, >= K rounded up to 32] zero padded, R % 32 == 0; u [M, R] contiguous. The mask is unscaled. */
+int clipvit_lora_down(void* stream, int dtype, const void* x, int64_t x_stride, const void* f, int64_t f_stride,
+                      void* u, int64_t M, int64_t K, int64_t R, float alpha, const clipvit_dropout_args* dropout);
+
+/* out(c, r) = sum_m mask(x)[m, c] u[m, r] for r < rank: an adapter factor's gradient, summed in a fixed order.
+ * x [M, C], u [M, R] contiguous, out at out + c out_col_stride + r out_rank_stride. */
+int clipvit_lora_grad_workspace(int64_t M, int64_t C, int64_t R, size_t* bytes);
+int clipvit_lora_grad(void* stream, int dtype, const void* x, int64_t x_stride, const void* u, void* out,
+                      int64_t out_col_stride, int64_t out_rank_stride, int64_t M, int64_t C, int64_t R, int64_t rank,
+                      const clipvit_dropout_args* dropout, void* workspace, size_t bytes);
+
 /* ---- kernel-level entry points (testing / benchmarking of single hot kernels) ----
  * These operate on caller-owned device buffers with the packed layouts documented in
  * DESIGN.md; they are what the per-kernel parity tests and the roofline probe call. */
