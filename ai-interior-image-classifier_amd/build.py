@@ -26,10 +26,7 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # accumulators of tiles whose occupancy allows > 256 registers (the class-token tail's 2-wave
 # 64x64 tile) in AGPRs and rotated them with v_accvgpr_mov/read/write every k-step.
 CFLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", f"-I{INCLUDE}", f"-I{CSRC}",
-          "-mllvm", "--amdgpu-mfma-vgpr-form", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-          "-Wno-unused-result", "-Wno-unused-value"]
-# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32. The compiler makes them from ordinary float code, and some
-# of their forms have given wrong results on this machine.
+          "-mllvm", "--amdgpu-mfma-vgpr-form", "-Wno-unused-result", "-Wno-unused-value"]
 # Per-source flags. gemm.hip: the max-memory-clause machine scheduler (clusters each k-step's
 # staging loads). Same-box A/B of the two builds (profiles/design_r05.md §11): B/32 +0.2 / +0.6 %, B/16
 # +0.5 %, L/14@336 +0.7 / +1.0 % img/s, patch GEMM -7 %; on attention.hip it cost 6 %, so
