@@ -32,6 +32,12 @@ CFLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", f"-I{INCLUDE}"
 # +0.5 %, L/14@336 +0.7 / +1.0 % img/s, patch GEMM -7 %; on attention.hip it cost 6 %, so
 # only the GEMMs get it.
 SRC_FLAGS = {"gemm": ["-mllvm", "--amdgpu-sched-strategy=max-memory-clause"]}
+# No v_pk_{add,mul,fma}_f32: the compiler makes them from ordinary float code, and some of their forms
+# have given wrong results on this machine. norm.hip is still built with them: without, its sums contract
+# differently and the encoder's outputs change in their last bits (every other unit's output is the same bits
+# either way, on B/32, B/16 and L/14@336 in fp16, bf16 and MX-fp8 and on the text tower).
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+PACKED_F32_UNITS = {"norm"}
 # options a unit is built without (none since the r05 one-wave-per-SIMD probes left the build)
 SRC_DROP: dict[str, list[str]] = {}
 
@@ -56,6 +62,8 @@ def _compile(src: Path) -> tuple[Path, str]:
     for f in SRC_DROP.get(src.stem, []):  # a dropped -mllvm option takes its -mllvm with it
         i = flags.index(f)
         del flags[i - 1:i + 1]
+    if src.stem not in PACKED_F32_UNITS:
+        flags += NO_PACKED_F32
     cmd = [HIPCC, *flags, *SRC_FLAGS.get(src.stem, []), "-c", str(src), "-o", str(obj)]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
