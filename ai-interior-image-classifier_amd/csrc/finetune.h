@@ -113,26 +113,25 @@ struct Epilogue {
     int R, low_mask;
 };
 
-// C consecutive columns n .. n + C - 1 (n % 4 == 0) of row m: v = acc (+ an unmasked low-rank term), t = the
-// masked low-rank term (LOW) or unused. Columns at or past N are not touched.
+// the bias of C columns from n, zeros past N or without one
+template <typename T, int C>
+__device__ __forceinline__ void bias_cols(const Epilogue& e, int n, float (&b)[C]) {
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+        b[j] = 0.f;
+        if (e.bias && n + j < e.N) b[j] = e.bias_f32 ? ((const float*)e.bias)[n + j] : T::to_f32(((const u16*)e.bias)[n + j]);
+    }
+}
+
+// C consecutive columns n .. n + C - 1 (n % C == 0) of row m: v = acc (+ an unmasked low-rank term), b their
+// bias, t = the masked low-rank term (LOW) or unused. Columns at or past N are not touched.
 template <typename T, int C, bool LOW>
-__device__ __forceinline__ void epilogue_cols(const Epilogue& e, const uint2& off, int m, int n, float (&v)[C], float (&t)[C]) {
+__device__ __forceinline__ void epilogue_cols(const Epilogue& e, const uint2& off, int m, int n, float (&v)[C], const float (&b)[C], float (&t)[C]) {
     const int nc = min(C, e.N - n);
     if (m >= e.M || nc <= 0) return;
     const bool whole = nc == C && e.vec;
-    if (e.bias) {
-        if (e.bias_f32) {
-            const float* b = (const float*)e.bias + n;
 #pragma unroll
-            for (int j = 0; j < C; ++j)
-                if (j < nc) v[j] += b[j];
-        } else {
-            const u16* b = (const u16*)e.bias + n;
-#pragma unroll
-            for (int j = 0; j < C; ++j)
-                if (j < nc) v[j] += T::to_f32(b[j]);
-        }
-    }
+    for (int j = 0; j < C; ++j) v[j] += b[j];
     if constexpr (LOW) {
 #pragma unroll
         for (int j = 0; j < C; j += 4) drop4(e.drop, off, m, n + j, 1.0f, t[j], t[j + 1], t[j + 2], t[j + 3]);

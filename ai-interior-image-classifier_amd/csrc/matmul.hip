@@ -3,21 +3,22 @@
 // its own index (a "column panel"): a Linear's forward is (k, k), its input gradient (k, column) and its
 // weight gradient (column, column), all on the tensors as the user's program holds them.
 //
-// Tile: WM x WN waves, each FM 16-row fragments x 64 columns, in 32-deep k-steps through a ring of four LDS
-// stages filled by buffer loads straight to LDS. The MFMA runs with swapped operands (B rows as its A), so
-// a lane holds consecutive columns of one row.
+// Every k-tile is 64 deep, so that a row panel's loads are whole 128-byte lines: at 64 bytes a row the products
+// of two row panels ran at 873 TFLOP/s where two column panels reached 1213 (8192^3, bf16; the delivered rate is
+// requests in flight times their size). Loads go from global memory straight to LDS (buffer_load ... lds). The
+// MFMA runs with swapped operands (B rows as its A), so a lane holds four consecutive columns of one row.
 //
-// LDS image of a stage: A then B.
-//  * row panel (R rows x 32 k, 64 B a row): 16-B chunk c of row r at chunk c ^ ((r >> 2) & 2); fragments by
-//    ds_read_b128. B's rows are staged permuted inside each group of 64 (LDS row 16 f + i holds column
-//    16 (i >> 2) + 4 f + (i & 3)), which leaves 16 consecutive columns in a lane.
-//  * column panel (32 k x R columns, 2 R bytes a k): fragments by ds_read_b64_tr_b16 (lane 4 q + p of a
-//    16-lane group supplies k row q, columns 4 p .. 4 p + 3; lane i receives column i of the four k). The
-//    32-B unit of a row is XORed with f(k), which makes the eight k rows that a half wave reads distinct in
-//    their banks. B's columns stay in order; four lane groups exchange their fragments in the epilogue
-//    (permlane32_swap, permlane16_swap) for the same 16 consecutive columns.
+// LDS image:
+//  * row panel (R rows x 64 k, 128 B a row): 16-B chunk c of row r at chunk c ^ (r & 7); fragments by ds_read_b128;
+//  * column panel (64 k x R columns, 2 R bytes a k): fragments by ds_read_b64_tr_b16 (lane 4 q + p of a 16-lane
+//    group supplies k row q, columns 4 p .. 4 p + 3; lane i receives column i of the four k). The 32-B unit of a
+//    row is XORed with a function of k that sends the eight k rows that a half wave reads to distinct banks.
 // Ragged edges: rows past the matrix and k past K lie outside the buffer resource (or get an offset that
 // does) and read as zeros.
+//
+// Epilogue: each wave passes its accumulators, 16 rows x 64 columns at a time, through 4 KB of LDS of its own
+// (chunks XORed with the row: no conflicts), and continues with eight consecutive columns a lane: 128 contiguous
+// bytes a row for the 16-bit residual, slope and output, whole groups of four for the dropout counter.
 #include <type_traits>
 
 #include "finetune.h"
@@ -27,10 +28,6 @@ namespace {
 
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 constexpr unsigned OOB = 0xFFFFFFF0u;
-constexpr int NS = 4;  // LDS stages
-
-template <int N>
-using ic = std::integral_constant<int, N>;
 
 // k-row swizzle of a column panel in 32-B units: R >= 128 columns (rows of at least 256 B) need 8 distinct
 // units, 64 columns (two rows per 256 B) 4
@@ -39,147 +36,345 @@ __device__ __forceinline__ int col_swz(int k) {
     return R >= 128 ? (k & 3) | ((k >> 1) & 4) : ((k >> 1) & 1) | ((k >> 2) & 2);
 }
 
-// One operand's panel of a tile: staging offsets and the per-step resource.
-// R rows (row panel) or columns (column panel) from index i0 of `count`; NW waves share its R / 16 pieces of 1 KB.
-template <bool KC, int R, int NW, bool PERM>
+// Position in a panel's LDS image -> row (column) of the tile. Whole: the panel is the tile's operand. Half<H>: the
+// 64-row halves H of both 128-row wave groups.
+struct Whole {
+    static __device__ __forceinline__ int at(int i) { return i; }
+};
+template <int H>
+struct Half {
+    static __device__ __forceinline__ int at(int i) { return ((i & 64) << 1) + 64 * H + (i & 63); }
+};
+
+// One operand's panel of a tile: R rows (KC) or columns, staged by NW waves, NP pieces of 1 KB each.
+template <bool KC, int R, int NW, class Map>
 struct Panel {
-    static constexpr int NP = R / 16 / NW;
+    static constexpr int NP = R / 8 / NW, BYTES = R * 128;
     const unsigned char* base;
-    unsigned long long kstep;  // column panel: bytes of 32 k rows
+    unsigned long long kstep;  // column panel: bytes of 64 k rows
     unsigned range;            // row panel: bytes; column panel: bytes of its last valid row from the first column
     unsigned ld2;
     int K, chunk;
     unsigned voff[NP];
 
+    // the operand's rows (columns) i0 .. of `count`; this wave is number w of NW
     __device__ __forceinline__ void init(const u16* p, int64_t ld, int i0, int count, int K_, int w, int lane) {
-        const int valid = min(R, count - i0);
+        const int valid = min(count - i0, 1 << 12);
         K = K_;
         ld2 = (unsigned)(ld * 2);
         if constexpr (KC) {
             base = (const unsigned char*)(p + (int64_t)i0 * ld);
-            range = (unsigned)(valid - 1) * ld2 + (unsigned)((K + 7) & ~7) * 2;  // (rows are padded to 8 elements)
+            range = (unsigned)(min(valid, 256) - 1) * ld2 + (unsigned)((K + 7) & ~7) * 2;  // (rows are padded to 8 elements)
             kstep = 0;
-            const int r = lane >> 2;
-            chunk = (lane & 3) ^ ((r >> 2) & 2);
+            const int r = lane >> 3;
+            chunk = (lane & 7) ^ r;
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
-                int row = (w * NP + i) * 16 + r;  // LDS row
-                if constexpr (PERM) row = (row & ~63) + 16 * ((row & 15) >> 2) + 4 * ((row >> 4) & 3) + (row & 3);
+                const int row = Map::at((w * NP + i) * 8 + r);
                 voff[i] = row < valid ? (unsigned)row * ld2 + chunk * 16 : OOB;
             }
         } else {
             base = (const unsigned char*)(p + i0);
-            range = (unsigned)((valid + 7) & ~7) * 2;
-            kstep = (unsigned long long)ld2 * 32;
+            range = (unsigned)((min(valid, 256) + 7) & ~7) * 2;
+            kstep = (unsigned long long)ld2 * 64;
             chunk = 0;
             constexpr int CPR = R / 8;  // 16-B chunks per k row
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
                 const int idx = (w * NP + i) * 64 + lane;
-                const int k = idx / CPR, c = (idx % CPR) ^ (col_swz<R>(k) << 1);
-                voff[i] = c * 8 < valid ? (unsigned)k * ld2 + c * 16 : OOB;
+                const int k = idx / CPR, c = Map::at(((idx % CPR) ^ (col_swz<R>(k) << 1)) * 8);
+                voff[i] = c < valid ? (unsigned)k * ld2 + c * 2 : OOB;
             }
         }
     }
-    // stage k-step kt (32 deep) into dst (this operand's part of a stage, the wave's first piece)
+    // stage k-tile kt into dst (the panel's part of a stage)
     __device__ __forceinline__ void stage(int kt, int w, unsigned char* dst) const {
-        const int left = K - kt * 32;
+        const int left = K - kt * 64;
         unsigned char* d = dst + w * NP * 1024;
         if constexpr (KC) {
             const i32x4_t rs = buf_rsrc(base, left > 0 ? range : 0u);
             const bool in = chunk * 8 < left;
 #pragma unroll
-            for (int i = 0; i < NP; ++i) blds16(rs, in ? voff[i] : OOB, left > 0 ? kt * 64 : 0, d + i * 1024);
+            for (int i = 0; i < NP; ++i) blds16(rs, in ? voff[i] : OOB, left > 0 ? kt * 128 : 0, d + i * 1024);
         } else {
             const i32x4_t rs = buf_rsrc(base + (left > 0 ? kstep * (unsigned)kt : 0ull),
-                                        left > 0 ? (unsigned)(min(left, 32) - 1) * ld2 + range : 0u);
+                                        left > 0 ? (unsigned)(min(left, 64) - 1) * ld2 + range : 0u);
 #pragma unroll
             for (int i = 0; i < NP; ++i) blds16(rs, voff[i], 0, d + i * 1024);
         }
     }
 };
 
-template <typename T>
-__device__ __forceinline__ typename T::vec8 vec_of(const u32x2& a, const u32x2& b) {
-    return __builtin_bit_cast(typename T::vec8, (u32x4){a.x, a.y, b.x, b.y});
+// Fragment reads of FR (1 or 4) 16-row fragments x 64 k from position i0 of a panel. Each asm block ends with its own
+// wait (hipcc does not see these reads, and a plain LDS read would make it drain the LDS-DMA loads in flight).
+template <typename T, bool KC, int R, int FR>
+struct Frags {
+    typedef typename T::vec8 vec8;
+    unsigned addr[KC ? 2 : FR];  // row panel: k halves 0, 1; column panel: one per fragment
+    __device__ __forceinline__ void init(unsigned lds, int i0, int lane) {
+        const int li = lane & 15, g = lane >> 4;
+        if constexpr (KC) {
+            addr[0] = lds + (i0 + li) * 128 + ((g ^ (li & 7)) << 4);
+            addr[1] = lds + (i0 + li) * 128 + (((4 + g) ^ (li & 7)) << 4);
+        } else {
+            const int k = 8 * g + (li >> 2), f = col_swz<R>(k);
+#pragma unroll
+            for (int i = 0; i < FR; ++i) addr[i] = lds + k * (R * 2) + (((i0 / 16 + i) ^ f) << 5) + (li & 3) * 8;
+        }
+    }
+    __device__ __forceinline__ void read(vec8 (&d)[2][FR], unsigned so) const {
+        if constexpr (KC && FR == 4) {
+            asm volatile(
+                "ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:2048\n\tds_read_b128 %2, %8 offset:4096\n\t"
+                "ds_read_b128 %3, %8 offset:6144\n\tds_read_b128 %4, %9\n\tds_read_b128 %5, %9 offset:2048\n\t"
+                "ds_read_b128 %6, %9 offset:4096\n\tds_read_b128 %7, %9 offset:6144\n\ts_waitcnt lgkmcnt(0)"
+                : "=&v"(d[0][0]), "=&v"(d[0][1]), "=&v"(d[0][2]), "=&v"(d[0][3]), "=&v"(d[1][0]), "=&v"(d[1][1]),
+                  "=&v"(d[1][2]), "=&v"(d[1][3])
+                : "v"(addr[0] + so), "v"(addr[1] + so)
+                : "memory");
+        } else if constexpr (KC) {
+            asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %3\n\ts_waitcnt lgkmcnt(0)"
+                         : "=&v"(d[0][0]), "=&v"(d[1][0])
+                         : "v"(addr[0] + so), "v"(addr[1] + so)
+                         : "memory");
+        } else if constexpr (FR == 4) {
+            u32x2 r[16];
+            asm volatile(
+                "ds_read_b64_tr_b16 %0, %16\n\tds_read_b64_tr_b16 %1, %16 offset:%20\n\t"
+                "ds_read_b64_tr_b16 %2, %17\n\tds_read_b64_tr_b16 %3, %17 offset:%20\n\t"
+                "ds_read_b64_tr_b16 %4, %18\n\tds_read_b64_tr_b16 %5, %18 offset:%20\n\t"
+                "ds_read_b64_tr_b16 %6, %19\n\tds_read_b64_tr_b16 %7, %19 offset:%20\n\t"
+                "ds_read_b64_tr_b16 %8, %16 offset:%21\n\tds_read_b64_tr_b16 %9, %16 offset:%22\n\t"
+                "ds_read_b64_tr_b16 %10, %17 offset:%21\n\tds_read_b64_tr_b16 %11, %17 offset:%22\n\t"
+                "ds_read_b64_tr_b16 %12, %18 offset:%21\n\tds_read_b64_tr_b16 %13, %18 offset:%22\n\t"
+                "ds_read_b64_tr_b16 %14, %19 offset:%21\n\tds_read_b64_tr_b16 %15, %19 offset:%22\n\ts_waitcnt lgkmcnt(0)"
+                : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7]),
+                  "=&v"(r[8]), "=&v"(r[9]), "=&v"(r[10]), "=&v"(r[11]), "=&v"(r[12]), "=&v"(r[13]), "=&v"(r[14]), "=&v"(r[15])
+                : "v"(addr[0] + so), "v"(addr[1] + so), "v"(addr[2] + so), "v"(addr[3] + so), "i"(R * 8), "i"(R * 64), "i"(R * 72)
+                : "memory");
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                d[i >> 2][i & 3] = __builtin_bit_cast(vec8, (u32x4){r[2 * i].x, r[2 * i].y, r[2 * i + 1].x, r[2 * i + 1].y});
+        } else {
+            u32x2 r[4];
+            asm volatile(
+                "ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:%5\n\t"
+                "ds_read_b64_tr_b16 %2, %4 offset:%6\n\tds_read_b64_tr_b16 %3, %4 offset:%7\n\ts_waitcnt lgkmcnt(0)"
+                : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
+                : "v"(addr[0] + so), "i"(R * 8), "i"(R * 64), "i"(R * 72)
+                : "memory");
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                d[i][0] = __builtin_bit_cast(vec8, (u32x4){r[2 * i].x, r[2 * i].y, r[2 * i + 1].x, r[2 * i + 1].y});
+        }
+    }
+};
+
+__device__ __forceinline__ void bar() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
 }
 
-// Fragment reads: four fragments per asm block, which ends with its own wait (hipcc does not see these
-// reads, and a plain LDS read would make it drain the LDS-DMA loads in flight).
-template <typename T>
-__device__ __forceinline__ void read_rows4(typename T::vec8 (&d)[4], unsigned a) {
-    asm volatile(
-        "ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:1024\n\tds_read_b128 %2, %4 offset:2048\n\t"
-        "ds_read_b128 %3, %4 offset:3072\n\ts_waitcnt lgkmcnt(0)"
-        : "=&v"(d[0]), "=&v"(d[1]), "=&v"(d[2]), "=&v"(d[3])
-        : "v"(a)
-        : "memory");
-}
-template <typename T>
-__device__ __forceinline__ void read_rows1(typename T::vec8& d, unsigned a) {
-    asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(d) : "v"(a) : "memory");
-}
-// HS = bytes of four k rows
-template <typename T, int HS>
-__device__ __forceinline__ void read_cols4(typename T::vec8 (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3) {
-    u32x2 r[8];
-    asm volatile(
-        "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\t"
-        "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
-        "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
-        "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\ts_waitcnt lgkmcnt(0)"
-        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
-        : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "i"(HS)
-        : "memory");
+// acc[i][j]: rows mw + 16 i .., columns nw + 16 j .. of C, in the MFMA's layout (lane: row lane & 15, columns
+// 4 (lane >> 4) .. + 3). eb: this wave's 4 KB of LDS. part != null: the slice's fp32 sums, row stride N4.
+template <typename T, int FM>
+__device__ __forceinline__ void store_tile(const Matmul& a, f32x4 (&acc)[FM][4], int mw, int nw, float* eb, float* part, int N4, int lane) {
+    typedef typename T::vec8 vec8;
+    const Epilogue& e = a.e;
+    const int li = lane & 15, g = lane >> 4, er = lane >> 3, ec = lane & 7;
+    const int n = nw + 8 * ec;
+    const uint2 off = e.drop.on ? drop_offset(e.drop) : make_uint2(0, 0);
+    const bool low = !part && e.R > 0, masked = low && e.low_mask;
+    float b[8];
+    if (!part) bias_cols<T, 8>(e, n, b);
+    auto put = [&](const f32x4& v, int j) { *(f32x4*)(eb + li * 64 + (((4 * j + g) ^ li) << 2)) = v; };
+    auto get = [&](int row, float (&v)[8]) {
+        const f32x4 x = *(const f32x4*)(eb + row * 64 + (((2 * ec) ^ row) << 2)), y = *(const f32x4*)(eb + row * 64 + (((2 * ec + 1) ^ row) << 2));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) d[i] = vec_of<T>(r[2 * i], r[2 * i + 1]);
-}
-template <typename T, int HS>
-__device__ __forceinline__ void read_cols1(typename T::vec8& d, unsigned a) {
-    u32x2 r0, r1;
-    asm volatile("ds_read_b64_tr_b16 %0, %2\n\tds_read_b64_tr_b16 %1, %2 offset:%3\n\ts_waitcnt lgkmcnt(0)"
-                 : "=&v"(r0), "=&v"(r1)
-                 : "v"(a), "i"(HS)
-                 : "memory");
-    d = vec_of<T>(r0, r1);
-}
-
-// four lane groups exchange their four 4-column fragments: group b then holds columns 16 b .. 16 b + 15
-__device__ __forceinline__ void group_transpose(f32x4 (&a)[4]) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        unsigned x[4];
-#pragma unroll
-        for (int f = 0; f < 4; ++f) x[f] = __float_as_uint(a[f][r]);
-#pragma unroll
-        for (int f = 0; f < 2; ++f) {
-            const auto s = __builtin_amdgcn_permlane32_swap(x[f], x[f + 2], false, false);
-            x[f] = s[0];
-            x[f + 2] = s[1];
+        for (int j = 0; j < 4; ++j) {
+            v[j] = x[j];
+            v[4 + j] = y[j];
         }
+    };
+#pragma unroll 1
+    for (int i0 = 0; i0 < FM; ++i0) {
+        const int m0 = mw + 16 * i0;
+        if (m0 >= a.M) break;
+        float t[2][8];
+        if (low) {
+            // rank-R term: fragments straight from global memory (u and v rows are padded to 32 columns)
+            f32x4 tl[4];
 #pragma unroll
-        for (int f = 0; f < 4; f += 2) {
-            const auto s = __builtin_amdgcn_permlane16_swap(x[f], x[f + 1], false, false);
-            x[f] = s[0];
-            x[f + 1] = s[1];
+            for (int j = 0; j < 4; ++j) tl[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            const u32x4 z = {0u, 0u, 0u, 0u};
+            for (int r = 0; r < e.R; r += 32) {
+                const u32x4 uf = m0 + li < a.M ? *(const u32x4*)(e.lu + (int64_t)(m0 + li) * e.R + r + 8 * g) : z;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int c = nw + 16 * j + li;
+                    const u32x4 vf = c < a.N ? *(const u32x4*)(e.lv + (int64_t)c * e.R + r + 8 * g) : z;
+                    tl[j] = T::mfma16(__builtin_bit_cast(vec8, vf), __builtin_bit_cast(vec8, uf), tl[j]);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) put(tl[j], j);
+            get(er, t[0]);
+            get(8 + er, t[1]);
         }
+        // (a rolled loop over a register array: uniform branches pick the fragment row)
 #pragma unroll
-        for (int f = 0; f < 4; ++f) a[f][r] = __uint_as_float(x[f]);
+        for (int i = 0; i < FM; ++i)
+            if (i == i0) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) put(acc[i][j], j);
+            }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int row = 8 * h + er, m = m0 + row;
+            float v[8];
+            get(row, v);
+            if (part) {
+                if (m < a.M && n < N4) {
+                    float* o = part + (int64_t)m * N4 + n;
+                    *(f32x4*)o = f32x4{v[0], v[1], v[2], v[3]};
+                    if (n + 4 < N4) *(f32x4*)(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
+                }
+                continue;
+            }
+            if (masked) {
+                epilogue_cols<T, 8, true>(e, off, m, n, v, b, t[h]);
+            } else {
+                if (low) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] += t[h][j];
+                }
+                epilogue_cols<T, 8, false>(e, off, m, n, v, b, t[h]);
+            }
+        }
     }
 }
 
-// part != null: split-k, slice z writes its fp32 partial sums to part + z * M * N4 (row stride N4)
-template <typename T, bool AK, bool BK, int WM, int WN, int FM, bool PP>
-__global__ __launch_bounds__(64 * WM * WN, PP ? 1 : 2) void matmul_kernel(Matmul a, float* part, int N4, int ksteps) {
+// 256 x 256 tiles. Eight waves in two groups of four, one barrier apart: while one group issues 32 MFMAs the other
+// reads fragments and stages. A k-tile T is two steps: step 0 reads B (kept in registers for both) and the group's
+// first 64 rows of A, step 1 its other 64 rows. Slot = barrier interval; group g reads step (T, h) in slot
+// 4 T + 2 h + g and computes it in the next one.
+//  * A's first halves of T are read in slots 4 T and 4 T + 1, so group 0 refills them (k-tile T + 2) in slot 4 T + 2;
+//    the second halves, read in 4 T + 2 and 4 T + 3, in slot 4 T + 4. Group 0 waits for its four oldest pieces (eight
+//    younger ones may fly) at the end of each of its MFMA segments: each half has six slots to land.
+//  * B of T, read in slots 4 T and 4 T + 1, is refilled by group 1 (k-tile T + 2) at the start of its MFMA segment
+//    in slot 4 T + 2; group 1 waits for the eight pieces of B(T + 1) in slot 4 T + 3.
+// Steps past the last k-tile stage zeros into parts nobody reads (kept, so that the counted waits hold).
+template <typename T, bool AK, bool BK>
+__global__ __launch_bounds__(512, 1) void matmul256_kernel(Matmul a, float* part, int N4, int kslice) {
+    typedef typename T::vec8 vec8;
+    using PA0 = Panel<AK, 128, 4, Half<0>>;
+    using PA1 = Panel<AK, 128, 4, Half<1>>;
+    using PB = Panel<BK, 256, 4, Whole>;
+    constexpr int A_HALF = 16384, A_ST = 32768, B_OFF = 65536, B_ST = 32768, E_OFF = 131072;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[E_OFF + 8 * 4096];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave >> 2, wn = wave & 3;
+    const int nM = (a.M + 255) / 256, nN = (a.N + 255) / 256;
+    int mt, nt;
+    if (!tile_of_block(blockIdx.x, nM, nN, 0, mt, nt)) return;
+    const int m0 = mt * 256, n0 = nt * 256;
+    const int nk_all = (a.K + 63) >> 6;
+    const int kt0 = blockIdx.y * kslice, nk = min(kslice, nk_all - kt0);
+    auto kt_of = [&](int t) { return t < nk ? kt0 + t : nk_all; };
+
+    const unsigned lds = (unsigned)(size_t)(LDS_AS unsigned char*)smem;
+    Frags<T, AK, 128, 4> fa;
+    Frags<T, BK, 256, 4> fb;
+    fa.init(lds, wm * 64, lane);
+    fb.init(lds + B_OFF, wn * 64, lane);
+    vec8 af[2][4], bf[2][4];
+    f32x4 acc[8][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto mfmas = [&](auto half) {
+        constexpr int H = decltype(half)::value * 4;
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[H + i][j] = T::mfma16(bf[ks][j], af[ks][i], acc[H + i][j]);
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    using H0 = std::integral_constant<int, 0>;
+    using H1 = std::integral_constant<int, 1>;
+    if (nk > 0) {
+        if (wm == 0) {
+            PA0 p0;
+            PA1 p1;
+            p0.init(a.A, a.lda, m0, a.M, a.K, wn, lane);
+            p1.init(a.A, a.lda, m0, a.M, a.K, wn, lane);
+            p0.stage(kt_of(0), wn, smem);
+            p1.stage(kt_of(0), wn, smem + A_HALF);
+            p0.stage(kt_of(1), wn, smem + A_ST);
+            vm_wait<8>();
+            bar();
+            for (int t = 0; t < nk; ++t) {
+                const int st = t & 1;
+                p1.stage(kt_of(t + 1), wn, smem + (st ^ 1) * A_ST + A_HALF);
+                fb.read(bf, st * B_ST);
+                fa.read(af, st * A_ST);
+                bar();
+                mfmas(H0{});
+                vm_wait<8>();
+                bar();
+                p0.stage(kt_of(t + 2), wn, smem + st * A_ST);
+                fa.read(af, st * A_ST + A_HALF);
+                bar();
+                mfmas(H1{});
+                vm_wait<8>();
+                bar();
+            }
+            bar();
+        } else {
+            PB pb;
+            pb.init(a.B, a.ldb, n0, a.N, a.K, wn, lane);
+            pb.stage(kt_of(0), wn, smem + B_OFF);
+            pb.stage(kt_of(1), wn, smem + B_OFF + B_ST);
+            vm_wait<8>();
+            bar();
+            bar();
+            for (int t = 0; t < nk; ++t) {
+                const int st = t & 1;
+                fb.read(bf, st * B_ST);
+                fa.read(af, st * A_ST);
+                bar();
+                pb.stage(kt_of(t + 2), wn, smem + B_OFF + st * B_ST);
+                mfmas(H0{});
+                bar();
+                fa.read(af, st * A_ST + A_HALF);
+                vm_wait<8>();
+                bar();
+                mfmas(H1{});
+                bar();
+            }
+        }
+        vm_wait<0>();  // no load into LDS outlives the workgroup
+    }
+    store_tile<T, 8>(a, acc, m0 + wm * 128, n0 + wn * 64, (float*)(smem + E_OFF) + wave * 1024,
+                     part ? part + (int64_t)blockIdx.y * a.M * N4 : nullptr, N4, lane);
+}
+
+// Smaller tiles: WM x WN waves of FM x 16 rows x 64 columns, NS stages, one barrier a k-tile.
+template <typename T, bool AK, bool BK, int WM, int WN, int FM, int NS>
+__global__ __launch_bounds__(64 * WM * WN, 2) void matmul_kernel(Matmul a, float* part, int N4, int kslice) {
     typedef typename T::vec8 vec8;
     constexpr int BM = WM * FM * 16, BN = WN * 64, W = WM * WN;
-    constexpr int A_ST = BM * 64, STAGE = (BM + BN) * 64;
-    static_assert(!PP || (WM == 2 && WN == 4), "ping-pong: two groups of four waves");
-    static_assert(FM == 1 || FM % 4 == 0, "fragment reads come in fours");
-    constexpr int NA = PP ? 4 : W;  // waves that stage A (PP: group 0 stages A, group 1 B)
-    using PA = Panel<AK, BM, NA, false>;
-    using PB = Panel<BK, BN, NA, BK>;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[NS * STAGE];
+    constexpr int A_ST = BM * 128, STAGE = (BM + BN) * 128;
+    using PA = Panel<AK, BM, W, Whole>;
+    using PB = Panel<BK, BN, W, Whole>;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[NS * STAGE + W * 4096];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
@@ -187,184 +382,54 @@ __global__ __launch_bounds__(64 * WM * WN, PP ? 1 : 2) void matmul_kernel(Matmul
     int mt, nt;
     if (!tile_of_block(blockIdx.x, nM, nN, 0, mt, nt)) return;
     const int m0 = mt * BM, n0 = nt * BN;
-    // this slice's k range
-    const int nk_all = (a.K + 31) >> 5;
-    const int kt0 = blockIdx.y * ksteps, nk = min(ksteps, nk_all - kt0);
+    const int nk_all = (a.K + 63) >> 6;
+    const int kt0 = blockIdx.y * kslice, nk = min(kslice, nk_all - kt0);
 
     PA pa;
     PB pb;
-    const int sw = PP ? wn : wave;
-    if (!PP || wm == 0) pa.init(a.A, a.lda, m0, a.M, a.K, sw, lane);
-    if (!PP || wm == 1) pb.init(a.B, a.ldb, n0, a.N, a.K, sw, lane);
-    auto stage = [&](int t) {
-        unsigned char* d = smem + (t & (NS - 1)) * STAGE;
-        // steps past the slice's end fill a stage that is not read (kept, so that the counted waits hold)
-        const int kt = t < nk ? kt0 + t : nk_all;
-        if (!PP || wm == 0) pa.stage(kt, sw, d);
-        if (!PP || wm == 1) pb.stage(kt, sw, d + A_ST);
+    pa.init(a.A, a.lda, m0, a.M, a.K, wave, lane);
+    pb.init(a.B, a.ldb, n0, a.N, a.K, wave, lane);
+    auto stage = [&](int t, int st) {
+        const int kt = t < nk ? kt0 + t : nk_all;  // past the slice: zeros into a stage nobody reads
+        pa.stage(kt, wave, smem + st * STAGE);
+        pb.stage(kt, wave, smem + st * STAGE + A_ST);
     };
-
-    // fragment addresses within a stage
-    const int li = lane & 15, g = lane >> 4, q = li >> 2, p = li & 3;
-    const unsigned lds0 = (unsigned)(size_t)(LDS_AS unsigned char*)smem;
-    unsigned aaddr[AK ? 1 : FM], baddr[BK ? 1 : 4];
-    if constexpr (AK) {
-        aaddr[0] = lds0 + (wm * FM * 16 + li) * 64 + ((g ^ ((li >> 2) & 2)) << 4);
-    } else {
-        const int k = 8 * g + q, f = col_swz<BM>(k);
-#pragma unroll
-        for (int i = 0; i < FM; ++i) aaddr[i] = lds0 + k * (BM * 2) + (((wm * FM + i) ^ f) << 5) + p * 8;
-    }
-    if constexpr (BK) {
-        baddr[0] = lds0 + A_ST + (wn * 64 + li) * 64 + ((g ^ ((li >> 2) & 2)) << 4);
-    } else {
-        const int k = 8 * g + q, f = col_swz<BN>(k);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) baddr[i] = lds0 + A_ST + k * (BN * 2) + (((wn * 4 + i) ^ f) << 5) + p * 8;
-    }
-    vec8 af[FM], bf[4];
+    const unsigned lds = (unsigned)(size_t)(LDS_AS unsigned char*)smem;
+    Frags<T, AK, BM, FM> fa;
+    Frags<T, BK, BN, 4> fb;
+    fa.init(lds, wm * FM * 16, lane);
+    fb.init(lds + A_ST, wn * 64, lane);
+    vec8 af[2][FM], bf[2][4];
     f32x4 acc[FM][4];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-    auto reads = [&](int t) {
-        const unsigned so = (unsigned)(t & (NS - 1)) * STAGE;
-        if constexpr (BK) read_rows4<T>(bf, baddr[0] + so);
-        else read_cols4<T, BN * 8>(bf, baddr[0] + so, baddr[1] + so, baddr[2] + so, baddr[3] + so);
-        if constexpr (FM == 1) {
-            if constexpr (AK) read_rows1<T>(af[0], aaddr[0] + so);
-            else read_cols1<T, BM * 8>(af[0], aaddr[0] + so);
-        } else {
-#pragma unroll
-            for (int i = 0; i < FM; i += 4) {
-                vec8 d[4];
-                if constexpr (AK) read_rows4<T>(d, aaddr[0] + so + i * 1024);
-                else read_cols4<T, BM * 8>(d, aaddr[i] + so, aaddr[i + 1] + so, aaddr[i + 2] + so, aaddr[i + 3] + so);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) af[i + j] = d[j];
-            }
-        }
-    };
-    auto mfmas = [&]() {
-        __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = T::mfma16(bf[j], af[i], acc[i][j]);
-        __builtin_amdgcn_s_setprio(0);
-    };
-    auto bar = [&]() {
-        __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
-    };
-
     if (nk > 0) {
-        stage(0);
-        stage(1);
-        stage(2);
-        if constexpr (PP) {
-            // Two groups of four waves, one barrier apart: while one issues its 32 MFMAs the other stages
-            // k-step t + 3 and reads its fragments. A wave waits for its own pieces of step t + 1 (two
-            // younger groups may be in flight) before the barrier that ends slot 2 t + 1.
-            constexpr int AHEAD_A = 2 * PA::NP, AHEAD_B = 2 * PB::NP;
-            if (wm == 0) {
-                vm_wait<AHEAD_A>();
-                bar();
-                for (int t = 0; t < nk; ++t) {
-                    stage(t + 3);
-                    reads(t);
-                    bar();
-                    mfmas();
-                    __builtin_amdgcn_sched_barrier(0);
-                    vm_wait<AHEAD_A>();
-                    bar();
-                }
-                bar();
-            } else {
-                vm_wait<AHEAD_B>();
-                bar();
-                bar();
-                for (int t = 0; t < nk; ++t) {
-                    stage(t + 3);
-                    vm_wait<AHEAD_B>();
-                    reads(t);
-                    bar();
-                    mfmas();
-                    bar();
-                }
-            }
-        } else {
-            constexpr int AHEAD = 2 * (PA::NP + PB::NP);
-            for (int t = 0; t < nk; ++t) {
-                vm_wait<AHEAD>();  // this wave's pieces of step t
-                bar();             // every wave's; and step t - 1 is read by all
-                stage(t + 3);
-                reads(t);
-                mfmas();
-            }
+        constexpr int NP = PA::NP + PB::NP;
+#pragma unroll
+        for (int t = 0; t < NS - 1; ++t) stage(t, t);
+        int st = 0;
+        for (int t = 0; t < nk; ++t) {
+            vm_wait<(NS - 2) * NP>();  // this wave's pieces of k-tile t
+            bar();                     // every wave's; and k-tile t - 1 is read by all
+            stage(t + NS - 1, st == 0 ? NS - 1 : st - 1);
+            fb.read(bf, st * STAGE);
+            fa.read(af, st * STAGE);
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[i][j] = T::mfma16(bf[ks][j], af[ks][i], acc[i][j]);
+            __builtin_amdgcn_s_setprio(0);
+            st = st == NS - 1 ? 0 : st + 1;
         }
         vm_wait<0>();  // no load into LDS outlives the workgroup
     }
-
-    // ---- epilogue ----
-    const uint2 off = a.e.drop.on ? drop_offset(a.e.drop) : make_uint2(0, 0);
-    const bool low = !part && a.e.R > 0;
-    const int nw = n0 + wn * 64;  // the wave's first column
-#pragma unroll 1
-    for (int i0 = 0; i0 < FM; ++i0) {
-        // (a rolled loop over a register array: the switch below selects the fragment row)
-        f32x4 c[4];
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-            if (i == i0) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) c[j] = acc[i][j];
-            }
-        const int m = m0 + (wm * FM + i0) * 16 + li;
-        f32x4 tl[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) tl[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (low) {
-            // rank-R term: fragments straight from global memory (u and v rows are padded to 32 columns)
-            for (int r = 0; r < a.e.R; r += 32) {
-                const u32x4 z = {0u, 0u, 0u, 0u};
-                const u32x4 uf = m < a.M ? *(const u32x4*)(a.e.lu + (int64_t)m * a.e.R + r + 8 * g) : z;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int n = nw + (BK ? 16 * (li >> 2) + 4 * j + (li & 3) : 16 * j + li);
-                    const u32x4 vf = n < a.N ? *(const u32x4*)(a.e.lv + (int64_t)n * a.e.R + r + 8 * g) : z;
-                    tl[j] = T::mfma16(__builtin_bit_cast(vec8, vf), __builtin_bit_cast(vec8, uf), tl[j]);
-                }
-            }
-        }
-        if constexpr (!BK) {
-            group_transpose(c);
-            if (low) group_transpose(tl);
-        }
-        const int n = nw + 16 * g;
-        if (part) {
-            if (m < a.M) {
-                float* o = part + ((int64_t)blockIdx.y * a.M + m) * N4 + n;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (n + 4 * j < N4) *(f32x4*)(o + 4 * j) = c[j];
-            }
-            continue;
-        }
-        float v[16], t[16];
-        const bool masked = low && a.e.low_mask;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            v[j] = c[j >> 2][j & 3];
-            t[j] = tl[j >> 2][j & 3];
-            if (!masked) v[j] += t[j];
-        }
-        if (masked) epilogue_cols<T, 16, true>(a.e, off, m, n, v, t);
-        else epilogue_cols<T, 16, false>(a.e, off, m, n, v, t);
-    }
+    store_tile<T, FM>(a, acc, m0 + wm * FM * 16, n0 + wn * 64, (float*)(smem + NS * STAGE) + wave * 1024,
+                      part ? part + (int64_t)blockIdx.y * a.M * N4 : nullptr, N4, lane);
 }
 
 // join of a split product: the slices' partial sums in order, then the epilogue; four columns a thread
@@ -391,8 +456,10 @@ __global__ __launch_bounds__(256) void matmul_join_kernel(Epilogue e, const floa
             else v[j] += d;
         }
     }
-    if (e.R > 0 && e.low_mask) epilogue_cols<T, 4, true>(e, off, m, n, v, t);
-    else epilogue_cols<T, 4, false>(e, off, m, n, v, t);
+    float b[4];
+    bias_cols<T, 4>(e, n, b);
+    if (e.R > 0 && e.low_mask) epilogue_cols<T, 4, true>(e, off, m, n, v, b, t);
+    else epilogue_cols<T, 4, false>(e, off, m, n, v, b, t);
 }
 
 // an operand whose rows the 16-byte loads cannot address (odd length, stride or base): copied to rows of
@@ -428,13 +495,13 @@ Plan plan_of(const Matmul& a) {
     if (a.K > 0 && !loadable(a.A, a.lda, al)) p.a_bytes = (size_t)up((int64_t)ar * up(al, 8) * 2, 256);
     if (a.K > 0 && !loadable(a.B, a.ldb, bl)) p.b_bytes = (size_t)up((int64_t)br * up(bl, 8) * 2, 256);
     p.tile = tiles(a.M, a.N, 256) >= 128 ? 2 : tiles(a.M, a.N, 128) >= 128 ? 1 : 0;
-    const int nk = (a.K + 31) / 32;
+    const int nk = (a.K + 63) / 64;
     p.S = 1;
     p.ksteps = nk > 0 ? nk : 1;
     p.N4 = (int)up(a.N, 4);
     const int nt = p.tile == 2 ? tiles(a.M, a.N, 256) : p.tile == 1 ? tiles(a.M, a.N, 128) : tiles(a.M, a.N, 64);
-    if (nt < 256 && nk >= 16) {  // few tiles and a long k: slices of at least 8 k-steps, about 512 workgroups
-        int S = min(min(512 / nt, nk / 8), 64);
+    if (nt < 256 && nk >= 8) {  // few tiles and a long k: slices of at least 4 k-tiles, about 512 workgroups
+        int S = min(min(512 / nt, nk / 4), 64);
         if (S > 1) {
             p.ksteps = (nk + S - 1) / S;
             p.S = (nk + p.ksteps - 1) / p.ksteps;
@@ -448,9 +515,9 @@ template <typename T, bool AK, bool BK>
 void launch_tile(hipStream_t s, const Matmul& a, const Plan& p, float* part) {
     const int bm = p.tile == 2 ? 256 : p.tile == 1 ? 128 : 64;
     const dim3 grid(tiles(a.M, a.N, bm), p.S);
-    if (p.tile == 2) matmul_kernel<T, AK, BK, 2, 4, 8, true><<<grid, 512, 0, s>>>(a, part, p.N4, p.ksteps);
-    else if (p.tile == 1) matmul_kernel<T, AK, BK, 2, 2, 4, false><<<grid, 256, 0, s>>>(a, part, p.N4, p.ksteps);
-    else matmul_kernel<T, AK, BK, 4, 1, 1, false><<<grid, 256, 0, s>>>(a, part, p.N4, p.ksteps);
+    if (p.tile == 2) matmul256_kernel<T, AK, BK><<<grid, 512, 0, s>>>(a, part, p.N4, p.ksteps);
+    else if (p.tile == 1) matmul_kernel<T, AK, BK, 2, 2, 4, 2><<<grid, 256, 0, s>>>(a, part, p.N4, p.ksteps);
+    else matmul_kernel<T, AK, BK, 4, 1, 1, 3><<<grid, 256, 0, s>>>(a, part, p.N4, p.ksteps);
 }
 
 template <typename T>
