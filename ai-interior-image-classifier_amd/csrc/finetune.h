@@ -58,32 +58,43 @@ __device__ __forceinline__ float logistic(float t) {
 }
 // value and derivative; the derivative's z factors are clamped so that it reaches its limit (0 or 1) at
 // +-inf instead of inf * 0 (a NaN z gives NaN through the gate)
-template <bool SLOPE>
-__device__ __forceinline__ float act_apply(int act, float z, float& slope) {
+template <bool SLOPE, int ACT>
+__device__ __forceinline__ float act_one(float beta, float z, float& slope) {
     const float zc = SLOPE ? fminf(fmaxf(z, -100.f), 100.f) : z;
-    if (act == ACT_QUICK_GELU || act == ACT_SILU) {
-        const float beta = act == ACT_SILU ? 1.0f : 1.702f;
-        const float s = logistic(beta * z);
-        if (SLOPE) slope = s * (1.0f + beta * zc * (1.0f - s));
+    if constexpr (ACT == ACT_SILU) {  // also quick_gelu: beta 1.702
+        const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(beta * z));  // beta = -log2(e) beta
+        if (SLOPE) slope = s * (1.0f - 0.69314718055994531f * beta * zc * (1.0f - s));
         return z * s;
-    }
-    if (act == ACT_GELU) {
+    } else if constexpr (ACT == ACT_GELU) {
         const float c = 0.5f + 0.5f * erff(0.70710678118654752f * z);
         if (SLOPE) slope = c + 0.39894228040143268f * zc * __builtin_amdgcn_exp2f(-0.72134752044448170f * zc * zc);
         return z * c;
-    }
-    if (act == ACT_GELU_TANH) {
-        const float z2 = zc * zc;
+    } else if constexpr (ACT == ACT_GELU_TANH) {
         const float s = logistic(1.5957691216057308f * (z + 0.044715f * z * (z * z)));
-        if (SLOPE) slope = s + zc * s * (1.0f - s) * (1.5957691216057308f * (1.0f + 0.134145f * z2));
+        if (SLOPE) slope = s + zc * s * (1.0f - s) * (1.5957691216057308f * (1.0f + 0.134145f * (zc * zc)));
         return z * s;
-    }
-    if (act == ACT_RELU) {
+    } else {
         if (SLOPE) slope = z != z ? z : (z > 0.f ? 1.f : 0.f);
         return z != z ? z : fmaxf(z, 0.f);
     }
-    slope = 1.f;
-    return z;
+}
+// C values at once: one uniform branch on the kind, not one an element
+template <bool SLOPE, int C>
+__device__ __forceinline__ void act_cols(int act, float (&v)[C], float (&g)[C]) {
+    if (act == ACT_QUICK_GELU || act == ACT_SILU) {
+        const float beta = act == ACT_SILU ? -1.4426950408889634f : -2.4554669595930157f;
+#pragma unroll
+        for (int j = 0; j < C; ++j) v[j] = act_one<SLOPE, ACT_SILU>(beta, v[j], g[j]);
+    } else if (act == ACT_GELU) {
+#pragma unroll
+        for (int j = 0; j < C; ++j) v[j] = act_one<SLOPE, ACT_GELU>(0.f, v[j], g[j]);
+    } else if (act == ACT_GELU_TANH) {
+#pragma unroll
+        for (int j = 0; j < C; ++j) v[j] = act_one<SLOPE, ACT_GELU_TANH>(0.f, v[j], g[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < C; ++j) v[j] = act_one<SLOPE, ACT_RELU>(0.f, v[j], g[j]);
+    }
 }
 // The derivative as the forward saves it: 16-bit fixed point, steps of 2^-14. All of these derivatives
 // lie in (-0.13, 1.13), so the rounding is at most 2^-15 absolute, 16 times below the half step of an fp16
@@ -139,14 +150,12 @@ __device__ __forceinline__ void epilogue_cols(const Epilogue& e, const uint2& of
         for (int j = 0; j < C; ++j) v[j] += t[j];
     }
     if (e.act != ACT_NONE) {
+        float gr[C];
         if (e.slope) {
             short q[C];
+            act_cols<true, C>(e.act, v, gr);
 #pragma unroll
-            for (int j = 0; j < C; ++j) {
-                float g;
-                v[j] = act_apply<true>(e.act, v[j], g);
-                q[j] = slope_encode(g);
-            }
+            for (int j = 0; j < C; ++j) q[j] = slope_encode(gr[j]);
             short* s = e.slope + (int64_t)m * e.N + n;
             if (whole) {
                 if constexpr (C % 8 == 0) {
@@ -167,9 +176,7 @@ __device__ __forceinline__ void epilogue_cols(const Epilogue& e, const uint2& of
                     if (j < nc) s[j] = q[j];
             }
         } else {
-            float g;
-#pragma unroll
-            for (int j = 0; j < C; ++j) v[j] = act_apply<false>(e.act, v[j], g);
+            act_cols<false, C>(e.act, v, gr);
         }
     }
     if (!LOW && e.drop.on) {

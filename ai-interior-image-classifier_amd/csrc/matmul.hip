@@ -133,6 +133,7 @@ struct Frags {
                 : "v"(addr[0] + so), "v"(addr[1] + so)
                 : "memory");
         } else if constexpr (KC) {
+            static_assert(FR == 1, "one or four fragments");
             asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %3\n\ts_waitcnt lgkmcnt(0)"
                          : "=&v"(d[0][0]), "=&v"(d[1][0])
                          : "v"(addr[0] + so), "v"(addr[1] + so)
@@ -169,6 +170,20 @@ struct Frags {
         }
     }
 };
+
+// Block -> tile. Blocks b, b + 8, .. share an XCD (speed only): each XCD takes a contiguous range of an order that
+// walks bands of six tile rows column by column, so the 32 tiles it runs at a time are about 6 x 5 and share their
+// operand panels in its L2 (against tiles in row-major order: 18464 x 1024 x 4096 forward 200 -> 167 us,
+// 36928 x 1024 x 4096 370 -> 330 us; bands of 4 and 8 rows measure the same within 1 %).
+__device__ __forceinline__ void tile_at(int bid, int nM, int nN, int& mt, int& nt) {
+    constexpr int G = 6;
+    const int nwg = nM * nN;
+    const int q = nwg >> 3, r = nwg & 7, x = bid & 7;
+    const int t = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (bid >> 3);
+    const int band = t / (G * nN), m0 = band * G, gm = min(G, nM - m0), rr = t - band * G * nN;
+    nt = rr / gm;
+    mt = m0 + rr - nt * gm;
+}
 
 __device__ __forceinline__ void bar() {
     __builtin_amdgcn_sched_barrier(0);
@@ -278,7 +293,7 @@ __global__ __launch_bounds__(512, 1) void matmul256_kernel(Matmul a, float* part
     const int wm = wave >> 2, wn = wave & 3;
     const int nM = (a.M + 255) / 256, nN = (a.N + 255) / 256;
     int mt, nt;
-    if (!tile_of_block(blockIdx.x, nM, nN, 0, mt, nt)) return;
+    tile_at(blockIdx.x, nM, nN, mt, nt);
     const int m0 = mt * 256, n0 = nt * 256;
     const int nk_all = (a.K + 63) >> 6;
     const int kt0 = blockIdx.y * kslice, nk = min(kslice, nk_all - kt0);
@@ -380,7 +395,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_kernel(Matmul a, float
     const int wm = wave / WN, wn = wave % WN;
     const int nM = (a.M + BM - 1) / BM, nN = (a.N + BN - 1) / BN;
     int mt, nt;
-    if (!tile_of_block(blockIdx.x, nM, nN, 0, mt, nt)) return;
+    tile_at(blockIdx.x, nM, nN, mt, nt);
     const int m0 = mt * BM, n0 = nt * BN;
     const int nk_all = (a.K + 63) >> 6;
     const int kt0 = blockIdx.y * kslice, nk = min(kslice, nk_all - kt0);
@@ -488,23 +503,44 @@ struct Plan {
 
 int tiles(int M, int N, int t) { return ((M + t - 1) / t) * ((N + t - 1) / t); }
 
+// Estimated time of a launch: rounds of workgroups times (k-tiles of a slice x time of one + start and epilogue),
+// and the join of a split. Fitted to forward products measured at every (tile, slices) on 12 shapes, M x K x N: e.g.
+// 12608 x 4096 x 1024 64 / 128 / 256-wide tiles 170 / 107 / 115 us, 256 in two slices 144; 4928 x 512 x 2048 27 / 23 / 24 us;
+// 4096 x 36928 x 1024 256 in 1 / 2 / 4 / 8 slices 864 / 452 / 275 / 297 us; 2048 x 4928 x 512 64 in 1 / 2 / 4 slices 27.5 / 24.0 / 26.9
+// us; 1237 x 768 x 440 7 / 13 / 26 us.
+double cost_us(int tile, int nt, int S, int ks, double out) {
+    // one 256-wide workgroup a CU; two of the smaller ones, each slower beside the other than alone
+    static const double alone[3] = {0.30, 0.83, 1.60}, beside[3] = {0.43, 1.13, 1.60}, fixed[3] = {2.5, 4.0, 10.0};
+    const int64_t wgs = (int64_t)nt * S, slots = tile == 2 ? 256 : 512, full = wgs / slots, rest = wgs % slots;
+    double t = full * (ks * beside[tile] + fixed[tile]);
+    if (rest) t += ks * (rest <= 256 ? alone[tile] : beside[tile]) + fixed[tile];
+    if (S > 1) t += 5.0 + (S * 8.0 + 2.0) * out / 4.5e6;
+    return t;
+}
+
 Plan plan_of(const Matmul& a) {
     Plan p{};
     const int al = a.a_k ? a.K : a.M, ar = a.a_k ? a.M : a.K, bl = a.b_k ? a.K : a.N, br = a.b_k ? a.N : a.K;
     auto up = [](int64_t v, int64_t q) { return (v + q - 1) / q * q; };
     if (a.K > 0 && !loadable(a.A, a.lda, al)) p.a_bytes = (size_t)up((int64_t)ar * up(al, 8) * 2, 256);
     if (a.K > 0 && !loadable(a.B, a.ldb, bl)) p.b_bytes = (size_t)up((int64_t)br * up(bl, 8) * 2, 256);
-    p.tile = tiles(a.M, a.N, 256) >= 128 ? 2 : tiles(a.M, a.N, 128) >= 128 ? 1 : 0;
     const int nk = (a.K + 63) / 64;
+    p.N4 = (int)up(a.N, 4);
+    p.tile = 0;
     p.S = 1;
     p.ksteps = nk > 0 ? nk : 1;
-    p.N4 = (int)up(a.N, 4);
-    const int nt = p.tile == 2 ? tiles(a.M, a.N, 256) : p.tile == 1 ? tiles(a.M, a.N, 128) : tiles(a.M, a.N, 64);
-    if (nt < 256 && nk >= 8) {  // few tiles and a long k: slices of at least 4 k-tiles, about 512 workgroups
-        int S = min(min(512 / nt, nk / 4), 64);
-        if (S > 1) {
-            p.ksteps = (nk + S - 1) / S;
-            p.S = (nk + p.ksteps - 1) / p.ksteps;
+    double best = 1e30;
+    for (int t = 0; t < 3; ++t) {
+        const int nt = tiles(a.M, a.N, 64 << t);
+        for (int S = 1; S <= 64 && (S == 1 || (nk >= 2 * S && (int64_t)nt * S <= 1024)); ++S) {
+            const int ks = nk > 0 ? (nk + S - 1) / S : 1;
+            const double c = cost_us(t, nt, S, ks, (double)a.M * p.N4);
+            if (c < best) {
+                best = c;
+                p.tile = t;
+                p.ksteps = ks;
+                p.S = nk > 0 ? (nk + ks - 1) / ks : 1;
+            }
         }
     }
     if (p.S > 1) p.part_bytes = (size_t)p.S * a.M * p.N4 * 4;
