@@ -27,8 +27,9 @@ EXPORTS = (
     "clipvit_gemm_mx8_test", "clipvit_preprocess", "clipvit_resample_plan",
     "clipvit_text_create", "clipvit_text_load_weights", "clipvit_text_load_lora",
     "clipvit_encode_text", "clipvit_text_destroy", "clipvit_residual_x24_test", "clipvit_set_tuning",
-    "clipvit_gemm_log", "clipvit_linear_workspace", "clipvit_linear", "clipvit_linear_dz", "clipvit_dropout",
-    "clipvit_lora_pad", "clipvit_lora_down", "clipvit_lora_grad_workspace", "clipvit_lora_grad",
+    "clipvit_gemm_log", "clipvit_linear_workspace", "clipvit_linear", "clipvit_linear_grad_workspace",
+    "clipvit_linear_grad", "clipvit_dropout", "clipvit_lora_linear_workspace", "clipvit_lora_linear",
+    "clipvit_lora_linear_grad_workspace", "clipvit_lora_linear_grad",
 )
 
 
@@ -69,26 +70,30 @@ class DropoutArgs(ctypes.Structure):
                 ("offset_dev", ctypes.c_void_p)]
 
 
+def _fields(spec: str):
+    """"name:t" items: i int, q int64, p pointer, f float, d DropoutArgs (x_row, x_col: the header's x_stride[2])."""
+    kind = {"i": ctypes.c_int, "q": ctypes.c_int64, "p": ctypes.c_void_p, "f": ctypes.c_float, "d": DropoutArgs}
+    return [(n, kind[t]) for n, t in (s.split(":") for s in spec.split())]
+
+
 class LinearArgs(ctypes.Structure):
-    _fields_ = [("dtype", ctypes.c_int), ("activation", ctypes.c_int), ("bias_dtype", ctypes.c_int),
-                ("low_mask", ctypes.c_int), ("M", ctypes.c_int64), ("N", ctypes.c_int64),
-                ("K", ctypes.c_int64), ("R", ctypes.c_int64), ("x", ctypes.c_void_p),
-                ("x_stride", ctypes.c_int64 * 2), ("w", ctypes.c_void_p), ("w_stride", ctypes.c_int64 * 2),
-                ("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("residual_stride", ctypes.c_int64),
-                ("y", ctypes.c_void_p), ("y_stride", ctypes.c_int64), ("slope", ctypes.c_void_p),
-                ("low_u", ctypes.c_void_p), ("low_v", ctypes.c_void_p), ("dropout", DropoutArgs)]
+    _fields_ = _fields("dtype:i activation:i bias_dtype:i reserved:i M:q N:q K:q x:p x_row:q x_col:q w:p w_row:q w_col:q "
+                       "bias:p residual:p residual_stride:q y:p y_stride:q slope:p dropout:d")
 
 
-class DzArgs(ctypes.Structure):
-    _fields_ = [("dtype", ctypes.c_int), ("db_dtype", ctypes.c_int), ("M", ctypes.c_int64), ("N", ctypes.c_int64),
-                ("dy", ctypes.c_void_p), ("dy_stride", ctypes.c_int64), ("slope", ctypes.c_void_p),
-                ("dz", ctypes.c_void_p), ("dz_stride", ctypes.c_int64), ("db", ctypes.c_void_p),
-                ("dropout", DropoutArgs)]
+class LinearGradArgs(ctypes.Structure):
+    _fields_ = _fields("dtype:i bias_dtype:i M:q N:q K:q dy:p dy_stride:q x:p x_row:q x_col:q w:p w_row:q w_col:q slope:p "
+                       "dx:p dw:p db:p dropout:d")
 
 
-class PadArgs(ctypes.Structure):
-    _fields_ = [("src", ctypes.c_void_p)] + [(n, ctypes.c_int64) for n in (
-        "row_stride", "col_stride", "rows", "cols", "rows_padded", "cols_padded")] + [("dst", ctypes.c_void_p)]
+class LoraArgs(ctypes.Structure):
+    _fields_ = _fields("dtype:i bias_dtype:i M:q N:q K:q rank:q x:p x_stride:q w:p w_row:q w_col:q a:p a_row:q a_col:q b:p "
+                       "b_row:q b_col:q bias:p y:p u:p scaling:f reserved:f dropout:d")
+
+
+class LoraGradArgs(ctypes.Structure):
+    _fields_ = _fields("dtype:i bias_dtype:i M:q N:q K:q rank:q dy:p dy_stride:q x:p x_stride:q w:p w_row:q w_col:q a:p "
+                       "a_row:q a_col:q b:p b_row:q b_col:q u:p dx:p dw:p da:p db_factor:p dbias:p scaling:f reserved:f dropout:d")
 
 
 _lock = threading.Lock()
@@ -136,17 +141,12 @@ def lib() -> ctypes.CDLL:
             "clipvit_preprocess": (i, [vp, vp, ctypes.POINTER(Image), i, i, i, vp]),
             "clipvit_resample_plan": (i, [i, i, ctypes.POINTER(i), ctypes.POINTER(i),
                                           ctypes.POINTER(ctypes.c_int32), i]),
-            "clipvit_linear_workspace": (i, [ctypes.POINTER(LinearArgs), ctypes.POINTER(sz)]),
-            "clipvit_linear": (i, [vp, ctypes.POINTER(LinearArgs), vp, sz]),
-            "clipvit_linear_dz": (i, [vp, ctypes.POINTER(DzArgs), vp, sz]),
             "clipvit_dropout": (i, [vp, i, vp, i64, vp, i64, vp, i64, i64, i64, ctypes.POINTER(DropoutArgs)]),
-            "clipvit_lora_pad": (i, [vp, ctypes.POINTER(PadArgs), ctypes.POINTER(PadArgs)]),
-            "clipvit_lora_down": (i, [vp, i, vp, i64, vp, i64, vp, i64, i64, i64, ctypes.c_float,
-                                      ctypes.POINTER(DropoutArgs)]),
-            "clipvit_lora_grad_workspace": (i, [i64, i64, i64, ctypes.POINTER(sz)]),
-            "clipvit_lora_grad": (i, [vp, i, vp, i64, vp, vp, i64, i64, i64, i64, i64, i64,
-                                      ctypes.POINTER(DropoutArgs), vp, sz]),
         }
+        for name, args in (("linear", LinearArgs), ("linear_grad", LinearGradArgs), ("lora_linear", LoraArgs),
+                           ("lora_linear_grad", LoraGradArgs)):
+            sig[f"clipvit_{name}_workspace"] = (i, [ctypes.POINTER(args), ctypes.POINTER(sz)])
+            sig[f"clipvit_{name}"] = (i, [vp, ctypes.POINTER(args), vp, sz])
         for name, (res, args) in sig.items():
             fn = getattr(L, name)
             fn.restype, fn.argtypes = res, args

@@ -429,71 +429,196 @@ Dropout make_dropout(const clipvit_dropout_args& d) {
 }
 
 // a [rows, cols] view with one unit stride -> (contiguous along columns?, row stride); false: refused
-bool panel_of(const int64_t (&st)[2], int64_t rows, int64_t cols, int& contig, int64_t& ld) {
-    if (st[1] == 1 || cols == 1) {
+bool panel_of(int64_t s0, int64_t s1, int64_t rows, int64_t cols, int& contig, int64_t& ld) {
+    if (s1 == 1 || cols == 1) {
         contig = 1;
-        ld = rows <= 1 ? up(cols, 8) : st[0];
-        if (cols == 1 && rows > 1 && st[0] == 1) {  // one column of consecutive elements
+        ld = rows <= 1 ? up(cols, 8) : s0;
+        if (cols == 1 && rows > 1 && s0 == 1) {  // one column of consecutive elements
             contig = 0;
             ld = up(rows, 8);
             return true;
         }
         return rows <= 1 || (ld >= cols && ld < MATMUL_MAX_LD);
     }
-    if (st[0] == 1 || rows == 1) {
+    if (s0 == 1 || rows == 1) {
         contig = 0;
-        ld = cols <= 1 ? up(rows, 8) : st[1];
+        ld = cols <= 1 ? up(rows, 8) : s1;
         return ld >= rows && ld < MATMUL_MAX_LD;
     }
     return false;
 }
 
-int matmul_of(const clipvit_linear_args* a, Matmul& m) {
+// C [M, N] = A(m, k) B(n, k)^T with the given strides; false: an operand is refused
+bool make_matmul(Matmul& m, const void* A, int64_t a0, int64_t a1, const void* B, int64_t b0, int64_t b1, int64_t M, int64_t N, int64_t K,
+                 void* y, int64_t ldy) {
+    m = Matmul{};
+    m.A = (const u16*)A;
+    m.B = (const u16*)B;
+    m.M = (int)M;
+    m.N = (int)N;
+    m.K = (int)K;
+    m.e.M = m.M;
+    m.e.N = m.N;
+    m.e.y = y;
+    m.e.ldy = M > 1 ? ldy : up(N, 8);
+    if (!M || !N || !K) return true;
+    return panel_of(a0, a1, M, K, m.a_k, m.lda) && panel_of(b0, b1, N, K, m.b_k, m.ldb);
+}
+
+// A workspace as consecutive 256-byte aligned parts; with a null base it only counts.
+struct Arena {
+    unsigned char* base;
+    size_t used = 0;
+    void* take(size_t bytes) {
+        void* p = base ? base + used : nullptr;
+        used += (bytes + 255) / 256 * 256;
+        return p;
+    }
+};
+
+struct Db {  // dz / bias-gradient launch
+    DzArgs d;
+    void* db;
+    int db_f32, blocks;
+};
+Db make_dz(const void* dy, int64_t dy_stride, const int16_t* slope, void* dz, int64_t lddz, void* db, int db_f32, int64_t M, int64_t N,
+           const Dropout& drop) {
+    Db b{};
+    DzArgs& d = b.d;
+    b.db = db;
+    b.db_f32 = db_f32;
+    // blocks of at least 64 rows, at most 512 of them
+    b.blocks = (int)((M + 63) / 64 < 512 ? (M + 63) / 64 : 512);
+    d.rows = b.blocks ? (int)up((M + b.blocks - 1) / b.blocks, 8) : 8;
+    d.dy = dy;
+    d.slope = slope;
+    d.dz = dz;
+    d.lddy = M > 1 ? dy_stride : up(N, 8);
+    d.lddz = lddz;
+    d.M = (int)M;
+    d.N = (int)N;
+    d.d = drop;
+    d.vec = aligned16(dy) && d.lddy % 8 == 0 && (!dz || (aligned16(dz) && lddz % 8 == 0)) && (!slope || (aligned16(slope) && N % 8 == 0));
+    return b;
+}
+size_t dz_part_bytes(const Db& b) { return b.db ? (size_t)b.blocks * b.d.N * 4 : 0; }
+void launch_dz(hipStream_t s, bool bf, Db& b, void* part) {
+    b.d.part = b.db ? (float*)part : nullptr;
+    if (b.blocks) {
+        const dim3 grid((b.d.N + 255) / 256, b.blocks);
+        if (bf) dz_kernel<BF16T><<<grid, 256, 0, s>>>(b.d);
+        else dz_kernel<F16T><<<grid, 256, 0, s>>>(b.d);
+    }
+    if (b.db) {
+        const int g = (b.d.N + 31) / 32;
+        if (bf) db_kernel<BF16T><<<g, 256, 0, s>>>(b.d.part, b.blocks, b.d.N, b.db, b.db_f32);
+        else db_kernel<F16T><<<g, 256, 0, s>>>(b.d.part, b.blocks, b.d.N, b.db, b.db_f32);
+    }
+}
+
+// ---- Linear ----
+int check_sizes(const char* what, int dtype, int bias_dtype, int64_t M, int64_t N, int64_t K) {
+    if (!is16(dtype)) FT_FAIL(CLIPVIT_E_INVALID, std::string(what) + ": dtype must be BF16 or F16");
+    if (bias_dtype != CLIPVIT_F32 && bias_dtype != dtype) FT_FAIL(CLIPVIT_E_INVALID, std::string(what) + ": bias must be F32 or of the operands' type");
+    if (M < 0 || N < 0 || K < 0 || M > MAX_DIM || N > MAX_DIM || K > MAX_DIM)
+        FT_FAIL(CLIPVIT_E_INVALID, std::string(what) + ": M, N and K must lie in [0, 2^30]");
+    return CLIPVIT_OK;
+}
+const char* const OPERANDS = "x and w need one unit stride, rows that do not overlap and a stride below 2^22";
+
+int linear_of(const clipvit_linear_args* a, Matmul& m) {
     if (!a) FT_FAIL(CLIPVIT_E_INVALID, "null arguments");
-    if (!is16(a->dtype)) FT_FAIL(CLIPVIT_E_INVALID, "linear: dtype must be BF16 or F16");
+    if (const int rc = check_sizes("linear", a->dtype, a->bias_dtype, a->M, a->N, a->K)) return rc;
     if (a->activation < 0 || a->activation > ACT_RELU) FT_FAIL(CLIPVIT_E_INVALID, "linear: unknown activation");
-    if (a->bias_dtype != CLIPVIT_F32 && a->bias_dtype != a->dtype) FT_FAIL(CLIPVIT_E_INVALID, "linear: bias must be F32 or of the operands' type");
-    if (a->M < 0 || a->N < 0 || a->K < 0 || a->R < 0 || a->M > MAX_DIM || a->N > MAX_DIM || a->K > MAX_DIM)
-        FT_FAIL(CLIPVIT_E_INVALID, "linear: M, N and K must lie in [0, 2^30]");
+    if (bad_dropout(a->dropout)) FT_FAIL(CLIPVIT_E_INVALID, "dropout: p must lie in [0, 1]");
     if (a->M && a->N) {
         if (!a->y || (a->K && (!a->x || !a->w))) FT_FAIL(CLIPVIT_E_INVALID, "linear: null operand");
         if (a->y_stride < a->N && a->M > 1) FT_FAIL(CLIPVIT_E_INVALID, "linear: y rows overlap");
         if (a->residual && a->residual_stride < 0) FT_FAIL(CLIPVIT_E_INVALID, "linear: residual stride");
-        if (a->K && (!panel_of(a->x_stride, a->M, a->K, m.a_k, m.lda) || !panel_of(a->w_stride, a->N, a->K, m.b_k, m.ldb)))
-            FT_FAIL(CLIPVIT_E_INVALID, "linear: x and w need one unit stride, rows that do not overlap and a stride below 2^22");
-        if (a->R && (a->R % 32 || !a->low_u || !a->low_v || !aligned16(a->low_u) || !aligned16(a->low_v)))
-            FT_FAIL(CLIPVIT_E_INVALID, "linear: the low-rank factors need 16-byte aligned rows padded to a multiple of 32");
     }
-    if (bad_dropout(a->dropout)) FT_FAIL(CLIPVIT_E_INVALID, "dropout: p must lie in [0, 1]");
-    if (a->low_mask && (a->activation || a->bias)) FT_FAIL(CLIPVIT_E_INVALID, "linear: a masked low-rank term takes no bias or activation");
-    m.A = (const u16*)a->x;
-    m.B = (const u16*)a->w;
-    m.M = (int)a->M;
-    m.N = (int)a->N;
-    m.K = (int)a->K;
+    if (!make_matmul(m, a->x, a->x_stride[0], a->x_stride[1], a->w, a->w_stride[0], a->w_stride[1], a->M, a->N, a->K, a->y, a->y_stride))
+        FT_FAIL(CLIPVIT_E_INVALID, std::string("linear: ") + OPERANDS);
     Epilogue& e = m.e;
-    e.y = a->y;
     e.bias = a->bias;
-    e.res = a->residual;
-    e.slope = a->activation ? a->slope : nullptr;
-    e.ldy = a->M > 1 ? a->y_stride : up(a->N, 8);
-    e.ldr = a->M > 1 ? a->residual_stride : up(a->N, 8);
-    e.M = m.M;
-    e.N = m.N;
     e.bias_f32 = a->bias_dtype == CLIPVIT_F32;
+    e.res = a->residual;
+    e.ldr = a->M > 1 ? a->residual_stride : up(a->N, 8);
+    e.slope = a->activation ? a->slope : nullptr;
     e.act = a->activation;
     e.drop = make_dropout(a->dropout);
-    e.lu = (const u16*)a->low_u;
-    e.lv = (const u16*)a->low_v;
-    e.R = (int)a->R;
-    e.low_mask = a->low_mask && e.drop.on;
-    if (a->low_mask && !e.drop.on) e.low_mask = 0;
     return CLIPVIT_OK;
 }
 
-int dz_blocks(int64_t M) { return (int)((M + 63) / 64 < 512 ? (M + 63) / 64 : 512); }
-int64_t dz_rows(int64_t M) { return up((M + dz_blocks(M) - 1) / (dz_blocks(M) ? dz_blocks(M) : 1), 8); }
+struct LinearGrad {
+    Matmul dx, dw;
+    Db dz;
+    bool want_dx, want_dw, changed;
+};
+int linear_grad_of(const clipvit_linear_grad_args* a, LinearGrad& g, Arena& ws, void*& part, void*& mm, size_t& mm_bytes) {
+    if (!a) FT_FAIL(CLIPVIT_E_INVALID, "null arguments");
+    if (const int rc = check_sizes("linear_grad", a->dtype, a->bias_dtype, a->M, a->N, a->K)) return rc;
+    if (bad_dropout(a->dropout)) FT_FAIL(CLIPVIT_E_INVALID, "dropout: p must lie in [0, 1]");
+    g.want_dx = a->dx && a->M && a->K;
+    g.want_dw = a->dw && a->N && a->K;
+    if (a->M && a->N && !a->dy) FT_FAIL(CLIPVIT_E_INVALID, "linear_grad: null dy");
+    if ((g.want_dx && a->N && !a->w) || (g.want_dw && a->M && !a->x)) FT_FAIL(CLIPVIT_E_INVALID, "linear_grad: null operand");
+    if (a->M > 1 && a->N && (a->dy_stride < a->N || a->dy_stride >= MATMUL_MAX_LD)) FT_FAIL(CLIPVIT_E_INVALID, "linear_grad: dy stride");
+    const Dropout drop = make_dropout(a->dropout);
+    g.changed = (a->slope || drop.on) && (g.want_dx || g.want_dw) && a->M && a->N;
+    const int64_t ld = g.changed ? up(a->N, 8) : a->dy_stride;
+    if (ld >= MATMUL_MAX_LD && (g.want_dx || g.want_dw) && a->M > 1) FT_FAIL(CLIPVIT_E_INVALID, "linear_grad: N too large");
+    void* dz = g.changed ? ws.take((size_t)a->M * ld * 2) : nullptr;
+    g.dz = make_dz(a->dy, a->dy_stride, a->slope, dz, ld, a->N ? a->db : nullptr, a->bias_dtype == CLIPVIT_F32, a->M, a->N, drop);
+    if (g.changed && !dz) g.dz.d.dz = (void*)256;  // counting the workspace: an aligned stand-in
+    part = ws.take(dz_part_bytes(g.dz));
+    const void* z = g.changed ? g.dz.d.dz : a->dy;
+    mm_bytes = 0;
+    if (g.want_dx) {
+        if (!make_matmul(g.dx, z, ld, 1, a->w, a->w_stride[1], a->w_stride[0], a->M, a->K, a->N, a->dx, a->K))
+            FT_FAIL(CLIPVIT_E_INVALID, std::string("linear_grad: ") + OPERANDS);
+        mm_bytes = matmul_workspace(g.dx);
+    }
+    if (g.want_dw) {
+        if (!make_matmul(g.dw, z, 1, ld, a->x, a->x_stride[1], a->x_stride[0], a->N, a->K, a->M, a->dw, a->K))
+            FT_FAIL(CLIPVIT_E_INVALID, std::string("linear_grad: ") + OPERANDS);
+        const size_t b = matmul_workspace(g.dw);
+        if (b > mm_bytes) mm_bytes = b;  // the two products run one after the other and share it
+    }
+    mm = ws.take(mm_bytes);
+    return CLIPVIT_OK;
+}
 
+// ---- LoRA Linear ----
+int64_t rank32(int64_t r) { return up(r, 32); }
+int check_lora(const char* what, int dtype, int bias_dtype, int64_t M, int64_t N, int64_t K, int64_t rank, const clipvit_dropout_args& d) {
+    if (const int rc = check_sizes(what, dtype, bias_dtype, M, N, K)) return rc;
+    if (rank < 1 || rank > 65536) FT_FAIL(CLIPVIT_E_INVALID, std::string(what) + ": rank must lie in [1, 65536]");
+    if (bad_dropout(d)) FT_FAIL(CLIPVIT_E_INVALID, "dropout: p must lie in [0, 1]");
+    return CLIPVIT_OK;
+}
+void launch_pad(hipStream_t s, const PadArgs& a, const PadArgs& b) {
+    const int64_t na = ((int64_t)a.I * a.J + 255) / 256, nb = ((int64_t)b.I * b.J + 255) / 256;
+    if (na + nb) pad_kernel<<<(unsigned)(na + nb), 256, 0, s>>>(a, b, (int)na);
+}
+void launch_down(hipStream_t s, bool bf, const void* x, int64_t ldx, const void* f, int64_t ldf, void* u, int64_t M, int64_t K, int64_t R,
+                 float alpha, const Dropout& drop) {
+    if (!M) return;
+    DownArgs d{};
+    d.x = (const u16*)x;
+    d.f = (const u16*)f;
+    d.u = (u16*)u;
+    d.ldx = M > 1 ? ldx : 0;
+    d.ldf = ldf;
+    d.M = (int)M;
+    d.K = (int)K;
+    d.R = (int)R;
+    d.vec = aligned16(x) && d.ldx % 8 == 0;
+    d.alpha = alpha;
+    d.d = drop;
+    const dim3 grid((unsigned)((M + 15) / 16), (unsigned)(R / 32));
+    if (bf) lora_down_kernel<BF16><<<grid, 256, 0, s>>>(d);
+    else lora_down_kernel<F16><<<grid, 256, 0, s>>>(d);
+}
 int grad_slices(int64_t M, int64_t C, int64_t R) {
     const int64_t wg = ((C + 127) / 128) * (R / 32);
     int64_t s = (1024 + wg - 1) / wg;
@@ -501,6 +626,121 @@ int grad_slices(int64_t M, int64_t C, int64_t R) {
     if (s > most) s = most;
     return (int)(s < 1 ? 1 : s);
 }
+size_t grad_bytes(int64_t M, int64_t C, int64_t R) { return C ? (size_t)grad_slices(M, C, R) * (size_t)R * (size_t)up(C, 4) * 4 : 0; }
+// out(c, r) = sum_m mask(x)[m, c] u[m, r], r < rank, at out + c so_c + r so_r
+void launch_grad(hipStream_t s, bool bf, const void* x, int64_t ldx, const void* u, void* out, int64_t so_c, int64_t so_r, int64_t M, int64_t C,
+                 int64_t R, int64_t rank, const Dropout& drop, void* part) {
+    if (!C) return;
+    GradArgs d{};
+    d.x = (const u16*)x;
+    d.u = (const u16*)u;
+    d.part = (float*)part;
+    d.ldx = M > 1 ? ldx : 0;
+    d.M = (int)M;
+    d.C = (int)C;
+    d.C4 = (int)up(C, 4);
+    d.R = (int)R;
+    d.vec = aligned16(x) && d.ldx % 8 == 0;
+    d.d = drop;
+    int slices = grad_slices(M, C, R);
+    d.rows = (int)up((M + slices - 1) / slices, 32);
+    slices = M ? (int)((M + d.rows - 1) / d.rows) : 0;
+    if (slices) {
+        const dim3 grid((unsigned)((C + 127) / 128), (unsigned)(R / 32), slices);
+        if (bf) lora_grad_kernel<BF16><<<grid, 256, 0, s>>>(d);
+        else lora_grad_kernel<F16><<<grid, 256, 0, s>>>(d);
+    }
+    const unsigned g = (unsigned)((rank * C + 255) / 256);
+    if (bf) lora_grad_join_kernel<BF16><<<g, 256, 0, s>>>(d.part, slices, d.R, d.C, d.C4, (int)rank, (u16*)out, so_c, so_r);
+    else lora_grad_join_kernel<F16><<<g, 256, 0, s>>>(d.part, slices, d.R, d.C, d.C4, (int)rank, (u16*)out, so_c, so_r);
+}
+PadArgs pad_of(const void* src, int64_t s0, int64_t s1, int64_t ri, int64_t rj, int64_t I, int64_t J, void* dst) {
+    return PadArgs{(const u16*)src, s0, s1, (int)ri, (int)rj, (int)I, (int)J, (u16*)dst};
+}
+
+struct Lora {
+    Matmul y;
+    void *f, *v, *mm;
+    size_t mm_bytes;
+};
+int lora_of(const clipvit_lora_args* a, Lora& l, Arena& ws) {
+    if (!a) FT_FAIL(CLIPVIT_E_INVALID, "null arguments");
+    if (const int rc = check_lora("lora_linear", a->dtype, a->bias_dtype, a->M, a->N, a->K, a->rank, a->dropout)) return rc;
+    const int64_t R = rank32(a->rank);
+    if (a->M && a->N) {
+        if (!a->y || !a->u || !aligned16(a->u) || !a->b || (a->K && (!a->x || !a->w || !a->a)))
+            FT_FAIL(CLIPVIT_E_INVALID, "lora_linear: null or misaligned operand");
+        if (a->M > 1 && a->x_stride < a->K) FT_FAIL(CLIPVIT_E_INVALID, "lora_linear: x rows overlap");
+    }
+    if (!make_matmul(l.y, a->x, a->x_stride, 1, a->w, a->w_stride[0], a->w_stride[1], a->M, a->N, a->K, a->y, a->N))
+        FT_FAIL(CLIPVIT_E_INVALID, std::string("lora_linear: ") + OPERANDS);
+    l.f = ws.take((size_t)R * up(a->K, 32) * 2);
+    l.v = ws.take((size_t)a->N * R * 2);
+    Epilogue& e = l.y.e;
+    e.bias = a->bias;
+    e.bias_f32 = a->bias_dtype == CLIPVIT_F32;
+    e.lu = (const u16*)a->u;
+    e.lv = (const u16*)l.v;
+    e.R = (int)R;
+    l.mm_bytes = matmul_workspace(l.y);
+    l.mm = ws.take(l.mm_bytes);
+    return CLIPVIT_OK;
+}
+
+struct LoraGrad {
+    Matmul dx, dw;
+    Db db;
+    bool want_dx, want_dw, want_du;
+    void *f, *v, *du, *grad, *part, *mm;
+    size_t mm_bytes;
+};
+int lora_grad_of(const clipvit_lora_grad_args* a, LoraGrad& g, Arena& ws) {
+    if (!a) FT_FAIL(CLIPVIT_E_INVALID, "null arguments");
+    if (const int rc = check_lora("lora_linear_grad", a->dtype, a->bias_dtype, a->M, a->N, a->K, a->rank, a->dropout)) return rc;
+    const int64_t R = rank32(a->rank);
+    g.want_dx = a->dx && a->M && a->K;
+    g.want_dw = a->dw && a->N && a->K;
+    g.want_du = g.want_dx || (a->da && a->K);
+    if (a->M && a->N && !a->dy) FT_FAIL(CLIPVIT_E_INVALID, "lora_linear_grad: null dy");
+    if ((g.want_dx && a->N && !a->w) || (g.want_dx && !a->a) || (g.want_du && a->N && !a->b) || ((g.want_dw || a->da) && a->M && a->K && !a->x) ||
+        (a->db_factor && a->M && (!a->u || !aligned16(a->u))))
+        FT_FAIL(CLIPVIT_E_INVALID, "lora_linear_grad: null or misaligned operand");
+    if (a->M > 1 && ((a->N && (a->dy_stride < a->N || a->dy_stride >= MATMUL_MAX_LD)) || a->x_stride < a->K))
+        FT_FAIL(CLIPVIT_E_INVALID, "lora_linear_grad: row stride");
+    const Dropout none{};
+    if (g.want_du) {
+        g.f = ws.take((size_t)R * up(a->N, 32) * 2);
+        g.v = ws.take((size_t)a->K * R * 2);
+        g.du = ws.take((size_t)a->M * R * 2);
+    }
+    const size_t ga = a->da ? grad_bytes(a->M, a->K, R) : 0, gb = a->db_factor ? grad_bytes(a->M, a->N, R) : 0;
+    g.grad = ws.take(ga > gb ? ga : gb);
+    g.db = make_dz(a->dy, a->dy_stride, nullptr, nullptr, 8, a->N ? a->dbias : nullptr, a->bias_dtype == CLIPVIT_F32, a->M, a->N, none);
+    g.part = ws.take(dz_part_bytes(g.db));
+    g.mm_bytes = 0;
+    if (g.want_dx) {
+        if (!make_matmul(g.dx, a->dy, a->dy_stride, 1, a->w, a->w_stride[1], a->w_stride[0], a->M, a->K, a->N, a->dx, a->K))
+            FT_FAIL(CLIPVIT_E_INVALID, std::string("lora_linear_grad: ") + OPERANDS);
+        Epilogue& e = g.dx.e;
+        e.lu = (const u16*)g.du;
+        e.lv = (const u16*)g.v;
+        e.R = (int)R;
+        e.drop = make_dropout(a->dropout);
+        e.low_mask = e.drop.on;
+        g.mm_bytes = matmul_workspace(g.dx);
+    }
+    if (g.want_dw) {
+        if (!make_matmul(g.dw, a->dy, 1, a->dy_stride, a->x, 1, a->x_stride, a->N, a->K, a->M, a->dw, a->K))
+            FT_FAIL(CLIPVIT_E_INVALID, std::string("lora_linear_grad: ") + OPERANDS);
+        const size_t b = matmul_workspace(g.dw);
+        if (b > g.mm_bytes) g.mm_bytes = b;
+    }
+    g.mm = ws.take(g.mm_bytes);
+    return CLIPVIT_OK;
+}
+
+bool bad_workspace(const Arena& need, const void* ws, size_t bytes) { return need.used > bytes || (need.used && (!ws || ((size_t)ws & 255))); }
+const char* const WORKSPACE = "workspace too small or not 256-byte aligned (ask the call's _workspace)";
 
 template <typename F>
 int guarded(F&& f) noexcept {
@@ -525,10 +765,9 @@ extern "C" {
 
 int clipvit_linear_workspace(const clipvit_linear_args* a, size_t* bytes) {
     return guarded([&]() -> int {
-        Matmul m{};
+        Matmul m;
         if (!bytes) FT_FAIL(CLIPVIT_E_INVALID, "null argument");
-        const int rc = matmul_of(a, m);
-        if (rc) return rc;
+        if (const int rc = linear_of(a, m)) return rc;
         *bytes = matmul_workspace(m);
         return CLIPVIT_OK;
     });
@@ -536,58 +775,46 @@ int clipvit_linear_workspace(const clipvit_linear_args* a, size_t* bytes) {
 
 int clipvit_linear(void* stream, const clipvit_linear_args* a, void* workspace, size_t bytes) {
     return guarded([&]() -> int {
-        Matmul m{};
-        const int rc = matmul_of(a, m);
-        if (rc) return rc;
-        if (matmul_workspace(m) > bytes || (bytes && !workspace) || ((size_t)workspace & 255))
-            FT_FAIL(CLIPVIT_E_INVALID, "linear: workspace too small or not 256-byte aligned (clipvit_linear_workspace)");
+        Matmul m;
+        if (const int rc = linear_of(a, m)) return rc;
         if (!m.M || !m.N) return CLIPVIT_OK;
-        if (launch_matmul((hipStream_t)stream, a->dtype, m, workspace, bytes)) FT_FAIL(CLIPVIT_E_INVALID, "linear: workspace");
+        if ((bytes && !workspace) || ((size_t)workspace & 255) || launch_matmul((hipStream_t)stream, a->dtype, m, workspace, bytes))
+            FT_FAIL(CLIPVIT_E_INVALID, std::string("linear: ") + WORKSPACE);
         FT_LAUNCHED();
         return CLIPVIT_OK;
     });
 }
 
-int clipvit_linear_dz(void* stream, const clipvit_dz_args* a, void* workspace, size_t bytes) {
+int clipvit_linear_grad_workspace(const clipvit_linear_grad_args* a, size_t* bytes) {
     return guarded([&]() -> int {
-        if (!a) FT_FAIL(CLIPVIT_E_INVALID, "null arguments");
-        if (!is16(a->dtype)) FT_FAIL(CLIPVIT_E_INVALID, "linear_dz: dtype must be BF16 or F16");
-        if (a->db_dtype != CLIPVIT_F32 && a->db_dtype != a->dtype) FT_FAIL(CLIPVIT_E_INVALID, "linear_dz: db must be F32 or of dy's type");
-        if (a->M < 0 || a->N < 0 || a->M > MAX_DIM || a->N > MAX_DIM) FT_FAIL(CLIPVIT_E_INVALID, "linear_dz: M and N must lie in [0, 2^30]");
-        if (bad_dropout(a->dropout)) FT_FAIL(CLIPVIT_E_INVALID, "dropout: p must lie in [0, 1]");
-        if (a->N == 0) return CLIPVIT_OK;
-        if (a->M && !a->dy) FT_FAIL(CLIPVIT_E_INVALID, "linear_dz: null dy");
-        if (a->M > 1 && (a->dy_stride < 0 || (a->dz && a->dz_stride < a->N))) FT_FAIL(CLIPVIT_E_INVALID, "linear_dz: row stride");
-        const int blocks = dz_blocks(a->M);
-        const size_t need = a->db ? (size_t)blocks * a->N * 4 : 0;
-        if (bytes < need || (need && !workspace) || ((size_t)workspace & 15))
-            FT_FAIL(CLIPVIT_E_INVALID, "linear_dz: workspace of 4 N ceil(M / 64) bytes (at most 512 blocks), 16-byte aligned");
-        DzArgs d{};
-        d.dy = a->dy;
-        d.slope = a->slope;
-        d.dz = a->dz;
-        d.part = a->db ? (float*)workspace : nullptr;
-        d.lddy = a->M > 1 ? a->dy_stride : up(a->N, 8);
-        d.lddz = a->M > 1 ? a->dz_stride : up(a->N, 8);
-        d.M = (int)a->M;
-        d.N = (int)a->N;
-        d.rows = (int)dz_rows(a->M);
-        d.d = make_dropout(a->dropout);
-        d.vec = aligned16(d.dy) && d.lddy % 8 == 0 && aligned16(d.dz) && d.lddz % 8 == 0 && aligned16(d.slope) && (!d.slope || d.N % 8 == 0);
-        if (!d.dz) d.vec = aligned16(d.dy) && d.lddy % 8 == 0 && aligned16(d.slope) && (!d.slope || d.N % 8 == 0);
+        if (!bytes) FT_FAIL(CLIPVIT_E_INVALID, "null argument");
+        LinearGrad g{};
+        Arena count{nullptr};
+        void *part, *mm;
+        size_t mm_bytes;
+        if (const int rc = linear_grad_of(a, g, count, part, mm, mm_bytes)) return rc;
+        *bytes = count.used;
+        return CLIPVIT_OK;
+    });
+}
+
+int clipvit_linear_grad(void* stream, const clipvit_linear_grad_args* a, void* workspace, size_t bytes) {
+    return guarded([&]() -> int {
+        LinearGrad g{};
+        Arena ws{(unsigned char*)workspace};
+        void *part, *mm;
+        size_t mm_bytes;
+        if (const int rc = linear_grad_of(a, g, ws, part, mm, mm_bytes)) return rc;
+        if (bad_workspace(ws, workspace, bytes)) FT_FAIL(CLIPVIT_E_INVALID, std::string("linear_grad: ") + WORKSPACE);
         hipStream_t s = (hipStream_t)stream;
-        const bool bf = a->dtype == CLIPVIT_BF16;
-        if (blocks) {
-            const dim3 grid((d.N + 255) / 256, blocks);
-            if (bf) dz_kernel<BF16T><<<grid, 256, 0, s>>>(d);
-            else dz_kernel<F16T><<<grid, 256, 0, s>>>(d);
+        bool any = false;
+        if (g.changed || g.dz.db) {
+            launch_dz(s, a->dtype == CLIPVIT_BF16, g.dz, part);
+            any = true;
         }
-        if (a->db) {
-            const int g = (d.N + 31) / 32;
-            if (bf) db_kernel<BF16T><<<g, 256, 0, s>>>(d.part, blocks, d.N, a->db, a->db_dtype == CLIPVIT_F32);
-            else db_kernel<F16T><<<g, 256, 0, s>>>(d.part, blocks, d.N, a->db, a->db_dtype == CLIPVIT_F32);
-        }
-        FT_LAUNCHED();
+        if ((g.want_dx && launch_matmul(s, a->dtype, g.dx, mm, mm_bytes)) || (g.want_dw && launch_matmul(s, a->dtype, g.dw, mm, mm_bytes)))
+            FT_FAIL(CLIPVIT_E_INVALID, std::string("linear_grad: ") + WORKSPACE);
+        if (any || g.want_dx || g.want_dw) FT_LAUNCHED();
         return CLIPVIT_OK;
     });
 }
@@ -633,108 +860,67 @@ int clipvit_dropout(void* stream, int dtype, const void* x, int64_t x_stride, co
     });
 }
 
-int clipvit_lora_pad(void* stream, const clipvit_pad_args* a, const clipvit_pad_args* b) {
+int clipvit_lora_linear_workspace(const clipvit_lora_args* a, size_t* bytes) {
     return guarded([&]() -> int {
-        PadArgs p[2]{};
-        unsigned blocks[2] = {0, 0};
-        const clipvit_pad_args* in[2] = {a, b};
-        for (int i = 0; i < 2; ++i) {
-            const clipvit_pad_args* q = in[i];
-            if (!q) continue;
-            if (q->rows < 0 || q->cols < 0 || q->rows_padded < q->rows || q->cols_padded < q->cols || q->rows_padded > MAX_DIM ||
-                q->cols_padded > MAX_DIM)
-                FT_FAIL(CLIPVIT_E_INVALID, "lora_pad: sizes");
-            const int64_t n = q->rows_padded * q->cols_padded;
-            if (!n) continue;
-            if (n > (int64_t)1 << 38) FT_FAIL(CLIPVIT_E_INVALID, "lora_pad: sizes");
-            if ((!q->src && q->rows && q->cols) || !q->dst) FT_FAIL(CLIPVIT_E_INVALID, "lora_pad: null argument");
-            p[i] = PadArgs{(const u16*)q->src, q->row_stride, q->col_stride, (int)q->rows, (int)q->cols, (int)q->rows_padded,
-                           (int)q->cols_padded, (u16*)q->dst};
-            blocks[i] = (unsigned)((n + 255) / 256);
-        }
-        if (blocks[0] + blocks[1] == 0) return CLIPVIT_OK;
-        pad_kernel<<<blocks[0] + blocks[1], 256, 0, (hipStream_t)stream>>>(p[0], p[1], (int)blocks[0]);
-        FT_LAUNCHED();
+        if (!bytes) FT_FAIL(CLIPVIT_E_INVALID, "null argument");
+        Lora l{};
+        Arena count{nullptr};
+        if (const int rc = lora_of(a, l, count)) return rc;
+        *bytes = count.used;
         return CLIPVIT_OK;
     });
 }
 
-int clipvit_lora_down(void* stream, int dtype, const void* x, int64_t x_stride, const void* f, int64_t f_stride, void* u, int64_t M, int64_t K,
-                      int64_t R, float alpha, const clipvit_dropout_args* dropout) {
+int clipvit_lora_linear(void* stream, const clipvit_lora_args* a, void* workspace, size_t bytes) {
     return guarded([&]() -> int {
-        if (!dropout || bad_dropout(*dropout)) FT_FAIL(CLIPVIT_E_INVALID, "dropout: p must lie in [0, 1]");
-        if (!is16(dtype)) FT_FAIL(CLIPVIT_E_INVALID, "lora_down: dtype must be BF16 or F16");
-        if (M < 0 || K < 0 || R < 0 || R % 32 || M > MAX_DIM || K > MAX_DIM || R > 65536) FT_FAIL(CLIPVIT_E_INVALID, "lora_down: sizes");
-        if (!M || !R) return CLIPVIT_OK;
-        if (!u || (K && (!x || !f))) FT_FAIL(CLIPVIT_E_INVALID, "lora_down: null argument");
-        if (!aligned16(f) || f_stride % 8 || f_stride < up(K, 32) || !aligned16(u)) FT_FAIL(CLIPVIT_E_INVALID, "lora_down: factor rows must be 16-byte aligned, zero padded to 32");
-        if (M > 1 && x_stride < 0) FT_FAIL(CLIPVIT_E_INVALID, "lora_down: row stride");
-        DownArgs d{};
-        d.x = (const u16*)x;
-        d.f = (const u16*)f;
-        d.u = (u16*)u;
-        d.ldx = M > 1 ? x_stride : 0;
-        d.ldf = f_stride;
-        d.M = (int)M;
-        d.K = (int)K;
-        d.R = (int)R;
-        d.vec = aligned16(x) && d.ldx % 8 == 0;
-        d.alpha = alpha;
-        d.d = make_dropout(*dropout);
-        const dim3 grid((unsigned)((M + 15) / 16), (unsigned)(R / 32));
-        if (dtype == CLIPVIT_BF16) lora_down_kernel<BF16><<<grid, 256, 0, (hipStream_t)stream>>>(d);
-        else lora_down_kernel<F16><<<grid, 256, 0, (hipStream_t)stream>>>(d);
-        FT_LAUNCHED();
-        return CLIPVIT_OK;
-    });
-}
-
-int clipvit_lora_grad_workspace(int64_t M, int64_t C, int64_t R, size_t* bytes) {
-    return guarded([&]() -> int {
-        if (!bytes || M < 0 || C < 0 || R < 0 || R % 32 || M > MAX_DIM || C > MAX_DIM || R > 65536) FT_FAIL(CLIPVIT_E_INVALID, "lora_grad: sizes");
-        *bytes = C && R ? (size_t)grad_slices(M, C, R) * (size_t)R * (size_t)up(C, 4) * 4 : 0;
-        return CLIPVIT_OK;
-    });
-}
-
-int clipvit_lora_grad(void* stream, int dtype, const void* x, int64_t x_stride, const void* u, void* out, int64_t out_col_stride,
-                      int64_t out_rank_stride, int64_t M, int64_t C, int64_t R, int64_t rank, const clipvit_dropout_args* dropout, void* workspace,
-                      size_t bytes) {
-    return guarded([&]() -> int {
-        if (!dropout || bad_dropout(*dropout)) FT_FAIL(CLIPVIT_E_INVALID, "dropout: p must lie in [0, 1]");
-        if (!is16(dtype)) FT_FAIL(CLIPVIT_E_INVALID, "lora_grad: dtype must be BF16 or F16");
-        size_t need = 0;
-        const int rc = clipvit_lora_grad_workspace(M, C, R, &need);
-        if (rc) return rc;
-        if (rank < 0 || rank > R) FT_FAIL(CLIPVIT_E_INVALID, "lora_grad: rank");
-        if (!C || !rank) return CLIPVIT_OK;
-        if (!out || (M && (!x || !u || !aligned16(u)))) FT_FAIL(CLIPVIT_E_INVALID, "lora_grad: null or misaligned argument");
-        if (M > 1 && x_stride < 0) FT_FAIL(CLIPVIT_E_INVALID, "lora_grad: row stride");
-        if (bytes < need || !workspace || !aligned16(workspace)) FT_FAIL(CLIPVIT_E_INVALID, "lora_grad: workspace too small or misaligned (clipvit_lora_grad_workspace)");
-        GradArgs d{};
-        d.x = (const u16*)x;
-        d.u = (const u16*)u;
-        d.part = (float*)workspace;
-        d.ldx = M > 1 ? x_stride : 0;
-        d.M = (int)M;
-        d.C = (int)C;
-        d.C4 = (int)up(C, 4);
-        d.R = (int)R;
-        d.vec = aligned16(x) && d.ldx % 8 == 0;
-        d.d = make_dropout(*dropout);
-        int slices = grad_slices(M, C, R);
-        d.rows = (int)up((M + slices - 1) / slices, 32);
-        slices = M ? (int)((M + d.rows - 1) / d.rows) : 0;
+        Lora l{};
+        Arena ws{(unsigned char*)workspace};
+        if (const int rc = lora_of(a, l, ws)) return rc;
+        if (!a->M || !a->N) return CLIPVIT_OK;
+        if (bad_workspace(ws, workspace, bytes)) FT_FAIL(CLIPVIT_E_INVALID, std::string("lora_linear: ") + WORKSPACE);
         hipStream_t s = (hipStream_t)stream;
-        const bool bf = dtype == CLIPVIT_BF16;
-        if (slices) {
-            const dim3 grid((unsigned)((C + 127) / 128), (unsigned)(R / 32), slices);
-            if (bf) lora_grad_kernel<BF16><<<grid, 256, 0, s>>>(d);
-            else lora_grad_kernel<F16><<<grid, 256, 0, s>>>(d);
+        const int64_t R = rank32(a->rank), Kp = up(a->K, 32);
+        const Dropout drop = make_dropout(a->dropout);
+        launch_pad(s, pad_of(a->a, a->a_stride[1], a->a_stride[0], a->rank, a->K, R, Kp, l.f),
+                   pad_of(a->b, a->b_stride[1], a->b_stride[0], a->N, a->rank, a->N, R, l.v));
+        launch_down(s, a->dtype == CLIPVIT_BF16, a->x, a->x_stride, l.f, Kp, a->u, a->M, a->K, R, a->scaling * (drop.on ? drop.scale : 1.f), drop);
+        if (launch_matmul(s, a->dtype, l.y, l.mm, l.mm_bytes)) FT_FAIL(CLIPVIT_E_INVALID, std::string("lora_linear: ") + WORKSPACE);
+        FT_LAUNCHED();
+        return CLIPVIT_OK;
+    });
+}
+
+int clipvit_lora_linear_grad_workspace(const clipvit_lora_grad_args* a, size_t* bytes) {
+    return guarded([&]() -> int {
+        if (!bytes) FT_FAIL(CLIPVIT_E_INVALID, "null argument");
+        LoraGrad g{};
+        Arena count{nullptr};
+        if (const int rc = lora_grad_of(a, g, count)) return rc;
+        *bytes = count.used;
+        return CLIPVIT_OK;
+    });
+}
+
+int clipvit_lora_linear_grad(void* stream, const clipvit_lora_grad_args* a, void* workspace, size_t bytes) {
+    return guarded([&]() -> int {
+        LoraGrad g{};
+        Arena ws{(unsigned char*)workspace};
+        if (const int rc = lora_grad_of(a, g, ws)) return rc;
+        if (bad_workspace(ws, workspace, bytes)) FT_FAIL(CLIPVIT_E_INVALID, std::string("lora_linear_grad: ") + WORKSPACE);
+        hipStream_t s = (hipStream_t)stream;
+        const bool bf = a->dtype == CLIPVIT_BF16;
+        const int64_t R = rank32(a->rank), Np = up(a->N, 32);
+        const Dropout drop = make_dropout(a->dropout), none{};
+        if (g.want_du) {
+            launch_pad(s, pad_of(a->b, a->b_stride[0], a->b_stride[1], a->rank, a->N, R, Np, g.f),
+                       pad_of(a->a, a->a_stride[0], a->a_stride[1], a->K, a->rank, g.want_dx ? a->K : 0, R, g.v));
+            launch_down(s, bf, a->dy, a->dy_stride, g.f, Np, g.du, a->M, a->N, R, a->scaling * (drop.on ? drop.scale : 1.f), none);
+            if (g.want_dx && launch_matmul(s, a->dtype, g.dx, g.mm, g.mm_bytes)) FT_FAIL(CLIPVIT_E_INVALID, std::string("lora_linear_grad: ") + WORKSPACE);
+            if (a->da) launch_grad(s, bf, a->x, a->x_stride, g.du, a->da, a->rank, 1, a->M, a->K, R, a->rank, drop, g.grad);
         }
-        const unsigned g = (unsigned)((rank * C + 255) / 256);
-        if (bf) lora_grad_join_kernel<BF16><<<g, 256, 0, s>>>(d.part, slices, d.R, d.C, d.C4, (int)rank, (u16*)out, out_col_stride, out_rank_stride);
-        else lora_grad_join_kernel<F16><<<g, 256, 0, s>>>(d.part, slices, d.R, d.C, d.C4, (int)rank, (u16*)out, out_col_stride, out_rank_stride);
+        if (a->db_factor) launch_grad(s, bf, a->dy, a->dy_stride, a->u, a->db_factor, 1, a->N, a->M, a->N, R, a->rank, none, g.grad);
+        if (g.want_dw && launch_matmul(s, a->dtype, g.dw, g.mm, g.mm_bytes)) FT_FAIL(CLIPVIT_E_INVALID, std::string("lora_linear_grad: ") + WORKSPACE);
+        if (g.db.db) launch_dz(s, bf, g.db, g.part);
         FT_LAUNCHED();
         return CLIPVIT_OK;
     });

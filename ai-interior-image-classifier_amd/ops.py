@@ -25,6 +25,7 @@ into a graph through ``torch.autograd.grad`` after the usual warm-up on a side s
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -107,6 +108,12 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 _MAX_LD = 1 << 22
 
 
+def _rows_ld(t: torch.Tensor) -> torch.Tensor:
+    """_rows with a row stride that the matrix products address (below 2^22, or one row)."""
+    t = _rows(t)
+    return t.contiguous() if t.shape[0] > 1 and t.stride(0) >= _MAX_LD else t
+
+
 def _panel(t: torch.Tensor) -> torch.Tensor:
     """A matrix operand: one unit stride, rows (or columns) that do not overlap, the other stride below 2^22."""
     r, c = t.shape
@@ -118,113 +125,73 @@ def _panel(t: torch.Tensor) -> torch.Tensor:
     return t.contiguous()
 
 
-class _On:
-    """The tensors' device as the current one (a no-op where it is already), and its current stream."""
+def _stream(index: int):
+    """The current stream of a device as the C entry points take it."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
-    def __init__(self, dev: torch.device):
-        self.index = dev.index
-        self.prev = torch.cuda.current_device()
+
+class _On:
+    """The tensors' device as the current one while kernels are launched; entered only where it is not already."""
+
+    def __init__(self, index: int):
+        self.index, self.prev = index, torch.cuda.current_device()
 
     def __enter__(self):
-        if self.prev != self.index:
-            torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream(self.index).cuda_stream
+        torch.cuda.set_device(self.index)
 
     def __exit__(self, *exc):
-        if self.prev != self.index:
-            torch.cuda.set_device(self.prev)
+        torch.cuda.set_device(self.prev)
 
 
-def _workspace(nbytes: int, dev: torch.device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+def _launch(name: str, index: int, args, ws, nbytes: int) -> None:
+    fn = getattr(_lib.lib(), name)
+    ptr = ws.data_ptr() if nbytes else None
+    if torch.cuda.current_device() == index:
+        rc = fn(_stream(index), _byref(args), ptr, nbytes)
+    else:
+        with _On(index):
+            rc = fn(_stream(index), _byref(args), ptr, nbytes)
+    if rc:
+        _lib.check(rc)
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-# ---------------------------------------------------------------- calls of the C entry points
-def _matmul(stream, x, w, *, bias=None, residual=None, act=0, slope=None, low=None, low_mask=False,
-            drop=_NO_DROPOUT) -> torch.Tensor:
-    """[M, N] of x [M, K] and w [N, K] views through clipvit_linear."""
-    L = _lib.lib()
-    x, w = _panel(x), _panel(w)
-    M, K = x.shape
-    N = w.shape[0]
-    y = torch.empty((M, N), dtype=x.dtype, device=x.device)
-    a = _lib.LinearArgs()
-    a.dtype, a.activation, a.low_mask = _DT[x.dtype], act, int(low_mask)
-    a.bias_dtype = a.dtype if bias is None else _DT[bias.dtype]
-    a.M, a.N, a.K = M, N, K
-    a.x, a.w, a.y = x.data_ptr(), w.data_ptr(), y.data_ptr()
-    a.x_stride[0], a.x_stride[1] = x.stride()
-    a.w_stride[0], a.w_stride[1] = w.stride()
-    a.y_stride = N
-    a.bias = _ptr(bias)
-    if residual is not None:
-        a.residual, a.residual_stride = residual.data_ptr(), residual.stride(0)
-    a.slope = _ptr(slope)
-    if low is not None:
-        u, v = low
-        a.R, a.low_u, a.low_v = u.shape[1], u.data_ptr(), v.data_ptr()
-    a.dropout = drop
+def _bytes(name: str, args) -> int:
     need = ctypes.c_size_t()
-    _lib.check(L.clipvit_linear_workspace(_byref(a), _byref(need)))
-    ws = _workspace(need.value, x.device)
-    _lib.check(L.clipvit_linear(stream, _byref(a), _ptr(ws), need.value))
-    return y
+    _lib.check(getattr(_lib.lib(), name)(_byref(args), _byref(need)))
+    return need.value
 
 
-def _dz(stream, dy, slope, drop, want_dz: bool, db_dtype):
-    """(dz or None, db or None) of dy [M, N] through clipvit_linear_dz."""
-    M, N = dy.shape
-    ld = (N + 7) // 8 * 8  # rows that 16-byte loads can address, whatever N is
-    dz = torch.empty((M, ld), dtype=dy.dtype, device=dy.device)[:, :N] if want_dz else None
-    db = torch.empty(N, dtype=db_dtype, device=dy.device) if db_dtype is not None else None
-    a = _lib.DzArgs()
-    a.dtype = _DT[dy.dtype]
-    a.db_dtype = a.dtype if db is None else _DT[db_dtype]
-    a.M, a.N, a.dy, a.dy_stride = M, N, dy.data_ptr(), dy.stride(0)
-    a.slope, a.dz, a.dz_stride, a.db, a.dropout = _ptr(slope), _ptr(dz), ld, _ptr(db), drop
-    need = 4 * N * min(512, (M + 63) // 64) if db is not None else 0
-    ws = _workspace(need, dy.device)
-    _lib.check(_lib.lib().clipvit_linear_dz(stream, _byref(a), _ptr(ws), need))
-    return dz, db
+# Workspace sizes by sizes, strides, alignments and wanted outputs, which is all they depend on (pointers are
+# stand-ins of the same alignment).
+@functools.lru_cache(maxsize=4096)
+def _linear_bytes(dt, m, n, k, x0, x1, xa, w0, w1, wa) -> int:
+    return _bytes("clipvit_linear_workspace", _lib.LinearArgs(
+        dt, 0, dt, 0, m, n, k, 4096 + xa, x0, x1, 4096 + wa, w0, w1, None, None, 0, 4096, n, None, _NO_DROPOUT))
 
 
-def _pad(stream, *factors):
-    """Zero-padded contiguous copies of one or two 16-bit factors: (view, rows, cols) each."""
-    out, args = [], []
-    for t, rows, cols in factors:
-        d = torch.empty((rows, cols), dtype=t.dtype, device=t.device)
-        out.append(d)
-        args.append(_lib.PadArgs(t.data_ptr(), t.stride(0), t.stride(1), t.shape[0], t.shape[1], rows, cols, d.data_ptr()))
-    _lib.check(_lib.lib().clipvit_lora_pad(stream, _byref(args[0]), _byref(args[1]) if len(args) > 1 else None))
-    return out
+@functools.lru_cache(maxsize=4096)
+def _linear_grad_bytes(dt, bdt, m, n, k, d0, da, x0, x1, xa, w0, w1, wa, slope, dx, dw, db, p) -> int:
+    return _bytes("clipvit_linear_grad_workspace", _lib.LinearGradArgs(
+        dt, bdt, m, n, k, 4096 + da, d0, 4096 + xa, x0, x1, 4096 + wa, w0, w1, 4096 if slope else None,
+        4096 if dx else None, 4096 if dw else None, 4096 if db else None, _lib.DropoutArgs(p, 0, 0, None)))
 
 
-def _down(stream, x, f, alpha: float, drop) -> torch.Tensor:
-    """u [M, R] = alpha mask(x) f^T."""
-    M, K = x.shape
-    u = torch.empty((M, f.shape[0]), dtype=x.dtype, device=x.device)
-    _lib.check(_lib.lib().clipvit_lora_down(stream, _DT[x.dtype], x.data_ptr(), x.stride(0), f.data_ptr(), f.stride(0),
-                                            u.data_ptr(), M, K, f.shape[0], alpha, _byref(drop)))
-    return u
+@functools.lru_cache(maxsize=4096)
+def _lora_bytes(dt, m, n, k, r, x0, xa, w0, w1, wa) -> int:
+    return _bytes("clipvit_lora_linear_workspace", _lib.LoraArgs(
+        dt, dt, m, n, k, r, 4096 + xa, x0, 4096 + wa, w0, w1, 4096, r, 1, 4096, n, 1, None, 4096, 4096, 1.0, 0.0, _NO_DROPOUT))
 
 
-def _low_grad(stream, x, u, rank: int, transposed: bool, drop) -> torch.Tensor:
-    """[C, rank] (or [rank, C]) = mask(x)^T u."""
-    L = _lib.lib()
-    M, C = x.shape
-    R = u.shape[1]
-    out = torch.empty((rank, C) if transposed else (C, rank), dtype=x.dtype, device=x.device)
-    need = ctypes.c_size_t()
-    _lib.check(L.clipvit_lora_grad_workspace(M, C, R, _byref(need)))
-    ws = _workspace(need.value, x.device)
-    sc, sr = (1, C) if transposed else (rank, 1)
-    _lib.check(L.clipvit_lora_grad(stream, _DT[x.dtype], x.data_ptr(), x.stride(0), u.data_ptr(), out.data_ptr(), sc, sr,
-                                   M, C, R, rank, _byref(drop), _ptr(ws), need.value))
-    return out
+@functools.lru_cache(maxsize=4096)
+def _lora_grad_bytes(dt, bdt, m, n, k, r, d0, da, x0, xa, w0, w1, wa, dx, dw, dA, dB, db, p) -> int:
+    return _bytes("clipvit_lora_linear_grad_workspace", _lib.LoraGradArgs(
+        dt, bdt, m, n, k, r, 4096 + da, d0, 4096 + xa, x0, 4096 + wa, w0, w1, 4096, r, 1, 4096, n, 1, 4096,
+        4096 if dx else None, 4096 if dw else None, 4096 if dA else None, 4096 if dB else None, 4096 if db else None, 1.0, 0.0,
+        _lib.DropoutArgs(p, 0, 0, None)))
 
 
 def _wants_grad(*tensors) -> bool:
@@ -232,47 +199,54 @@ def _wants_grad(*tensors) -> bool:
 
 
 # ---------------------------------------------------------------- linear
-def _linear_forward(x2, weight, bias, res2, act, p, seed, offset, save):
-    with _On(x2.device) as stream:
-        slope = None
-        if save and act:
-            slope = torch.empty((x2.shape[0], weight.shape[0]), dtype=torch.int16, device=x2.device)
-        y = _matmul(stream, x2, weight, bias=bias, residual=res2, act=act, slope=slope,
-                    drop=_dropout_args(p, seed, offset))
+def _linear_forward(x2, weight, bias, res2, act, drop, save):
+    """(y [M, N], act'(z) or None) of x2 [M, K]."""
+    x2, weight = _panel(x2), _panel(weight)
+    (m, k), n, dt = x2.shape, weight.shape[0], _DT[x2.dtype]
+    (x0, x1), (w0, w1), xp, wp = x2.stride(), weight.stride(), x2.data_ptr(), weight.data_ptr()
+    y = x2.new_empty((m, n))
+    slope = torch.empty((m, n), dtype=torch.int16, device=x2.device) if save and act else None
+    need = _linear_bytes(dt, m, n, k, x0, x1, xp & 15, w0, w1, wp & 15)
+    ws = torch.empty(need, dtype=torch.uint8, device=x2.device) if need else None
+    _launch("clipvit_linear", x2.device.index, _lib.LinearArgs(
+        dt, act, dt if bias is None else _DT[bias.dtype], 0, m, n, k, xp, x0, x1, wp, w0, w1, _ptr(bias), _ptr(res2),
+        0 if res2 is None else res2.stride(0), y.data_ptr(), n, _ptr(slope), drop), ws, need)
     return y, slope
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, p, seed, offset):
-        x2 = _rows(x)
-        res2 = None if residual is None else _rows(residual)
-        save = ctx.needs_input_grad[0] or ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        y, slope = _linear_forward(x2, weight, bias, res2, act, p, seed, offset, save)
+        needs = ctx.needs_input_grad
+        drop = _dropout_args(p, seed, offset)
+        y, slope = _linear_forward(_rows(x), weight, bias, None if residual is None else _rows(residual), act, drop,
+                                   needs[0] or needs[1] or needs[2])
+        # (the offset is saved so that autograd notices when it changes before the backward pass)
         ctx.save_for_backward(x, weight, slope, offset if torch.is_tensor(offset) else None)
-        ctx.bias_dtype = None if bias is None else bias.dtype
-        ctx.p, ctx.seed, ctx.offset = p, seed, None if torch.is_tensor(offset) else offset
+        ctx.drop, ctx.bias_dtype = drop, None if bias is None else bias.dtype
         return y.view(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weight, slope, off = ctx.saved_tensors
+        x, weight, slope, _ = ctx.saved_tensors
         nx, nw, nb, nr = ctx.needs_input_grad[:4]
         dx = dw = db = None
         if nx or nw or nb:
-            x2, dy2 = _rows(x), _rows(dy)
-            drop = _dropout_args(ctx.p, ctx.seed, ctx.offset if off is None else off)
-            with _On(x.device) as stream:
-                dz = dy2
-                changed = slope is not None or ctx.p > 0.0
-                if nb or changed:
-                    dz, db = _dz(stream, dy2, slope, drop, changed and (nx or nw), ctx.bias_dtype if nb else None)
-                    dz = dy2 if dz is None else dz
-                if nx:
-                    dx = _matmul(stream, dz, weight.t()).view(x.shape)
-                if nw:
-                    dw = _matmul(stream, dz.t(), x2.t())
+            x2, w, dy2 = _panel(_rows(x)), _panel(weight), _rows_ld(dy)
+            (m, k), n, dt, drop = x2.shape, w.shape[0], _DT[x2.dtype], ctx.drop
+            (x0, x1), (w0, w1), d0 = x2.stride(), w.stride(), dy2.stride(0)
+            xp, wp, dp = x2.data_ptr(), w.data_ptr(), dy2.data_ptr()
+            dx = x2.new_empty((m, k)) if nx else None
+            dw = x2.new_empty((n, k)) if nw else None
+            db = torch.empty(n, dtype=ctx.bias_dtype, device=x.device) if nb else None
+            bdt = _DT[ctx.bias_dtype] if nb else dt
+            need = _linear_grad_bytes(dt, bdt, m, n, k, d0, dp & 15, x0, x1, xp & 15, w0, w1, wp & 15, slope is not None, nx, nw, nb, drop.p)
+            ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+            _launch("clipvit_linear_grad", x.device.index, _lib.LinearGradArgs(
+                dt, bdt, m, n, k, dp, d0, xp, x0, x1, wp, w0, w1, _ptr(slope), _ptr(dx), _ptr(dw), _ptr(db), drop), ws, need)
+            if nx:
+                dx = dx.view(x.shape)
         return dx, dw, db, dy if nr else None, None, None, None, None
 
 
@@ -302,34 +276,40 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
         bias = bias.contiguous()
     if _wants_grad(x, weight, bias, residual):
         return _Linear.apply(x, weight, bias, residual, act, p, seed, offset)
-    y, _ = _linear_forward(_rows(x), weight, bias, None if residual is None else _rows(residual), act, p, seed, offset, False)
+    y, _ = _linear_forward(_rows(x), weight, bias, None if residual is None else _rows(residual), act,
+                           _dropout_args(p, seed, offset) if p else _NO_DROPOUT, False)
     return y.view(*x.shape[:-1], n)
 
 
 # ---------------------------------------------------------------- dropout
-def _dropout_call(x, residual, p, seed, offset):
+def _dropout_call(x, residual, drop):
     x2 = _rows(x)
     res2 = None if residual is None else _rows(residual)
-    y = torch.empty(x2.shape, dtype=x.dtype, device=x.device)
-    with _On(x.device) as stream:
-        _lib.check(_lib.lib().clipvit_dropout(
-            stream, _DT[x.dtype], x2.data_ptr(), x2.stride(0), _ptr(res2), 0 if res2 is None else res2.stride(0), y.data_ptr(),
-            y.stride(0), x2.shape[0], x2.shape[1], _byref(_dropout_args(p, seed, offset))))
+    y, index = torch.empty(x2.shape, dtype=x.dtype, device=x.device), x.device.index
+    args = (_DT[x.dtype], x2.data_ptr(), x2.stride(0), _ptr(res2), 0 if res2 is None else res2.stride(0), y.data_ptr(), y.stride(0),
+            x2.shape[0], x2.shape[1], _byref(drop))
+    if torch.cuda.current_device() == index:
+        rc = _lib.lib().clipvit_dropout(_stream(index), *args)
+    else:
+        with _On(index):
+            rc = _lib.lib().clipvit_dropout(_stream(index), *args)
+    if rc:
+        _lib.check(rc)
     return y.view(x.shape)
 
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, p, seed, offset):
+        ctx.drop = _dropout_args(p, seed, offset)
         ctx.save_for_backward(offset if torch.is_tensor(offset) else None)
-        ctx.p, ctx.seed, ctx.offset = p, seed, None if torch.is_tensor(offset) else offset
-        return _dropout_call(x, residual, p, seed, offset)
+        return _dropout_call(x, residual, ctx.drop)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        (off,) = ctx.saved_tensors
-        dx = _dropout_call(dy, None, ctx.p, ctx.seed, ctx.offset if off is None else off) if ctx.needs_input_grad[0] else None
+        ctx.saved_tensors  # raises where a tensor offset changed since the forward pass
+        dx = _dropout_call(dy, None, ctx.drop) if ctx.needs_input_grad[0] else None
         return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
 
 
@@ -348,58 +328,54 @@ def dropout(x: torch.Tensor, p: float, *, seed: int, offset=0, residual: torch.T
     _need_device(x, residual)
     if _wants_grad(x, residual):
         return _Dropout.apply(x, residual, p, seed, offset)
-    return _dropout_call(x, residual, p, seed, offset)
+    return _dropout_call(x, residual, _dropout_args(p, seed, offset))
 
 
 # ---------------------------------------------------------------- LoRA linear
-def _up32(n: int) -> int:
-    return (n + 31) // 32 * 32
-
-
-def _lora_forward(x2, weight, A, B, bias, scaling, p, seed, offset):
-    R = _up32(A.shape[1])
-    with _On(x2.device) as stream:
-        f, v = _pad(stream, (A.t(), R, _up32(A.shape[0])), (B.t(), B.shape[1], R))
-        keep = 1.0 / (1.0 - p) if p < 1.0 else 0.0
-        u = _down(stream, x2, f, scaling * keep, _dropout_args(p, seed, offset))
-        y = _matmul(stream, x2, weight, bias=bias, low=(u, v))
+def _lora_forward(x2, weight, A, B, bias, scaling, drop):
+    """(y [M, N], u [M, rank rounded up to 32]) of x2 [M, K]."""
+    w = _panel(weight)
+    (m, k), n, r, dt = x2.shape, w.shape[0], A.shape[1], _DT[x2.dtype]
+    x0, (w0, w1), xp, wp = x2.stride(0), w.stride(), x2.data_ptr(), w.data_ptr()
+    y, u = x2.new_empty((m, n)), x2.new_empty((m, (r + 31) // 32 * 32))
+    need = _lora_bytes(dt, m, n, k, r, x0, xp & 15, w0, w1, wp & 15)
+    ws = torch.empty(need, dtype=torch.uint8, device=x2.device) if need else None
+    _launch("clipvit_lora_linear", x2.device.index, _lib.LoraArgs(
+        dt, dt if bias is None else _DT[bias.dtype], m, n, k, r, xp, x0, wp, w0, w1, A.data_ptr(), A.stride(0), A.stride(1),
+        B.data_ptr(), B.stride(0), B.stride(1), _ptr(bias), y.data_ptr(), u.data_ptr(), scaling, 0.0, drop), ws, need)
     return y, u
 
 
 class _LoraLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, A, B, bias, scaling, p, seed, offset):
-        y, u = _lora_forward(_rows(x), weight, A, B, bias, scaling, p, seed, offset)
+        drop = _dropout_args(p, seed, offset)
+        y, u = _lora_forward(_rows_ld(x), weight, A, B, bias, scaling, drop)
         ctx.save_for_backward(x, weight, A, B, u, offset if torch.is_tensor(offset) else None)
-        ctx.bias_dtype = None if bias is None else bias.dtype
-        ctx.scaling, ctx.p, ctx.seed, ctx.offset = scaling, p, seed, None if torch.is_tensor(offset) else offset
+        ctx.drop, ctx.scaling, ctx.bias_dtype = drop, scaling, None if bias is None else bias.dtype
         return y.view(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weight, A, B, u, off = ctx.saved_tensors
+        x, weight, A, B, u, _ = ctx.saved_tensors
         nx, nw, nA, nB, nb = ctx.needs_input_grad[:5]
-        dx = dw = dA = dB = db = None
-        x2, dy2 = _rows(x), _rows(dy)
-        (K, rank), N, R = A.shape, weight.shape[0], u.shape[1]
-        drop = _dropout_args(ctx.p, ctx.seed, ctx.offset if off is None else off)
-        with _On(x.device) as stream:
-            if nx or nA:
-                f, v = _pad(stream, (B, R, _up32(N)), (A, K, R))
-                keep = 1.0 / (1.0 - ctx.p) if ctx.p < 1.0 else 0.0
-                du = _down(stream, dy2, f, ctx.scaling * keep, _NO_DROPOUT)
-                if nx:
-                    dx = _matmul(stream, dy2, weight.t(), low=(du, v), low_mask=True, drop=drop).view(x.shape)
-                if nA:
-                    dA = _low_grad(stream, x2, du, rank, False, drop)
-            if nB:
-                dB = _low_grad(stream, dy2, u, rank, True, _NO_DROPOUT)
-            if nw:
-                dw = _matmul(stream, dy2.t(), x2.t())
-            if nb:
-                _, db = _dz(stream, dy2, None, _NO_DROPOUT, False, ctx.bias_dtype)
-        return dx, dw, dA, dB, db, None, None, None, None
+        x2, w, dy2 = _rows_ld(x), _panel(weight), _rows_ld(dy)
+        (m, k), n, r, dt, drop = x2.shape, w.shape[0], A.shape[1], _DT[x2.dtype], ctx.drop
+        x0, (w0, w1), d0 = x2.stride(0), w.stride(), dy2.stride(0)
+        xp, wp, dp = x2.data_ptr(), w.data_ptr(), dy2.data_ptr()
+        dx = x2.new_empty((m, k)) if nx else None
+        dw = x2.new_empty((n, k)) if nw else None
+        dA = x2.new_empty((k, r)) if nA else None
+        dB = x2.new_empty((r, n)) if nB else None
+        db = torch.empty(n, dtype=ctx.bias_dtype, device=x.device) if nb else None
+        bdt = _DT[ctx.bias_dtype] if nb else dt
+        need = _lora_grad_bytes(dt, bdt, m, n, k, r, d0, dp & 15, x0, xp & 15, w0, w1, wp & 15, nx, nw, nA, nB, nb, drop.p)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+        _launch("clipvit_lora_linear_grad", x.device.index, _lib.LoraGradArgs(
+            dt, bdt, m, n, k, r, dp, d0, xp, x0, wp, w0, w1, A.data_ptr(), A.stride(0), A.stride(1), B.data_ptr(), B.stride(0),
+            B.stride(1), u.data_ptr(), _ptr(dx), _ptr(dw), _ptr(dA), _ptr(dB), _ptr(db), ctx.scaling, 0.0, drop), ws, need)
+        return dx if dx is None else dx.view(x.shape), dw, dA, dB, db, None, None, None, None
 
 
 def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_A: torch.Tensor, lora_B: torch.Tensor,
@@ -427,4 +403,5 @@ def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_A: torch.Tensor, lor
         bias = bias.contiguous()
     if _wants_grad(x, weight, lora_A, lora_B, bias):
         return _LoraLinear.apply(x, weight, lora_A, lora_B, bias, float(scaling), p, seed, offset)
-    return _lora_forward(_rows(x), weight, lora_A, lora_B, bias, float(scaling), p, seed, offset)[0].view(*x.shape[:-1], n)
+    return _lora_forward(_rows_ld(x), weight, lora_A, lora_B, bias, float(scaling), _dropout_args(p, seed, offset))[0].view(
+        *x.shape[:-1], n)

@@ -269,20 +269,18 @@ typedef enum {
     CLIPVIT_ACT_RELU = 5,
 } clipvit_activation;
 
-/* y[m, n] = residual[m, n] + dropout(act(z))[m, n],  z = sum_k x[m, k] w[n, k] + bias[n] + sum_r u[m, r] v[n, r].
- * x [M, K] and w [N, K] are views with two strides, one of them 1 (so a gradient's product takes the forward's
- * tensors transposed); the other is below 2^22 and at least the row's length. y and residual have unit column
- * stride. slope (or NULL): act'(z) as [M, N] contiguous 16-bit fixed point, q / 2^14 (-32768 = NaN), what
- * clipvit_linear_dz takes. R > 0: the low-rank term, u [M, R] and v [N, R] contiguous, R % 32 == 0. low_mask:
- * the dropout mask, unscaled, applies to the low-rank term instead (no bias and no activation then).
- * Rows of any length, stride and alignment are taken; those that 16-byte loads cannot address are copied into the
- * workspace first. y must not overlap an input other than an identical residual. */
+/* y[m, n] = residual[m, n] + dropout(act(z))[m, n],  z = sum_k x[m, k] w[n, k] + bias[n].
+ * x [M, K] and w [N, K] are views with two strides, one of them 1; the other is below 2^22 and at least the row's
+ * length. y and residual have unit column stride. slope (or NULL, with an activation): act'(z) as [M, N] contiguous
+ * 16-bit fixed point, q / 2^14 (-32768 = NaN), what the gradient takes. Rows of any length, stride and alignment
+ * are taken; those that 16-byte loads cannot address are copied into the workspace first. y must not overlap an
+ * input other than an identical residual. */
 typedef struct {
-    int dtype;      /* CLIPVIT_BF16 or CLIPVIT_F16: x, w, residual, y, u, v */
+    int dtype;      /* CLIPVIT_BF16 or CLIPVIT_F16: x, w, residual, y */
     int activation; /* clipvit_activation */
     int bias_dtype; /* CLIPVIT_F32 or dtype */
-    int low_mask;
-    int64_t M, N, K, R;
+    int reserved;
+    int64_t M, N, K;
     const void* x;
     int64_t x_stride[2];
     const void* w;
@@ -293,30 +291,36 @@ typedef struct {
     void* y;
     int64_t y_stride;
     int16_t* slope;
-    const void* low_u;
-    const void* low_v;
     clipvit_dropout_args dropout;
 } clipvit_linear_args;
 
-/* Bytes of workspace (256-byte aligned) that clipvit_linear needs for these arguments; may be 0. */
+/* Bytes of workspace (256-byte aligned) that the call needs for these arguments; may be 0. It depends on the sizes,
+ * strides, pointer alignments and on which outputs are asked for, not on the data. (The same holds below.) */
 int clipvit_linear_workspace(const clipvit_linear_args* args, size_t* bytes);
 int clipvit_linear(void* stream, const clipvit_linear_args* args, void* workspace, size_t bytes);
 
-/* dz[m, n] = dropout(dy)[m, n] slope[m, n] (dz, slope may be NULL) and db[n] = sum_m of the unrounded dz (or NULL),
- * summed in a fixed order. Workspace with db: 4 N min(512, ceil(M / 64)) bytes, 16-byte aligned. */
+/* Gradients of clipvit_linear, each output NULL or wanted: dz = dropout(dy) slope (slope NULL: no activation);
+ * dx [M, K] = dz w, dw [N, K] = dz^T x (contiguous, of dtype; dz is rounded to dtype for them when there is a slope
+ * or a dropout), db [N] = column sums of the unrounded dz. The residual's gradient is dy itself. dy [M, N] has unit
+ * column stride. Every sum is taken in a fixed order. */
 typedef struct {
     int dtype;
-    int db_dtype; /* CLIPVIT_F32 or dtype */
-    int64_t M, N;
+    int bias_dtype; /* of db: CLIPVIT_F32 or dtype */
+    int64_t M, N, K;
     const void* dy;
     int64_t dy_stride;
+    const void* x;
+    int64_t x_stride[2];
+    const void* w;
+    int64_t w_stride[2];
     const int16_t* slope;
-    void* dz;
-    int64_t dz_stride;
+    void* dx;
+    void* dw;
     void* db;
     clipvit_dropout_args dropout;
-} clipvit_dz_args;
-int clipvit_linear_dz(void* stream, const clipvit_dz_args* args, void* workspace, size_t bytes);
+} clipvit_linear_grad_args;
+int clipvit_linear_grad_workspace(const clipvit_linear_grad_args* args, size_t* bytes);
+int clipvit_linear_grad(void* stream, const clipvit_linear_grad_args* args, void* workspace, size_t bytes);
 
 /* y = residual + dropout(x) on [rows, cols] F32, BF16 or F16 rows of unit column stride (residual may be NULL, y may
  * be x or residual). The gradient of x is the same call on dy. */
@@ -324,27 +328,61 @@ int clipvit_dropout(void* stream, int dtype, const void* x, int64_t x_stride, co
                     int64_t residual_stride, void* y, int64_t y_stride, int64_t rows, int64_t cols,
                     const clipvit_dropout_args* dropout);
 
-/* dst[i, j] = src(i, j) for i < rows, j < cols, 0 up to [rows_padded, cols_padded] (contiguous): a 16-bit low-rank
- * factor in the padded (and, by its strides, transposed) form the calls below and clipvit_linear take. Two
- * factors a launch; either may be NULL. */
+/* The reference's LoRALinear (main.py:30-31, 42-43), unmerged: y = x w^T + bias + scaling (dropout(x) a) b with
+ * a [K, rank], b [rank, N] (any two strides), x [M, K] rows of unit column stride, w as in clipvit_linear, y [M, N]
+ * contiguous. u [M, rank rounded up to 32] (output, 16-byte aligned): the thin product scaling / (1 - p)
+ * (mask x) a rounded to dtype, what the gradient takes. */
 typedef struct {
-    const void* src;
-    int64_t row_stride, col_stride, rows, cols, rows_padded, cols_padded;
-    void* dst;
-} clipvit_pad_args;
-int clipvit_lora_pad(void* stream, const clipvit_pad_args* a, const clipvit_pad_args* b);
+    int dtype;
+    int bias_dtype;
+    int64_t M, N, K, rank;
+    const void* x;
+    int64_t x_stride;
+    const void* w;
+    int64_t w_stride[2];
+    const void* a;
+    int64_t a_stride[2];
+    const void* b;
+    int64_t b_stride[2];
+    const void* bias;
+    void* y;
+    void* u;
+    float scaling;
+    float reserved;
+    clipvit_dropout_args dropout;
+} clipvit_lora_args;
+int clipvit_lora_linear_workspace(const clipvit_lora_args* args, size_t* bytes);
+int clipvit_lora_linear(void* stream, const clipvit_lora_args* args, void* workspace, size_t bytes);
 
-/* u[m, r] = alpha sum_k mask(x)[m, k] f[r, k]: the adapter's thin product. x [M, K] of row stride x_stride;
- * f [R, >= K rounded up to 32] zero padded, R % 32 == 0; u [M, R] contiguous. The mask is unscaled. */
-int clipvit_lora_down(void* stream, int dtype, const void* x, int64_t x_stride, const void* f, int64_t f_stride,
-                      void* u, int64_t M, int64_t K, int64_t R, float alpha, const clipvit_dropout_args* dropout);
-
-/* out(c, r) = sum_m mask(x)[m, c] u[m, r] for r < rank: an adapter factor's gradient, summed in a fixed order.
- * x [M, C], u [M, R] contiguous, out at out + c out_col_stride + r out_rank_stride. */
-int clipvit_lora_grad_workspace(int64_t M, int64_t C, int64_t R, size_t* bytes);
-int clipvit_lora_grad(void* stream, int dtype, const void* x, int64_t x_stride, const void* u, void* out,
-                      int64_t out_col_stride, int64_t out_rank_stride, int64_t M, int64_t C, int64_t R, int64_t rank,
-                      const clipvit_dropout_args* dropout, void* workspace, size_t bytes);
+/* Its gradients, each output NULL or wanted, contiguous: dx [M, K], dw [N, K], da [K, rank], db_factor [rank, N] of
+ * dtype and dbias [N]. du = scaling / (1 - p) dy b^T is rounded to dtype; dx = dy w + mask (du a^T), da = (mask x)^T du,
+ * db_factor = u^T dy, dw = dy^T x, dbias = column sums of dy, in fixed orders. */
+typedef struct {
+    int dtype;
+    int bias_dtype;
+    int64_t M, N, K, rank;
+    const void* dy;
+    int64_t dy_stride;
+    const void* x;
+    int64_t x_stride;
+    const void* w;
+    int64_t w_stride[2];
+    const void* a;
+    int64_t a_stride[2];
+    const void* b;
+    int64_t b_stride[2];
+    const void* u;
+    void* dx;
+    void* dw;
+    void* da;
+    void* db_factor;
+    void* dbias;
+    float scaling;
+    float reserved;
+    clipvit_dropout_args dropout;
+} clipvit_lora_grad_args;
+int clipvit_lora_linear_grad_workspace(const clipvit_lora_grad_args* args, size_t* bytes);
+int clipvit_lora_linear_grad(void* stream, const clipvit_lora_grad_args* args, void* workspace, size_t bytes);
 
 /* ---- kernel-level entry points (testing / benchmarking of single hot kernels) ----
  * These operate on caller-owned device buffers with the packed layouts documented in

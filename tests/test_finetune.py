@@ -64,80 +64,114 @@ def test_python_refusals(call, error):
         call()
 
 
-def linear_args(**kw):
-    a = _lib.LinearArgs()
-    a.dtype = a.bias_dtype = _lib.BF16
-    a.M, a.N, a.K = 4, 8, 16
-    a.x = a.w = a.y = 4096  # never dereferenced: every call below is refused before a launch
-    a.x_stride[:] = [16, 1]
-    a.w_stride[:] = [16, 1]
-    a.y_stride = 8
+FAKE = 4096  # never dereferenced: every call below is refused before a launch
+
+
+def build(cls, base, kw):
+    a = cls(**{k: v for k, v in base.items()})
     for k, v in kw.items():
-        if isinstance(v, list):
-            getattr(a, k)[:] = v
-        elif k == "p":
+        if k == "p":
             a.dropout.p = v
         else:
             setattr(a, k, v)
     return a
 
 
-@pytest.mark.parametrize("kw", [
-    {"dtype": _lib.F32}, {"dtype": 7}, {"activation": 6}, {"activation": -1}, {"bias_dtype": _lib.F16}, {"M": -1},
-    {"K": 1 << 31}, {"x": None}, {"w": None}, {"y": None}, {"y_stride": 7}, {"x_stride": [8, 1]}, {"x_stride": [32, 2]},
-    {"w_stride": [0, 1]}, {"w_stride": [1 << 22, 1]}, {"R": 16, "low_u": 4096, "low_v": 4096}, {"R": 32},
-    {"R": 32, "low_u": 4096, "low_v": 4104}, {"p": 1.01}, {"p": -0.5}, {"p": float("nan")}, {"low_mask": 1, "activation": 1},
-])
-def test_linear_entry_refuses(kw):
+def linear_args(**kw):
+    return build(_lib.LinearArgs, dict(dtype=_lib.BF16, bias_dtype=_lib.BF16, M=4, N=8, K=16, x=FAKE, w=FAKE, y=FAKE, x_row=16,
+                                       x_col=1, w_row=16, w_col=1, y_stride=8), kw)
+
+
+def linear_grad_args(**kw):
+    return build(_lib.LinearGradArgs, dict(dtype=_lib.BF16, bias_dtype=_lib.BF16, M=4, N=8, K=16, dy=FAKE, dy_stride=8, x=FAKE,
+                                           w=FAKE, x_row=16, x_col=1, w_row=16, w_col=1, dx=FAKE, dw=FAKE, db=FAKE), kw)
+
+
+def lora_args(**kw):
+    return build(_lib.LoraArgs, dict(dtype=_lib.F16, bias_dtype=_lib.F32, M=4, N=8, K=16, rank=4, x=FAKE, x_stride=16, w=FAKE, w_row=16,
+                                     w_col=1, a=FAKE, a_row=4, a_col=1, b=FAKE, b_row=8, b_col=1, y=FAKE, u=FAKE, scaling=1.0), kw)
+
+
+def lora_grad_args(**kw):
+    return build(_lib.LoraGradArgs, dict(dtype=_lib.F16, bias_dtype=_lib.F32, M=4, N=8, K=16, rank=4, dy=FAKE, dy_stride=8, x=FAKE,
+                                         x_stride=16, w=FAKE, w_row=16, w_col=1, a=FAKE, a_row=4, a_col=1, b=FAKE, b_row=8, b_col=1,
+                                         u=FAKE, dx=FAKE, dw=FAKE, da=FAKE, db_factor=FAKE, dbias=FAKE, scaling=1.0), kw)
+
+
+def refused(name, a):
     L, need = _lib.lib(), ctypes.c_size_t()
-    a = linear_args(**kw)
-    assert L.clipvit_linear_workspace(ctypes.byref(a), ctypes.byref(need)) == _lib.E_INVALID
-    assert L.clipvit_linear(None, ctypes.byref(a), None, 0) == _lib.E_INVALID
+    assert getattr(L, f"clipvit_{name}_workspace")(ctypes.byref(a), ctypes.byref(need)) == _lib.E_INVALID
+    assert getattr(L, f"clipvit_{name}")(None, ctypes.byref(a), None, 0) == _lib.E_INVALID
     assert L.clipvit_last_error()
 
 
-def test_linear_workspace_rules():
+COMMON = [{"dtype": _lib.F32}, {"dtype": 7}, {"bias_dtype": _lib.MXFP8}, {"M": -1}, {"N": -1}, {"K": 1 << 31}, {"p": 1.01}, {"p": -0.5},
+          {"p": float("nan")}, {"w_row": 0}, {"w_row": 1 << 22}, {"w_row": 32, "w_col": 2}]
+
+
+@pytest.mark.parametrize("kw", COMMON + [{"activation": 6}, {"activation": -1}, {"x": None}, {"w": None}, {"y": None}, {"y_stride": 7},
+                                         {"x_row": 8}, {"x_row": 32, "x_col": 2}, {"residual": FAKE, "residual_stride": -8}])
+def test_linear_entry_refuses(kw):
+    refused("linear", linear_args(**kw))
+
+
+@pytest.mark.parametrize("kw", COMMON + [{"dy": None}, {"x": None}, {"w": None}, {"dy_stride": 7}, {"dy_stride": 1 << 22}, {"x_row": 8}])
+def test_linear_grad_entry_refuses(kw):
+    refused("linear_grad", linear_grad_args(**kw))
+
+
+@pytest.mark.parametrize("kw", COMMON + [{"rank": 0}, {"rank": 65537}, {"x": None}, {"w": None}, {"a": None}, {"b": None}, {"y": None},
+                                         {"u": None}, {"u": FAKE + 8}, {"x_stride": 15}])
+def test_lora_entry_refuses(kw):
+    refused("lora_linear", lora_args(**kw))
+
+
+@pytest.mark.parametrize("kw", COMMON + [{"rank": 0}, {"dy": None}, {"x": None}, {"w": None}, {"a": None}, {"b": None}, {"u": None},
+                                         {"u": FAKE + 8}, {"dy_stride": 7}, {"x_stride": 15}])
+def test_lora_grad_entry_refuses(kw):
+    refused("lora_linear_grad", lora_grad_args(**kw))
+
+
+@pytest.mark.parametrize("name, args", [
+    ("linear", linear_args(K=17, x_row=17, w_row=17)),  # odd rows: both operands are copied first
+    ("linear_grad", linear_grad_args()), ("lora_linear", lora_args()), ("lora_linear_grad", lora_grad_args())])
+def test_workspace_rules(name, args):
     L, need = _lib.lib(), ctypes.c_size_t()
-    assert L.clipvit_linear_workspace(None, ctypes.byref(need)) == _lib.E_INVALID
-    assert L.clipvit_linear_workspace(ctypes.byref(linear_args()), None) == _lib.E_INVALID
-    a = linear_args(K=17, x_stride=[17, 1], w_stride=[17, 1])  # odd rows: both operands are copied first
-    assert L.clipvit_linear_workspace(ctypes.byref(a), ctypes.byref(need)) == 0 and need.value > 0
-    assert L.clipvit_linear(None, ctypes.byref(a), None, 0) == _lib.E_INVALID
-    assert L.clipvit_linear(None, ctypes.byref(a), ctypes.c_void_p(4096 + 16), need) == _lib.E_INVALID
-    assert L.clipvit_linear(None, ctypes.byref(a), ctypes.c_void_p(4096), ctypes.c_size_t(need.value - 1)) == _lib.E_INVALID
-    empty = linear_args(M=0, x=None, y=None)
-    assert L.clipvit_linear(None, ctypes.byref(empty), None, 0) == 0  # nothing to do, nothing launched
+    size, call = getattr(L, f"clipvit_{name}_workspace"), getattr(L, f"clipvit_{name}")
+    assert size(None, ctypes.byref(need)) == _lib.E_INVALID and size(ctypes.byref(args), None) == _lib.E_INVALID
+    assert call(None, None, None, 0) == _lib.E_INVALID
+    assert size(ctypes.byref(args), ctypes.byref(need)) == 0 and need.value > 0
+    assert call(None, ctypes.byref(args), None, 0) == _lib.E_INVALID
+    assert call(None, ctypes.byref(args), None, need.value) == _lib.E_INVALID
+    assert call(None, ctypes.byref(args), FAKE + 16, need.value) == _lib.E_INVALID
+    assert call(None, ctypes.byref(args), FAKE, need.value - 1) == _lib.E_INVALID
 
 
-def test_other_entries_refuse():
+def test_empty_calls_launch_nothing():
+    L = _lib.lib()
+    for name, a in (("linear", linear_args(M=0, x=None, y=None)), ("linear", linear_args(N=0, w=None, y=None)),
+                    ("linear_grad", linear_grad_args(dx=None, dw=None, db=None)), ("lora_linear", lora_args(M=0, x=None))):
+        assert getattr(L, f"clipvit_{name}")(None, ctypes.byref(a), None, 0) == 0
+
+
+def test_dropout_entry_refuses():
     L, d, bad = _lib.lib(), _lib.DropoutArgs(0.5, 1, 0, None), _lib.DropoutArgs(2.0, 1, 0, None)
-    v, B = ctypes.c_void_p(4096), ctypes.byref
+    v, B = FAKE, ctypes.byref
     assert L.clipvit_dropout(None, _lib.BF16, v, 8, None, 0, v, 8, 4, 8, None) == _lib.E_INVALID
     assert L.clipvit_dropout(None, _lib.BF16, v, 8, None, 0, v, 8, 4, 8, B(bad)) == _lib.E_INVALID
     assert L.clipvit_dropout(None, _lib.MXFP8, v, 8, None, 0, v, 8, 4, 8, B(d)) == _lib.E_INVALID
     assert L.clipvit_dropout(None, _lib.BF16, None, 8, None, 0, v, 8, 4, 8, B(d)) == _lib.E_INVALID
     assert L.clipvit_dropout(None, _lib.BF16, v, 8, None, 0, v, 7, 4, 8, B(d)) == _lib.E_INVALID
     assert L.clipvit_dropout(None, _lib.BF16, v, 8, None, 0, v, 8, -1, 8, B(d)) == _lib.E_INVALID
-    a = _lib.DzArgs()
-    a.dtype = a.db_dtype = _lib.F16
-    a.M, a.N, a.dy, a.dy_stride, a.db = 100, 8, 4096, 8, 4096
-    assert L.clipvit_linear_dz(None, B(a), v, 4 * 8 * 2 - 1) == _lib.E_INVALID
-    a.dy = None
-    assert L.clipvit_linear_dz(None, B(a), v, 1 << 20) == _lib.E_INVALID
-    p = _lib.PadArgs(4096, 1, 1, 4, 4, 3, 4, 4096)
-    assert L.clipvit_lora_pad(None, B(p), None) == _lib.E_INVALID
-    assert L.clipvit_lora_pad(None, None, None) == 0
-    assert L.clipvit_lora_down(None, _lib.BF16, v, 16, v, 16, v, 4, 16, 32, 1.0, B(d)) == _lib.E_INVALID  # f rows < 32
-    assert L.clipvit_lora_down(None, _lib.BF16, v, 16, v, 32, v, 4, 16, 16, 1.0, B(d)) == _lib.E_INVALID  # R % 32
-    assert L.clipvit_lora_grad(None, _lib.BF16, v, 16, v, v, 1, 16, 4, 16, 32, 33, B(d), v, 1 << 30) == _lib.E_INVALID
-    assert L.clipvit_lora_grad(None, _lib.BF16, v, 16, v, v, 1, 16, 4, 16, 32, 4, B(d), v, 0) == _lib.E_INVALID
+    assert L.clipvit_dropout(None, _lib.BF16, None, 8, None, 0, None, 8, 0, 8, B(d)) == 0
 
 
 def test_struct_layouts():
     assert ctypes.sizeof(_lib.DropoutArgs) == 32
-    assert ctypes.sizeof(_lib.LinearArgs) == 16 + 4 * 8 + 3 * 8 + 3 * 8 + 8 + 16 + 16 + 8 + 16 + 32
-    assert ctypes.sizeof(_lib.DzArgs) == 8 + 16 + 16 + 8 + 16 + 8 + 32
-    assert ctypes.sizeof(_lib.PadArgs) == 64
+    assert ctypes.sizeof(_lib.LinearArgs) == 16 + 24 + 2 * 24 + 8 + 16 + 16 + 8 + 32
+    assert ctypes.sizeof(_lib.LinearGradArgs) == 8 + 24 + 16 + 2 * 24 + 8 + 24 + 32
+    assert ctypes.sizeof(_lib.LoraArgs) == 8 + 32 + 16 + 3 * 24 + 3 * 8 + 8 + 32
+    assert ctypes.sizeof(_lib.LoraGradArgs) == 8 + 32 + 2 * 16 + 3 * 24 + 8 + 5 * 8 + 8 + 32
 
 
 @pytest.mark.parametrize("kind", ["none", "quick_gelu", "gelu", "gelu_tanh", "silu", "relu"])
