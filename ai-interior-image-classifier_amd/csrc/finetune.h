@@ -66,8 +66,14 @@ __device__ __forceinline__ float act_one(float beta, float z, float& slope) {
         if (SLOPE) slope = s * (1.0f - 0.69314718055994531f * beta * zc * (1.0f - s));
         return z * s;
     } else if constexpr (ACT == ACT_GELU) {
-        const float c = 0.5f + 0.5f * erff(0.70710678118654752f * z);
-        if (SLOPE) slope = c + 0.39894228040143268f * zc * __builtin_amdgcn_exp2f(-0.72134752044448170f * zc * zc);
+        // Phi(-|z|) = t (a1 + t (a2 + ..)) e^(-z^2 / 2) / 2, t = 1 / (1 + p |z| / sqrt 2): Abramowitz and Stegun
+        // 7.1.26, off by at most 7.5e-8; it shares the exponential with the derivative (erff and its own exponential:
+        // 70 instructions an element against 30, 4928 x 512 x 2048 with the derivative 52 us against 38)
+        const float az = fabsf(z), t = __builtin_amdgcn_rcpf(1.0f + 0.23164189f * az);
+        const float e = __builtin_amdgcn_exp2f(-0.72134752044448170f * az * az);
+        const float q = t * (0.127414796f + t * (-0.142248368f + t * (0.710706871f + t * (-0.726576014f + t * 0.530702714f)))) * e;
+        const float c = z < 0.f ? q : 1.0f - q;
+        if (SLOPE) slope = c + 0.39894228040143268f * zc * e;
         return z * c;
     } else if constexpr (ACT == ACT_GELU_TANH) {
         const float s = logistic(1.5957691216057308f * (z + 0.044715f * z * (z * z)));

@@ -36,14 +36,14 @@ __device__ __forceinline__ int col_swz(int k) {
     return R >= 128 ? (k & 3) | ((k >> 1) & 4) : ((k >> 1) & 1) | ((k >> 2) & 2);
 }
 
-// Position in a panel's LDS image -> row (column) of the tile. Whole: the panel is the tile's operand. Half<H>: the
-// 64-row halves H of both 128-row wave groups.
+// Position in a panel's LDS image -> row (column) of the tile. Whole: the panel is the tile's operand. Half<H, W>: the
+// W-wide halves H of every 2 W rows.
 struct Whole {
     static __device__ __forceinline__ int at(int i) { return i; }
 };
-template <int H>
+template <int H, int W>
 struct Half {
-    static __device__ __forceinline__ int at(int i) { return ((i & 64) << 1) + 64 * H + (i & 63); }
+    static __device__ __forceinline__ int at(int i) { return (i & ~(W - 1)) * 2 + W * H + (i & (W - 1)); }
 };
 
 // One operand's panel of a tile: R rows (KC) or columns, staged by NW waves, NP pieces of 1 KB each.
@@ -105,7 +105,7 @@ struct Panel {
     }
 };
 
-// Fragment reads of FR (1 or 4) 16-row fragments x 64 k from position i0 of a panel. Each asm block ends with its own
+// Fragment reads of FR (1, 2 or 4) 16-row fragments x 64 k from position i0 of a panel. Each asm block ends with its own
 // wait (hipcc does not see these reads, and a plain LDS read would make it drain the LDS-DMA loads in flight).
 template <typename T, bool KC, int R, int FR>
 struct Frags {
@@ -132,8 +132,14 @@ struct Frags {
                   "=&v"(d[1][2]), "=&v"(d[1][3])
                 : "v"(addr[0] + so), "v"(addr[1] + so)
                 : "memory");
+        } else if constexpr (KC && FR == 2) {
+            asm volatile(
+                "ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:2048\n\tds_read_b128 %2, %5\n\t"
+                "ds_read_b128 %3, %5 offset:2048\n\ts_waitcnt lgkmcnt(0)"
+                : "=&v"(d[0][0]), "=&v"(d[0][1]), "=&v"(d[1][0]), "=&v"(d[1][1])
+                : "v"(addr[0] + so), "v"(addr[1] + so)
+                : "memory");
         } else if constexpr (KC) {
-            static_assert(FR == 1, "one or four fragments");
             asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %3\n\ts_waitcnt lgkmcnt(0)"
                          : "=&v"(d[0][0]), "=&v"(d[1][0])
                          : "v"(addr[0] + so), "v"(addr[1] + so)
@@ -156,6 +162,19 @@ struct Frags {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 d[i >> 2][i & 3] = __builtin_bit_cast(vec8, (u32x4){r[2 * i].x, r[2 * i].y, r[2 * i + 1].x, r[2 * i + 1].y});
+        } else if constexpr (FR == 2) {
+            u32x2 r[8];
+            asm volatile(
+                "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%10\n\t"
+                "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%10\n\t"
+                "ds_read_b64_tr_b16 %4, %8 offset:%11\n\tds_read_b64_tr_b16 %5, %8 offset:%12\n\t"
+                "ds_read_b64_tr_b16 %6, %9 offset:%11\n\tds_read_b64_tr_b16 %7, %9 offset:%12\n\ts_waitcnt lgkmcnt(0)"
+                : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+                : "v"(addr[0] + so), "v"(addr[1] + so), "i"(R * 8), "i"(R * 64), "i"(R * 72)
+                : "memory");
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                d[i >> 1][i & 1] = __builtin_bit_cast(vec8, (u32x4){r[2 * i].x, r[2 * i].y, r[2 * i + 1].x, r[2 * i + 1].y});
         } else {
             u32x2 r[4];
             asm volatile(
@@ -271,22 +290,25 @@ __device__ __forceinline__ void store_tile(const Matmul& a, f32x4 (&acc)[FM][4],
 }
 
 // 256 x 256 tiles. Eight waves in two groups of four, one barrier apart: while one group issues 32 MFMAs the other
-// reads fragments and stages. A k-tile T is two steps: step 0 reads B (kept in registers for both) and the group's
-// first 64 rows of A, step 1 its other 64 rows. Slot = barrier interval; group g reads step (T, h) in slot
-// 4 T + 2 h + g and computes it in the next one.
-//  * A's first halves of T are read in slots 4 T and 4 T + 1, so group 0 refills them (k-tile T + 2) in slot 4 T + 2;
-//    the second halves, read in 4 T + 2 and 4 T + 3, in slot 4 T + 4. Group 0 waits for its four oldest pieces (eight
-//    younger ones may fly) at the end of each of its MFMA segments: each half has six slots to land.
-//  * B of T, read in slots 4 T and 4 T + 1, is refilled by group 1 (k-tile T + 2) at the start of its MFMA segment
-//    in slot 4 T + 2; group 1 waits for the eight pieces of B(T + 1) in slot 4 T + 3.
+// reads fragments and stages. A k-tile T is two steps: step (T, 0) computes the group's first 64 rows, (T, 1) its other
+// 64. B's fragments stay in registers for both; to balance the reads (twelve ds_read_b128 a step, under the 512 cycles
+// of the other group's MFMAs), step (T, 0) reads A's first half and B's second 32 columns of T, step (T, 1) A's second
+// half and B's first 32 columns of T + 1. Slot = barrier interval; group g reads step (T, h) in slot 4 T + 2 h + g and
+// computes it in the next one. LDS holds two k-tiles; each half panel is refilled as soon as both groups have read it:
+//  * A0(T), read in slots 4 T and 4 T + 1, by A0(T + 2) in slot 4 T + 2; A1(T), read in 4 T + 2 and 4 T + 3, by A1(T + 2)
+//    in slot 4 T + 4: group 0, at the start of its read segments. It waits for its four oldest pieces (eight younger
+//    ones may fly) at the end of each of its MFMA segments, six slots after their issue.
+//  * B0(T + 1), read in slots 4 T + 2 and 4 T + 3, by B0(T + 3) in slot 4 T + 4; B1(T), read in 4 T and 4 T + 1, by
+//    B1(T + 2) in slot 4 T + 2: group 1, at the start of its MFMA segments. It waits likewise in its read segments.
 // Steps past the last k-tile stage zeros into parts nobody reads (kept, so that the counted waits hold).
 template <typename T, bool AK, bool BK>
 __global__ __launch_bounds__(512, 1) void matmul256_kernel(Matmul a, float* part, int N4, int kslice) {
     typedef typename T::vec8 vec8;
-    using PA0 = Panel<AK, 128, 4, Half<0>>;
-    using PA1 = Panel<AK, 128, 4, Half<1>>;
-    using PB = Panel<BK, 256, 4, Whole>;
-    constexpr int A_HALF = 16384, A_ST = 32768, B_OFF = 65536, B_ST = 32768, E_OFF = 131072;
+    using PA0 = Panel<AK, 128, 4, Half<0, 64>>;
+    using PA1 = Panel<AK, 128, 4, Half<1, 64>>;
+    using PB0 = Panel<BK, 128, 4, Half<0, 32>>;
+    using PB1 = Panel<BK, 128, 4, Half<1, 32>>;
+    constexpr int HALF = 16384, ST = 32768, B_OFF = 65536, E_OFF = 131072;
     __shared__ __attribute__((aligned(16))) unsigned char smem[E_OFF + 8 * 4096];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -301,10 +323,10 @@ __global__ __launch_bounds__(512, 1) void matmul256_kernel(Matmul a, float* part
 
     const unsigned lds = (unsigned)(size_t)(LDS_AS unsigned char*)smem;
     Frags<T, AK, 128, 4> fa;
-    Frags<T, BK, 256, 4> fb;
+    Frags<T, BK, 128, 2> fb;
     fa.init(lds, wm * 64, lane);
-    fb.init(lds + B_OFF, wn * 64, lane);
-    vec8 af[2][4], bf[2][4];
+    fb.init(lds + B_OFF, wn * 32, lane);
+    vec8 af[2][4], b0[2][2], b1[2][2], bn[2][2];
     f32x4 acc[8][4];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -314,13 +336,19 @@ __global__ __launch_bounds__(512, 1) void matmul256_kernel(Matmul a, float* part
         constexpr int H = decltype(half)::value * 4;
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[H + i][j] = T::mfma16(bf[ks][j], af[ks][i], acc[H + i][j]);
+                for (int i = 0; i < 4; ++i) acc[H + i][j] = T::mfma16(j < 2 ? b0[ks][j & 1] : b1[ks][j & 1], af[ks][i], acc[H + i][j]);
         __builtin_amdgcn_s_setprio(0);
         __builtin_amdgcn_sched_barrier(0);
+    };
+    auto next_b0 = [&]() {
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) b0[ks][j] = bn[ks][j];
     };
     using H0 = std::integral_constant<int, 0>;
     using H1 = std::integral_constant<int, 1>;
@@ -331,47 +359,62 @@ __global__ __launch_bounds__(512, 1) void matmul256_kernel(Matmul a, float* part
             p0.init(a.A, a.lda, m0, a.M, a.K, wn, lane);
             p1.init(a.A, a.lda, m0, a.M, a.K, wn, lane);
             p0.stage(kt_of(0), wn, smem);
-            p1.stage(kt_of(0), wn, smem + A_HALF);
-            p0.stage(kt_of(1), wn, smem + A_ST);
+            p1.stage(kt_of(0), wn, smem + HALF);
+            p0.stage(kt_of(1), wn, smem + ST);
             vm_wait<8>();
             bar();
+            fb.read(b0, 0);
+            bar();
             for (int t = 0; t < nk; ++t) {
-                const int st = t & 1;
-                p1.stage(kt_of(t + 1), wn, smem + (st ^ 1) * A_ST + A_HALF);
-                fb.read(bf, st * B_ST);
-                fa.read(af, st * A_ST);
+                const int so = (t & 1) * ST;
+                p1.stage(kt_of(t + 1), wn, smem + (so ^ ST) + HALF);
+                fb.read(b1, so + HALF);
+                fa.read(af, so);
                 bar();
                 mfmas(H0{});
                 vm_wait<8>();
                 bar();
-                p0.stage(kt_of(t + 2), wn, smem + st * A_ST);
-                fa.read(af, st * A_ST + A_HALF);
+                p0.stage(kt_of(t + 2), wn, smem + so);
+                fb.read(bn, so ^ ST);
+                fa.read(af, so + HALF);
                 bar();
                 mfmas(H1{});
+                next_b0();
                 vm_wait<8>();
                 bar();
             }
             bar();
         } else {
-            PB pb;
-            pb.init(a.B, a.ldb, n0, a.N, a.K, wn, lane);
-            pb.stage(kt_of(0), wn, smem + B_OFF);
-            pb.stage(kt_of(1), wn, smem + B_OFF + B_ST);
+            PB0 p0;
+            PB1 p1;
+            p0.init(a.B, a.ldb, n0, a.N, a.K, wn, lane);
+            p1.init(a.B, a.ldb, n0, a.N, a.K, wn, lane);
+            p0.stage(kt_of(0), wn, smem + B_OFF);
+            p1.stage(kt_of(0), wn, smem + B_OFF + HALF);
+            p0.stage(kt_of(1), wn, smem + B_OFF + ST);
+            p1.stage(kt_of(1), wn, smem + B_OFF + ST + HALF);
             vm_wait<8>();
             bar();
+            fb.read(b0, 0);
+            bar();
+            p0.stage(kt_of(2), wn, smem + B_OFF);
             bar();
             for (int t = 0; t < nk; ++t) {
-                const int st = t & 1;
-                fb.read(bf, st * B_ST);
-                fa.read(af, st * A_ST);
+                const int so = (t & 1) * ST;
+                vm_wait<8>();
+                fb.read(b1, so + HALF);
+                fa.read(af, so);
                 bar();
-                pb.stage(kt_of(t + 2), wn, smem + B_OFF + st * B_ST);
+                p1.stage(kt_of(t + 2), wn, smem + B_OFF + so + HALF);
                 mfmas(H0{});
                 bar();
-                fa.read(af, st * A_ST + A_HALF);
                 vm_wait<8>();
+                fb.read(bn, so ^ ST);
+                fa.read(af, so + HALF);
                 bar();
+                p0.stage(kt_of(t + 3), wn, smem + B_OFF + (so ^ ST));
                 mfmas(H1{});
+                next_b0();
                 bar();
             }
         }
