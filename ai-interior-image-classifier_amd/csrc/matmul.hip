@@ -289,17 +289,84 @@ __device__ __forceinline__ void store_tile(const Matmul& a, f32x4 (&acc)[FM][4],
     }
 }
 
+// One step's fragment reads of the 256 x 256 tile: A's four fragments and B's two, 64 k each, from 128-wide half panels,
+// then TAIL (the barrier) and only then the wait: the reads land while the wave waits at the barrier. All of it is one
+// asm block, so no register of a read in flight is visible to the compiler.
+#define STEP_A_ROWS                                                                                       \
+    "ds_read_b128 %[a0], %[pa0]\n\tds_read_b128 %[a1], %[pa0] offset:2048\n\t"                            \
+    "ds_read_b128 %[a2], %[pa0] offset:4096\n\tds_read_b128 %[a3], %[pa0] offset:6144\n\t"                \
+    "ds_read_b128 %[a4], %[pa1]\n\tds_read_b128 %[a5], %[pa1] offset:2048\n\t"                            \
+    "ds_read_b128 %[a6], %[pa1] offset:4096\n\tds_read_b128 %[a7], %[pa1] offset:6144\n\t"
+#define STEP_B_ROWS                                                                                       \
+    "ds_read_b128 %[b0], %[pb0]\n\tds_read_b128 %[b1], %[pb0] offset:2048\n\t"                            \
+    "ds_read_b128 %[b2], %[pb1]\n\tds_read_b128 %[b3], %[pb1] offset:2048\n\t"
+// column panels of 128 columns: four k rows are 1024 bytes, 32 are 8192
+#define STEP_COL(d, e, f, g, p)                                                                           \
+    "ds_read_b64_tr_b16 %[" d "], %[" p "]\n\tds_read_b64_tr_b16 %[" e "], %[" p "] offset:1024\n\t"      \
+    "ds_read_b64_tr_b16 %[" f "], %[" p "] offset:8192\n\tds_read_b64_tr_b16 %[" g "], %[" p "] offset:9216\n\t"
+#define STEP_A_COLS                                                                                       \
+    STEP_COL("a0", "a1", "a8", "a9", "pa0") STEP_COL("a2", "a3", "aa", "ab", "pa1")                       \
+    STEP_COL("a4", "a5", "ac", "ad", "pa2") STEP_COL("a6", "a7", "ae", "af", "pa3")
+#define STEP_B_COLS STEP_COL("b0", "b1", "b4", "b5", "pb0") STEP_COL("b2", "b3", "b6", "b7", "pb1")
+#define OUT_A_ROWS                                                                                        \
+    [a0] "=&v"(a[0][0]), [a1] "=&v"(a[0][1]), [a2] "=&v"(a[0][2]), [a3] "=&v"(a[0][3]), [a4] "=&v"(a[1][0]),  \
+    [a5] "=&v"(a[1][1]), [a6] "=&v"(a[1][2]), [a7] "=&v"(a[1][3])
+#define OUT_B_ROWS [b0] "=&v"(b[0][0]), [b1] "=&v"(b[0][1]), [b2] "=&v"(b[1][0]), [b3] "=&v"(b[1][1])
+#define OUT_A_COLS                                                                                        \
+    [a0] "=&v"(ra[0]), [a1] "=&v"(ra[1]), [a2] "=&v"(ra[2]), [a3] "=&v"(ra[3]), [a4] "=&v"(ra[4]),       \
+    [a5] "=&v"(ra[5]), [a6] "=&v"(ra[6]), [a7] "=&v"(ra[7]), [a8] "=&v"(ra[8]), [a9] "=&v"(ra[9]),       \
+    [aa] "=&v"(ra[10]), [ab] "=&v"(ra[11]), [ac] "=&v"(ra[12]), [ad] "=&v"(ra[13]), [ae] "=&v"(ra[14]),  \
+    [af] "=&v"(ra[15])
+#define OUT_B_COLS                                                                                        \
+    [b0] "=&v"(rb[0]), [b1] "=&v"(rb[1]), [b2] "=&v"(rb[2]), [b3] "=&v"(rb[3]), [b4] "=&v"(rb[4]),       \
+    [b5] "=&v"(rb[5]), [b6] "=&v"(rb[6]), [b7] "=&v"(rb[7])
+#define IN_A_ROWS [pa0] "v"(fa.addr[0] + sa), [pa1] "v"(fa.addr[1] + sa)
+#define IN_A_COLS [pa0] "v"(fa.addr[0] + sa), [pa1] "v"(fa.addr[1] + sa), [pa2] "v"(fa.addr[2] + sa), [pa3] "v"(fa.addr[3] + sa)
+#define IN_B [pb0] "v"(fb.addr[0] + sb), [pb1] "v"(fb.addr[1] + sb)
+#define STEP_ASM(READS, TAIL, OUTS, INS) asm volatile(READS TAIL "s_barrier\n\ts_waitcnt lgkmcnt(0)" : OUTS : INS : "memory")
+#define COMMA ,
+#define STEP(TAIL)                                                                                                           \
+    if constexpr (AK && BK) STEP_ASM(STEP_B_ROWS STEP_A_ROWS, TAIL, OUT_B_ROWS COMMA OUT_A_ROWS, IN_B COMMA IN_A_ROWS);        \
+    else if constexpr (AK) STEP_ASM(STEP_B_COLS STEP_A_ROWS, TAIL, OUT_B_COLS COMMA OUT_A_ROWS, IN_B COMMA IN_A_ROWS);         \
+    else if constexpr (BK) STEP_ASM(STEP_B_ROWS STEP_A_COLS, TAIL, OUT_B_ROWS COMMA OUT_A_COLS, IN_B COMMA IN_A_COLS);         \
+    else STEP_ASM(STEP_B_COLS STEP_A_COLS, TAIL, OUT_B_COLS COMMA OUT_A_COLS, IN_B COMMA IN_A_COLS);
+// VM8: also waits until at most eight of the wave's loads are in flight before the barrier
+template <typename T, bool AK, bool BK, bool VM8>
+__device__ __forceinline__ void read_step(const Frags<T, AK, 128, 4>& fa, unsigned sa, typename T::vec8 (&a)[2][4], const Frags<T, BK, 128, 2>& fb,
+                                          unsigned sb, typename T::vec8 (&b)[2][2]) {
+    typedef typename T::vec8 vec8;
+    u32x2 ra[AK ? 1 : 16], rb[BK ? 1 : 8];
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (VM8) {
+        STEP("s_waitcnt vmcnt(8)\n\t")
+    } else {
+        STEP("")
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (!AK) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            a[i >> 2][i & 3] = __builtin_bit_cast(vec8, (u32x4){ra[2 * i].x, ra[2 * i].y, ra[2 * i + 1].x, ra[2 * i + 1].y});
+    }
+    if constexpr (!BK) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            b[i >> 1][i & 1] = __builtin_bit_cast(vec8, (u32x4){rb[2 * i].x, rb[2 * i].y, rb[2 * i + 1].x, rb[2 * i + 1].y});
+    }
+}
+
 // 256 x 256 tiles. Eight waves in two groups of four, one barrier apart: while one group issues 32 MFMAs the other
-// reads fragments and stages. A k-tile T is two steps: step (T, 0) computes the group's first 64 rows, (T, 1) its other
-// 64. B's fragments stay in registers for both; to balance the reads (twelve ds_read_b128 a step, under the 512 cycles
-// of the other group's MFMAs), step (T, 0) reads A's first half and B's second 32 columns of T, step (T, 1) A's second
-// half and B's first 32 columns of T + 1. Slot = barrier interval; group g reads step (T, h) in slot 4 T + 2 h + g and
-// computes it in the next one. LDS holds two k-tiles; each half panel is refilled as soon as both groups have read it:
-//  * A0(T), read in slots 4 T and 4 T + 1, by A0(T + 2) in slot 4 T + 2; A1(T), read in 4 T + 2 and 4 T + 3, by A1(T + 2)
-//    in slot 4 T + 4: group 0, at the start of its read segments. It waits for its four oldest pieces (eight younger
-//    ones may fly) at the end of each of its MFMA segments, six slots after their issue.
-//  * B0(T + 1), read in slots 4 T + 2 and 4 T + 3, by B0(T + 3) in slot 4 T + 4; B1(T), read in 4 T and 4 T + 1, by
-//    B1(T + 2) in slot 4 T + 2: group 1, at the start of its MFMA segments. It waits likewise in its read segments.
+// reads its next fragments. A k-tile T is two steps: step (T, 0) computes the group's first 64 rows, (T, 1) its other
+// 64. B's fragments stay in registers for both; to balance the reads, step (T, 0) reads A's first half and B's second
+// 32 columns of T, step (T, 1) A's second half and B's first 32 columns of T + 1. Slot = barrier interval; group g
+// issues the reads of step (T, h) in slot 4 T + 2 h + g, has them at the start of the next slot and computes there.
+// LDS holds two k-tiles. A part read in slots s (group 0) and s + 1 (group 1) is out of every wave's reads before the
+// barrier that ends slot s + 2, and is refilled from slot s + 3 on:
+//  * A0(T), read in 4 T and 4 T + 1, by A0(T + 2) in slot 4 T + 3; A1(T - 1), read in 4 T - 2 and 4 T - 1, by A1(T + 1) in
+//    slot 4 T + 1: group 0, at the start of its MFMA segments. At their end it waits for its four oldest pieces (eight
+//    younger ones may fly): five slots after their issue, one before their first read.
+//  * B0(T), read in 4 T - 2 and 4 T - 1, by B0(T + 2) in slot 4 T + 1; B1(T), read in 4 T and 4 T + 1, by B1(T + 2) in
+//    slot 4 T + 3: group 1, in its read segments, where it also waits, five slots after the issue.
 // Steps past the last k-tile stage zeros into parts nobody reads (kept, so that the counted waits hold).
 template <typename T, bool AK, bool BK>
 __global__ __launch_bounds__(512, 1) void matmul256_kernel(Matmul a, float* part, int N4, int kslice) {
@@ -367,17 +434,13 @@ __global__ __launch_bounds__(512, 1) void matmul256_kernel(Matmul a, float* part
             bar();
             for (int t = 0; t < nk; ++t) {
                 const int so = (t & 1) * ST;
+                read_step<T, AK, BK, false>(fa, so, af, fb, so + HALF, b1);
                 p1.stage(kt_of(t + 1), wn, smem + (so ^ ST) + HALF);
-                fb.read(b1, so + HALF);
-                fa.read(af, so);
-                bar();
                 mfmas(H0{});
                 vm_wait<8>();
                 bar();
+                read_step<T, AK, BK, false>(fa, so + HALF, af, fb, so ^ ST, bn);
                 p0.stage(kt_of(t + 2), wn, smem + so);
-                fb.read(bn, so ^ ST);
-                fa.read(af, so + HALF);
-                bar();
                 mfmas(H1{});
                 next_b0();
                 vm_wait<8>();
@@ -397,22 +460,15 @@ __global__ __launch_bounds__(512, 1) void matmul256_kernel(Matmul a, float* part
             bar();
             fb.read(b0, 0);
             bar();
-            p0.stage(kt_of(2), wn, smem + B_OFF);
             bar();
             for (int t = 0; t < nk; ++t) {
                 const int so = (t & 1) * ST;
-                vm_wait<8>();
-                fb.read(b1, so + HALF);
-                fa.read(af, so);
-                bar();
-                p1.stage(kt_of(t + 2), wn, smem + B_OFF + so + HALF);
+                p0.stage(kt_of(t + 2), wn, smem + B_OFF + so);
+                read_step<T, AK, BK, true>(fa, so, af, fb, so + HALF, b1);
                 mfmas(H0{});
                 bar();
-                vm_wait<8>();
-                fb.read(bn, so ^ ST);
-                fa.read(af, so + HALF);
-                bar();
-                p0.stage(kt_of(t + 3), wn, smem + B_OFF + (so ^ ST));
+                p1.stage(kt_of(t + 2), wn, smem + B_OFF + so + HALF);
+                read_step<T, AK, BK, true>(fa, so + HALF, af, fb, so ^ ST, bn);
                 mfmas(H1{});
                 next_b0();
                 bar();
