@@ -123,6 +123,7 @@ struct Epilogue {
     int M, N;
     int bias_f32, act;
     int vec;               // every 8-column group of y, res and slope rows is 16-byte aligned
+    int nt;                // store y and slope past the caches' retention (outputs far larger than the L2s)
     Dropout drop;
     // low-rank term u v^T (u [M, R], v [N, R], both zero-padded to R % 32 == 0 columns); low_mask: the
     // dropout mask (scale 1) is applied to this term instead of the activation's value
@@ -140,21 +141,15 @@ __device__ __forceinline__ void bias_cols(const Epilogue& e, int n, float (&b)[C
     }
 }
 
-// C consecutive columns n .. n + C - 1 (n % C == 0) of row m: v = acc (+ an unmasked low-rank term), b their
-// bias, t = the masked low-rank term (LOW) or unused. Columns at or past N are not touched.
-template <typename T, int C, bool LOW>
-__device__ __forceinline__ void epilogue_cols(const Epilogue& e, const uint2& off, int m, int n, float (&v)[C], const float (&b)[C], float (&t)[C]) {
+// C consecutive columns n .. n + C - 1 (n % C == 0) of row m: v = acc (+ the low-rank term), b their bias. Columns at or
+// past N are not touched.
+template <typename T, int C>
+__device__ __forceinline__ void epilogue_cols(const Epilogue& e, const uint2& off, int m, int n, float (&v)[C], const float (&b)[C]) {
     const int nc = min(C, e.N - n);
     if (m >= e.M || nc <= 0) return;
     const bool whole = nc == C && e.vec;
 #pragma unroll
     for (int j = 0; j < C; ++j) v[j] += b[j];
-    if constexpr (LOW) {
-#pragma unroll
-        for (int j = 0; j < C; j += 4) drop4(e.drop, off, m, n + j, 1.0f, t[j], t[j + 1], t[j + 2], t[j + 3]);
-#pragma unroll
-        for (int j = 0; j < C; ++j) v[j] += t[j];
-    }
     if (e.act != ACT_NONE) {
         float gr[C];
         if (e.slope) {
@@ -185,7 +180,7 @@ __device__ __forceinline__ void epilogue_cols(const Epilogue& e, const uint2& of
             act_cols<false, C>(e.act, v, gr);
         }
     }
-    if (!LOW && e.drop.on) {
+    if (e.drop.on && !e.low_mask) {
 #pragma unroll
         for (int j = 0; j < C; j += 4) drop4(e.drop, off, m, n + j, e.drop.scale, v[j], v[j + 1], v[j + 2], v[j + 3]);
     }

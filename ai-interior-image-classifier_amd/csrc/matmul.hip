@@ -16,8 +16,8 @@
 // Ragged edges: rows past the matrix and k past K lie outside the buffer resource (or get an offset that
 // does) and read as zeros.
 //
-// Epilogue: each wave passes its accumulators, 16 rows x 64 columns at a time, through 4 KB of LDS of its own
-// (chunks XORed with the row: no conflicts), and continues with eight consecutive columns a lane: 128 contiguous
+// Epilogue: each wave passes its accumulators, 64 rows x 64 columns at a time, through a part of the stages' LDS of its
+// own (chunks XORed with the row: no conflicts), and continues with eight consecutive columns a lane: 128 contiguous
 // bytes a row for the 16-bit residual, slope and output, whole groups of four for the dropout counter.
 #include <type_traits>
 
@@ -211,39 +211,29 @@ __device__ __forceinline__ void bar() {
 }
 
 // acc[i][j]: rows mw + 16 i .., columns nw + 16 j .. of C, in the MFMA's layout (lane: row lane & 15, columns
-// 4 (lane >> 4) .. + 3). eb: this wave's 4 KB of LDS. part != null: the slice's fp32 sums, row stride N4.
+// 4 (lane >> 4) .. + 3). eb: LDS of this wave's own, 4 KB for each of up to four fragment rows. part != null: the
+// slice's fp32 sums, row stride N4.
 template <typename T, int FM>
 __device__ __forceinline__ void store_tile(const Matmul& a, f32x4 (&acc)[FM][4], int mw, int nw, float* eb, float* part, int N4, int lane) {
     typedef typename T::vec8 vec8;
     const Epilogue& e = a.e;
+    constexpr int H = FM < 4 ? FM : 4;
     const int li = lane & 15, g = lane >> 4, er = lane >> 3, ec = lane & 7;
     const int n = nw + 8 * ec;
+    if (mw >= a.M || nw >= (part ? N4 : a.N)) return;
     const uint2 off = e.drop.on ? drop_offset(e.drop) : make_uint2(0, 0);
-    const bool low = !part && e.R > 0, masked = low && e.low_mask;
-    float b[8];
-    if (!part) bias_cols<T, 8>(e, n, b);
-    auto put = [&](const f32x4& v, int j) { *(f32x4*)(eb + li * 64 + (((4 * j + g) ^ li) << 2)) = v; };
-    auto get = [&](int row, float (&v)[8]) {
-        const f32x4 x = *(const f32x4*)(eb + row * 64 + (((2 * ec) ^ row) << 2)), y = *(const f32x4*)(eb + row * 64 + (((2 * ec + 1) ^ row) << 2));
+    if (!part && e.R > 0) {
+        // rank-R term, in the accumulators' layout: fragments straight from global memory (u and v rows are padded to
+        // 32 columns); its mask is one counter a lane and fragment
+        const u32x4 z = {0u, 0u, 0u, 0u};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            v[j] = x[j];
-            v[4 + j] = y[j];
-        }
-    };
-#pragma unroll 1
-    for (int i0 = 0; i0 < FM; ++i0) {
-        const int m0 = mw + 16 * i0;
-        if (m0 >= a.M) break;
-        float t[2][8];
-        if (low) {
-            // rank-R term: fragments straight from global memory (u and v rows are padded to 32 columns)
+        for (int i = 0; i < FM; ++i) {
+            const int m = mw + 16 * i + li;
             f32x4 tl[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) tl[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            const u32x4 z = {0u, 0u, 0u, 0u};
             for (int r = 0; r < e.R; r += 32) {
-                const u32x4 uf = m0 + li < a.M ? *(const u32x4*)(e.lu + (int64_t)(m0 + li) * e.R + r + 8 * g) : z;
+                const u32x4 uf = m < a.M ? *(const u32x4*)(e.lu + (int64_t)m * e.R + r + 8 * g) : z;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int c = nw + 16 * j + li;
@@ -252,38 +242,99 @@ __device__ __forceinline__ void store_tile(const Matmul& a, f32x4 (&acc)[FM][4],
                 }
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) put(tl[j], j);
-            get(er, t[0]);
-            get(8 + er, t[1]);
-        }
-        // (a rolled loop over a register array: uniform branches pick the fragment row)
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-            if (i == i0) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) put(acc[i][j], j);
+            for (int j = 0; j < 4; ++j) {
+                float t0 = tl[j][0], t1 = tl[j][1], t2 = tl[j][2], t3 = tl[j][3];
+                if (e.low_mask) drop4(e.drop, off, m, nw + 16 * j + 4 * g, 1.0f, t0, t1, t2, t3);
+                acc[i][j] += f32x4{t0, t1, t2, t3};
             }
+        }
+    }
+    auto get = [&](int row, float (&v)[8]) {
+        const f32x4 x = *(const f32x4*)(eb + row * 64 + (((2 * ec) ^ (row & 15)) << 2));
+        const f32x4 y = *(const f32x4*)(eb + row * 64 + (((2 * ec + 1) ^ (row & 15)) << 2));
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int row = 8 * h + er, m = m0 + row;
-            float v[8];
-            get(row, v);
-            if (part) {
+        for (int j = 0; j < 4; ++j) {
+            v[j] = x[j];
+            v[4 + j] = y[j];
+        }
+    };
+    float b[8];
+    if (!part) bias_cols<T, 8>(e, n, b);
+    const bool full = !part && e.vec && mw + 16 * FM <= a.M && nw + 64 <= a.N;
+    const int64_t r0 = mw + er;
+    u16* y = (u16*)e.y + r0 * e.ldy + n;
+    const u16* res = (const u16*)e.res + r0 * e.ldr + n;
+    short* sl = e.slope + r0 * e.N + n;
+    const bool drop = e.drop.on && !e.low_mask;
+#pragma unroll
+    for (int i0 = 0; i0 < FM; i0 += H) {
+#pragma unroll
+        for (int i = 0; i < H; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) *(f32x4*)(eb + (i * 16 + li) * 64 + (((4 * j + g) ^ li) << 2)) = acc[i0 + i][j];
+        const int mr = mw + 16 * i0;
+        if (part) {
+#pragma unroll 1
+            for (int s = 0; s < 2 * H; ++s) {
+                const int m = mr + 8 * s + er;
+                float v[8];
+                get(8 * s + er, v);
                 if (m < a.M && n < N4) {
                     float* o = part + (int64_t)m * N4 + n;
                     *(f32x4*)o = f32x4{v[0], v[1], v[2], v[3]};
                     if (n + 4 < N4) *(f32x4*)(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
                 }
-                continue;
             }
-            if (masked) {
-                epilogue_cols<T, 8, true>(e, off, m, n, v, b, t[h]);
-            } else {
-                if (low) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] += t[h][j];
+        } else if (full) {
+            // every row and column of the wave's part is inside C and 16-byte aligned
+#pragma unroll 2
+            for (int s = 0; s < 2 * H; ++s) {
+                float v[8], gr[8];
+                get(8 * s + er, v);
+                u32x4 rw;
+                if (e.res) {
+                    rw = *(const u32x4*)res;
+                    res += 8 * e.ldr;
                 }
-                epilogue_cols<T, 8, false>(e, off, m, n, v, b, t[h]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] += b[j];
+                if (e.act != ACT_NONE) {
+                    if (e.slope) {
+                        act_cols<true, 8>(e.act, v, gr);
+                        short q[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) q[j] = slope_encode(gr[j]);
+                        u32x4 w;
+                        __builtin_memcpy(&w, q, 16);
+                        if (e.nt) __builtin_nontemporal_store(w, (u32x4*)sl);
+                        else *(u32x4*)sl = w;
+                        sl += 8 * (int64_t)e.N;
+                    } else {
+                        act_cols<false, 8>(e.act, v, gr);
+                    }
+                }
+                if (drop) {
+                    const int m = mr + 8 * s + er;
+                    drop4(e.drop, off, m, n, e.drop.scale, v[0], v[1], v[2], v[3]);
+                    drop4(e.drop, off, m, n + 4, e.drop.scale, v[4], v[5], v[6], v[7]);
+                }
+                if (e.res) {
+                    u16 rr[8];
+                    __builtin_memcpy(rr, &rw, 16);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] += T::to_f32(rr[j]);
+                }
+                const u32x4 w = {pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7])};
+                if (e.nt) __builtin_nontemporal_store(w, (u32x4*)y);
+                else *(u32x4*)y = w;
+                y += 8 * e.ldy;
+            }
+        } else {
+#pragma unroll 1
+            for (int s = 0; s < 2 * H; ++s) {
+                float v[8];
+                get(8 * s + er, v);
+                epilogue_cols<T, 8>(e, off, mr + 8 * s + er, n, v, b);
             }
         }
     }
@@ -375,8 +426,8 @@ __global__ __launch_bounds__(512, 1) void matmul256_kernel(Matmul a, float* part
     using PA1 = Panel<AK, 128, 4, Half<1, 64>>;
     using PB0 = Panel<BK, 128, 4, Half<0, 32>>;
     using PB1 = Panel<BK, 128, 4, Half<1, 32>>;
-    constexpr int HALF = 16384, ST = 32768, B_OFF = 65536, E_OFF = 131072;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[E_OFF + 8 * 4096];
+    constexpr int HALF = 16384, ST = 32768, B_OFF = 65536;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[131072];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave >> 2, wn = wave & 3;
@@ -474,9 +525,10 @@ __global__ __launch_bounds__(512, 1) void matmul256_kernel(Matmul a, float* part
                 bar();
             }
         }
-        vm_wait<0>();  // no load into LDS outlives the workgroup
+        vm_wait<0>();  // no load into LDS outlives the k loop: the epilogue takes the stages over
+        bar();
     }
-    store_tile<T, 8>(a, acc, m0 + wm * 128, n0 + wn * 64, (float*)(smem + E_OFF) + wave * 1024,
+    store_tile<T, 8>(a, acc, m0 + wm * 128, n0 + wn * 64, (float*)smem + wave * 4096,
                      part ? part + (int64_t)blockIdx.y * a.M * N4 : nullptr, N4, lane);
 }
 
@@ -488,7 +540,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_kernel(Matmul a, float
     constexpr int A_ST = BM * 128, STAGE = (BM + BN) * 128;
     using PA = Panel<AK, BM, W, Whole>;
     using PB = Panel<BK, BN, W, Whole>;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[NS * STAGE + W * 4096];
+    __shared__ __attribute__((aligned(16))) unsigned char smem[NS * STAGE];
+    static_assert(NS * STAGE >= W * 4096 * FM, "the epilogue's LDS");
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
@@ -540,9 +593,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_kernel(Matmul a, float
             __builtin_amdgcn_s_setprio(0);
             st = st == NS - 1 ? 0 : st + 1;
         }
-        vm_wait<0>();  // no load into LDS outlives the workgroup
+        vm_wait<0>();  // no load into LDS outlives the k loop: the epilogue takes the stages over
+        bar();
     }
-    store_tile<T, FM>(a, acc, m0 + wm * FM * 16, n0 + wn * 64, (float*)(smem + NS * STAGE) + wave * 1024,
+    store_tile<T, FM>(a, acc, m0 + wm * FM * 16, n0 + wn * 64, (float*)smem + wave * FM * 1024,
                       part ? part + (int64_t)blockIdx.y * a.M * N4 : nullptr, N4, lane);
 }
 
@@ -557,23 +611,23 @@ __global__ __launch_bounds__(256) void matmul_join_kernel(Epilogue e, const floa
     const float* p = part + (int64_t)m * N4 + n;
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
     for (int z = 0; z < S; ++z) s += *(const f32x4*)(p + z * sl);
-    float v[4] = {s[0], s[1], s[2], s[3]}, t[4] = {0.f, 0.f, 0.f, 0.f};
+    float v[4] = {s[0], s[1], s[2], s[3]};
     const uint2 off = e.drop.on ? drop_offset(e.drop) : make_uint2(0, 0);
     if (e.R > 0) {
-        const u16 *u = e.lu + (int64_t)m * e.R;
+        float t[4] = {0.f, 0.f, 0.f, 0.f};
+        const u16* u = e.lu + (int64_t)m * e.R;
         for (int j = 0; j < 4; ++j) {
             if (n + j >= e.N) break;
             const u16* w = e.lv + (int64_t)(n + j) * e.R;
-            float d = 0.f;
-            for (int r = 0; r < e.R; ++r) d += T::to_f32(u[r]) * T::to_f32(w[r]);
-            if (e.low_mask) t[j] = d;
-            else v[j] += d;
+            for (int r = 0; r < e.R; ++r) t[j] += T::to_f32(u[r]) * T::to_f32(w[r]);
         }
+        if (e.low_mask) drop4(e.drop, off, m, n, 1.0f, t[0], t[1], t[2], t[3]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += t[j];
     }
     float b[4];
     bias_cols<T, 4>(e, n, b);
-    if (e.R > 0 && e.low_mask) epilogue_cols<T, 4, true>(e, off, m, n, v, b, t);
-    else epilogue_cols<T, 4, false>(e, off, m, n, v, b, t);
+    epilogue_cols<T, 4>(e, off, m, n, v, b);
 }
 
 // an operand whose rows the 16-byte loads cannot address (odd length, stride or base): copied to rows of
@@ -701,6 +755,7 @@ int launch_matmul(hipStream_t s, int dtype, const Matmul& a0, void* ws, size_t w
     a.e.vec = ((size_t)a.e.y & 15) == 0 && a.e.ldy % 8 == 0 &&
               (!a.e.res || (((size_t)a.e.res & 15) == 0 && a.e.ldr % 8 == 0)) &&
               (!a.e.slope || (((size_t)a.e.slope & 15) == 0 && a.N % 8 == 0));
+    a.e.nt = (int64_t)a.M * a.N * 2 >= (int64_t)64 << 20;
     if (dtype == 1) launch_typed<BF16>(s, a, p, part);
     else launch_typed<F16>(s, a, p, part);
     return 0;
