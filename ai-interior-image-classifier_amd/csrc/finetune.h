@@ -121,6 +121,7 @@ struct Epilogue {
     short* slope;          // [M, N] contiguous (row stride N) or null
     int64_t ldy, ldr;
     int M, N;
+    int m_base;            // row of the whole operand that row 0 is (the dropout counter's)
     int bias_f32, act;
     int vec;               // every 8-column group of y, res and slope rows is 16-byte aligned
     int nt;                // store y and slope past the caches' retention (outputs far larger than the L2s)
@@ -182,7 +183,7 @@ __device__ __forceinline__ void epilogue_cols(const Epilogue& e, const uint2& of
     }
     if (e.drop.on && !e.low_mask) {
 #pragma unroll
-        for (int j = 0; j < C; j += 4) drop4(e.drop, off, m, n + j, e.drop.scale, v[j], v[j + 1], v[j + 2], v[j + 3]);
+        for (int j = 0; j < C; j += 4) drop4(e.drop, off, e.m_base + m, n + j, e.drop.scale, v[j], v[j + 1], v[j + 2], v[j + 3]);
     }
     u16* y = (u16*)e.y + (int64_t)m * e.ldy + n;
     const u16* r = e.res ? (const u16*)e.res + (int64_t)m * e.ldr + n : nullptr;

@@ -172,8 +172,10 @@ __global__ __launch_bounds__(256) void db_kernel(const float* __restrict__ part,
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const int n = blockIdx.x * 32 + tx;
     float s = 0.f;
-    if (n < N)
+    if (n < N) {
+#pragma unroll 8
         for (int b = ty; b < blocks; b += 8) s += part[(int64_t)b * N + n];
+    }
     sums[ty][tx] = s;
     __syncthreads();
     if (ty || n >= N) return;
@@ -202,10 +204,12 @@ __global__ __launch_bounds__(256) void pad_kernel(PadArgs a, PadArgs b, int bloc
 }
 
 // ---- thin product u[m, r] = alpha sum_k mask(x)[m, k] f[r, k], 32 ranks a launch row ----
-// One workgroup: 16 rows of x, its four waves a quarter of k each, so x is read once, by 16-byte loads
-// straight into the MFMA fragment (lane: row lane & 15, eight k at 8 (lane >> 4)); the quarters meet in LDS.
+// One workgroup: 16 rows of x, its four waves a quarter of k each, so x is read once, by 16-byte loads straight into the
+// MFMA fragment (lane: row lane & 15). Steps are 64 deep: lane group g takes k 16 g .. 16 g + 15 of it as two fragments
+// (the order of k inside a step is free, f is read in the same one), so the first load touches every whole 128-byte
+// line of the 16 rows (against 64 bytes a row and step: 18464 x 4096 73 -> 42 us). The quarters meet in LDS.
 struct DownArgs {
-    const u16 *x, *f;  // x [M, K] row stride ldx; f [R, K] row stride ldf, rows past r and columns past K zero
+    const u16 *x, *f;  // x [M, K] row stride ldx; f [R, K] row stride ldf, rows past r and columns past K (to 64) zero
     u16* u;            // [M, R]
     int64_t ldx, ldf;
     int M, K, R, vec;
@@ -219,36 +223,49 @@ __global__ __launch_bounds__(256) void lora_down_kernel(DownArgs a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int li = lane & 15, g = lane >> 4;
     const int m = blockIdx.x * 16 + li, r0 = blockIdx.y * 32;
-    const int nk = (a.K + 31) >> 5, k0 = nk * wave / 4, k1 = nk * (wave + 1) / 4;
-    const u16* xr = a.x + (int64_t)m * a.ldx;
+    const int nk = (a.K + 63) >> 6, k0 = nk * wave / 4, k1 = nk * (wave + 1) / 4;
+    const u16* xr = a.x + (int64_t)min(m, a.M - 1) * a.ldx;
     const u16* f0 = a.f + (int64_t)(r0 + li) * a.ldf;
     const u16* f1 = f0 + 16 * a.ldf;
     const uint2 off = drop_offset(a.d);
     f32x4 c0 = {0.f, 0.f, 0.f, 0.f}, c1 = c0;
-#pragma unroll 4
-    for (int kt = k0; kt < k1; ++kt) {
-        const int k = kt * 32 + 8 * g;
+    auto mask = [&](u16 (&v)[8], int k) {
+        const uint4 p = philox4((unsigned)k >> 2, (unsigned)m, off.x, off.y, a.d.k0, a.d.k1);
+        const uint4 q = philox4(((unsigned)k >> 2) + 1, (unsigned)m, off.x, off.y, a.d.k0, a.d.k1);
+        const unsigned w[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = w[j] > a.d.drop_max ? v[j] : (u16)0;
+    };
+    auto step = [&](const uint4& x, int k) {
         u16 v[8];
-        const int n = m < a.M ? min(8, a.K - k) : 0;
-        if (a.vec && n == 8) {
-            const uint4 w = *(const uint4*)(xr + k);
-            __builtin_memcpy(v, &w, 16);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = j < n ? xr[k + j] : (u16)0;
-        }
-        if (a.d.on) {
-            const uint4 p = philox4((unsigned)k >> 2, (unsigned)m, off.x, off.y, a.d.k0, a.d.k1);
-            const uint4 q = philox4(((unsigned)k >> 2) + 1, (unsigned)m, off.x, off.y, a.d.k0, a.d.k1);
-            const unsigned w[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = w[j] > a.d.drop_max ? v[j] : (u16)0;
-        }
+        __builtin_memcpy(v, &x, 16);
+        if (a.d.on) mask(v, k);
         vec8 xf;
         __builtin_memcpy(&xf, v, 16);
-        const vec8 p0 = *(const vec8*)(f0 + k), p1 = *(const vec8*)(f1 + k);
-        c0 = T::mfma16(p0, xf, c0);  // lane: row m, ranks 4 g .. 4 g + 3
-        c1 = T::mfma16(p1, xf, c1);
+        c0 = T::mfma16(*(const vec8*)(f0 + k), xf, c0);  // lane: row m, ranks 4 g .. 4 g + 3
+        c1 = T::mfma16(*(const vec8*)(f1 + k), xf, c1);
+    };
+    // (rows past M repeat the last one and are not stored)
+    const int whole = a.vec ? a.K >> 6 : 0;  // steps of 64 whole columns
+    int kt = k0;
+#pragma unroll 4
+    for (; kt < min(k1, whole); ++kt) {
+        const int k = kt * 64 + 16 * g;
+        const uint4 x0 = *(const uint4*)(xr + k), x1 = *(const uint4*)(xr + k + 8);
+        step(x0, k);
+        step(x1, k + 8);
+    }
+    for (; kt < k1; ++kt) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int k = kt * 64 + 16 * g + 8 * h;
+            u16 v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = k + j < a.K ? xr[k + j] : (u16)0;
+            uint4 x;
+            __builtin_memcpy(&x, v, 16);
+            step(x, k);
+        }
     }
     if (wave) {
 #pragma unroll
@@ -383,16 +400,21 @@ __global__ __launch_bounds__(256) void lora_grad_kernel(GradArgs a) {
             if (c < a.C4) *(f32x4*)(a.part + ((int64_t)blockIdx.z * a.R + r0 + 16 * i + li) * a.C4 + c) = acc[i][j];
         }
 }
-// the slices' sums in order; out[c, r] (or [r, c]) by strides, r < rank
+// the slices' sums in order; out[c, r] (or [r, c]) by strides, r < rank; four columns a thread
 template <typename T>
 __global__ __launch_bounds__(256) void lora_grad_join_kernel(const float* __restrict__ part, int slices, int R, int C, int C4, int rank,
                                                              u16* out, int64_t so_c, int64_t so_r) {
+    const int q = C4 >> 2;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int r = (int)(i / C), c = (int)(i - (int64_t)r * C);
+    const int r = (int)(i / q), c = (int)(i - (int64_t)r * q) * 4;
     if (r >= rank) return;
-    float s = 0.f;
-    for (int z = 0; z < slices; ++z) s += part[((int64_t)z * R + r) * C4 + c];
-    out[c * so_c + r * so_r] = T::from_f32(s);
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    const float* p = part + (int64_t)r * C4 + c;
+#pragma unroll 8
+    for (int z = 0; z < slices; ++z) s += *(const f32x4*)(p + (int64_t)z * R * C4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (c + j < C) out[(c + j) * so_c + r * so_r] = T::from_f32(s[j]);
 }
 
 // ---- host side ----
@@ -487,8 +509,10 @@ Db make_dz(const void* dy, int64_t dy_stride, const int16_t* slope, void* dz, in
     DzArgs& d = b.d;
     b.db = db;
     b.db_f32 = db_f32;
-    // blocks of at least 64 rows, at most 512 of them
-    b.blocks = (int)((M + 63) / 64 < 512 ? (M + 63) / 64 : 512);
+    // about 2048 workgroups of 256 columns and at least 8 rows (fewer rows a block fill the chip on small products:
+    // 1237 x 437 21 -> 8 us; fewer blocks shorten the join: 36928 x 4096 23 -> 6 us)
+    const int64_t most = 2048 / ((N + 255) / 256 ? (N + 255) / 256 : 1), need = (M + 7) / 8;
+    b.blocks = (int)(need < most ? need : most > 1 ? most : (M ? 1 : 0));
     d.rows = b.blocks ? (int)up((M + b.blocks - 1) / b.blocks, 8) : 8;
     d.dy = dy;
     d.slope = slope;
@@ -650,7 +674,7 @@ void launch_grad(hipStream_t s, bool bf, const void* x, int64_t ldx, const void*
         if (bf) lora_grad_kernel<BF16><<<grid, 256, 0, s>>>(d);
         else lora_grad_kernel<F16><<<grid, 256, 0, s>>>(d);
     }
-    const unsigned g = (unsigned)((rank * C + 255) / 256);
+    const unsigned g = (unsigned)((rank * (up(C, 4) / 4) + 255) / 256);
     if (bf) lora_grad_join_kernel<BF16><<<g, 256, 0, s>>>(d.part, slices, d.R, d.C, d.C4, (int)rank, (u16*)out, so_c, so_r);
     else lora_grad_join_kernel<F16><<<g, 256, 0, s>>>(d.part, slices, d.R, d.C, d.C4, (int)rank, (u16*)out, so_c, so_r);
 }
@@ -674,7 +698,7 @@ int lora_of(const clipvit_lora_args* a, Lora& l, Arena& ws) {
     }
     if (!make_matmul(l.y, a->x, a->x_stride, 1, a->w, a->w_stride[0], a->w_stride[1], a->M, a->N, a->K, a->y, a->N))
         FT_FAIL(CLIPVIT_E_INVALID, std::string("lora_linear: ") + OPERANDS);
-    l.f = ws.take((size_t)R * up(a->K, 32) * 2);
+    l.f = ws.take((size_t)R * up(a->K, 64) * 2);
     l.v = ws.take((size_t)a->N * R * 2);
     Epilogue& e = l.y.e;
     e.bias = a->bias;
@@ -709,7 +733,7 @@ int lora_grad_of(const clipvit_lora_grad_args* a, LoraGrad& g, Arena& ws) {
         FT_FAIL(CLIPVIT_E_INVALID, "lora_linear_grad: row stride");
     const Dropout none{};
     if (g.want_du) {
-        g.f = ws.take((size_t)R * up(a->N, 32) * 2);
+        g.f = ws.take((size_t)R * up(a->N, 64) * 2);
         g.v = ws.take((size_t)a->K * R * 2);
         g.du = ws.take((size_t)a->M * R * 2);
     }
@@ -879,7 +903,7 @@ int clipvit_lora_linear(void* stream, const clipvit_lora_args* a, void* workspac
         if (!a->M || !a->N) return CLIPVIT_OK;
         if (bad_workspace(ws, workspace, bytes)) FT_FAIL(CLIPVIT_E_INVALID, std::string("lora_linear: ") + WORKSPACE);
         hipStream_t s = (hipStream_t)stream;
-        const int64_t R = rank32(a->rank), Kp = up(a->K, 32);
+        const int64_t R = rank32(a->rank), Kp = up(a->K, 64);
         const Dropout drop = make_dropout(a->dropout);
         launch_pad(s, pad_of(a->a, a->a_stride[1], a->a_stride[0], a->rank, a->K, R, Kp, l.f),
                    pad_of(a->b, a->b_stride[1], a->b_stride[0], a->N, a->rank, a->N, R, l.v));
@@ -909,7 +933,7 @@ int clipvit_lora_linear_grad(void* stream, const clipvit_lora_grad_args* a, void
         if (bad_workspace(ws, workspace, bytes)) FT_FAIL(CLIPVIT_E_INVALID, std::string("lora_linear_grad: ") + WORKSPACE);
         hipStream_t s = (hipStream_t)stream;
         const bool bf = a->dtype == CLIPVIT_BF16;
-        const int64_t R = rank32(a->rank), Np = up(a->N, 32);
+        const int64_t R = rank32(a->rank), Np = up(a->N, 64);
         const Dropout drop = make_dropout(a->dropout), none{};
         if (g.want_du) {
             launch_pad(s, pad_of(a->b, a->b_stride[0], a->b_stride[1], a->rank, a->N, R, Np, g.f),

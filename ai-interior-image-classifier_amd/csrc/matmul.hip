@@ -226,26 +226,25 @@ __device__ __forceinline__ void store_tile(const Matmul& a, f32x4 (&acc)[FM][4],
         // rank-R term, in the accumulators' layout: fragments straight from global memory (u and v rows are padded to
         // 32 columns); its mask is one counter a lane and fragment
         const u32x4 z = {0u, 0u, 0u, 0u};
-#pragma unroll
-        for (int i = 0; i < FM; ++i) {
-            const int m = mw + 16 * i + li;
-            f32x4 tl[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) tl[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            for (int r = 0; r < e.R; r += 32) {
-                const u32x4 uf = m < a.M ? *(const u32x4*)(e.lu + (int64_t)m * e.R + r + 8 * g) : z;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int c = nw + 16 * j + li;
-                    const u32x4 vf = c < a.N ? *(const u32x4*)(e.lv + (int64_t)c * e.R + r + 8 * g) : z;
-                    tl[j] = T::mfma16(__builtin_bit_cast(vec8, vf), __builtin_bit_cast(vec8, uf), tl[j]);
-                }
-            }
+#pragma unroll 1
+        for (int r = 0; r < e.R; r += 32) {
+            vec8 vf[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                float t0 = tl[j][0], t1 = tl[j][1], t2 = tl[j][2], t3 = tl[j][3];
-                if (e.low_mask) drop4(e.drop, off, m, nw + 16 * j + 4 * g, 1.0f, t0, t1, t2, t3);
-                acc[i][j] += f32x4{t0, t1, t2, t3};
+                const int c = nw + 16 * j + li;
+                vf[j] = __builtin_bit_cast(vec8, c < a.N ? *(const u32x4*)(e.lv + (int64_t)c * e.R + r + 8 * g) : z);
+            }
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+                const int m = mw + 16 * i + li;
+                const vec8 uf = __builtin_bit_cast(vec8, m < a.M ? *(const u32x4*)(e.lu + (int64_t)m * e.R + r + 8 * g) : z);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const f32x4 t = T::mfma16(vf[j], uf, f32x4{0.f, 0.f, 0.f, 0.f});
+                    float t0 = t[0], t1 = t[1], t2 = t[2], t3 = t[3];
+                    if (e.low_mask) drop4(e.drop, off, e.m_base + m, nw + 16 * j + 4 * g, 1.0f, t0, t1, t2, t3);
+                    acc[i][j] += f32x4{t0, t1, t2, t3};
+                }
             }
         }
     }
@@ -314,7 +313,7 @@ __device__ __forceinline__ void store_tile(const Matmul& a, f32x4 (&acc)[FM][4],
                     }
                 }
                 if (drop) {
-                    const int m = mr + 8 * s + er;
+                    const int m = e.m_base + mr + 8 * s + er;
                     drop4(e.drop, off, m, n, e.drop.scale, v[0], v[1], v[2], v[3]);
                     drop4(e.drop, off, m, n + 4, e.drop.scale, v[4], v[5], v[6], v[7]);
                 }
@@ -621,7 +620,7 @@ __global__ __launch_bounds__(256) void matmul_join_kernel(Epilogue e, const floa
             const u16* w = e.lv + (int64_t)(n + j) * e.R;
             for (int r = 0; r < e.R; ++r) t[j] += T::to_f32(u[r]) * T::to_f32(w[r]);
         }
-        if (e.low_mask) drop4(e.drop, off, m, n, 1.0f, t[0], t[1], t[2], t[3]);
+        if (e.low_mask) drop4(e.drop, off, e.m_base + m, n, 1.0f, t[0], t[1], t[2], t[3]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] += t[j];
     }
@@ -630,45 +629,73 @@ __global__ __launch_bounds__(256) void matmul_join_kernel(Epilogue e, const floa
     epilogue_cols<T, 4>(e, off, m, n, v, b);
 }
 
-// an operand whose rows the 16-byte loads cannot address (odd length, stride or base): copied to rows of
-// `cp` elements (a multiple of 8), zero padded; 8 elements a thread
-__global__ __launch_bounds__(256) void repack_kernel(const u16* __restrict__ src, int64_t ld, int rows, int cols, u16* __restrict__ dst, int cp) {
-    const int cq = cp >> 3;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+// operands whose rows the 16-byte loads cannot address (odd length, stride or base), up to two a launch: copied to
+// rows of `cp` elements (a multiple of 8), zero padded; 8 elements a thread
+struct RepackArgs {
+    const u16* src;
+    int64_t ld;
+    int rows, cols;
+    u16* dst;
+    int cp;
+};
+__global__ __launch_bounds__(256) void repack_kernel(RepackArgs a, RepackArgs b, int blocks_a) {
+    const bool first = (int)blockIdx.x < blocks_a;
+    const RepackArgs& p = first ? a : b;
+    const int cq = p.cp >> 3;
+    const int64_t i = ((int64_t)blockIdx.x - (first ? 0 : blocks_a)) * 256 + threadIdx.x;
     const int64_t r = i / cq;
     const int c = (int)(i - r * cq) * 8;
-    if (r >= rows) return;
-    const u16* s = src + r * ld + c;
+    if (r >= p.rows) return;
+    const u16* s = p.src + r * p.ld + c;
     u16 v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? s[j] : (u16)0;
+    for (int j = 0; j < 8; ++j) v[j] = c + j < p.cols ? s[j] : (u16)0;
     uint4 w;
     __builtin_memcpy(&w, v, 16);
-    *(uint4*)(dst + r * cp + c) = w;
+    *(uint4*)(p.dst + r * p.cp + c) = w;
 }
 
 bool loadable(const u16* p, int64_t ld, int len) { return ((size_t)p & 15) == 0 && ld % 8 == 0 && len % 8 == 0; }
 
+// One launch: tile (0 = 64 x 64, 1 = 128 x 128, 2 = 256 x 256), slices of k, and its estimated time.
+struct Part {
+    int rows, tile, S, kslice;
+    double us;
+};
 struct Plan {
     size_t a_bytes, b_bytes, part_bytes;
-    int tile, S, ksteps, N4;  // tile: 0 = 64 x 64, 1 = 128 x 128, 2 = 256 x 256
+    int N4, parts;
+    Part part[2];  // rows [0, part[0].rows), then the rest
 };
 
 int tiles(int M, int N, int t) { return ((M + t - 1) / t) * ((N + t - 1) / t); }
 
 // Estimated time of a launch: rounds of workgroups times (k-tiles of a slice x time of one + start and epilogue),
-// and the join of a split. Fitted to forward products measured at every (tile, slices) on 12 shapes, M x K x N: e.g.
-// 12608 x 4096 x 1024 64 / 128 / 256-wide tiles 170 / 107 / 115 us, 256 in two slices 144; 4928 x 512 x 2048 27 / 23 / 24 us;
-// 4096 x 36928 x 1024 256 in 1 / 2 / 4 / 8 slices 864 / 452 / 275 / 297 us; 2048 x 4928 x 512 64 in 1 / 2 / 4 slices 27.5 / 24.0 / 26.9
+// and the join of a split. Fitted to products measured at every (tile, slices) on 12 shapes, M x K x N: e.g.
+// 12608 x 4096 x 1024 64 / 128 / 256-wide tiles 170 / 107 / 95 us, 256 in two slices 144; 4928 x 512 x 2048 27 / 23 / 22 us;
+// 4096 x 36928 x 1024 256 in 1 / 2 / 4 / 8 slices 864 / 452 / 272 / 297 us; 2048 x 4928 x 512 64 in 1 / 2 / 4 slices 27.5 / 24.0 / 26.9
 // us; 1237 x 768 x 440 7 / 13 / 26 us.
 double cost_us(int tile, int nt, int S, int ks, double out) {
     // one 256-wide workgroup a CU; two of the smaller ones, each slower beside the other than alone
-    static const double alone[3] = {0.30, 0.83, 1.60}, beside[3] = {0.43, 1.13, 1.60}, fixed[3] = {2.5, 4.0, 10.0};
+    static const double alone[3] = {0.30, 0.83, 1.42}, beside[3] = {0.43, 1.13, 1.42}, fixed[3] = {2.5, 4.0, 8.5};
     const int64_t wgs = (int64_t)nt * S, slots = tile == 2 ? 256 : 512, full = wgs / slots, rest = wgs % slots;
     double t = full * (ks * beside[tile] + fixed[tile]);
     if (rest) t += ks * (rest <= 256 ? alone[tile] : beside[tile]) + fixed[tile];
     if (S > 1) t += 5.0 + (S * 8.0 + 2.0) * out / 4.5e6;
     return t;
+}
+
+Part best_part(int M, int N, int nk, int N4) {
+    Part b{M, 0, 1, nk > 0 ? nk : 1, 1e30};
+    for (int t = 0; t < 3; ++t) {
+        const int nt = tiles(M, N, 64 << t);
+        for (int S = 1; S <= 64 && (S == 1 || (nk >= 2 * S && (int64_t)nt * S <= 1024)); ++S) {
+            const int ks = nk > 0 ? (nk + S - 1) / S : 1;
+            const double c = cost_us(t, nt, S, ks, (double)M * N4);
+            if (c < b.us) b = Part{M, t, nk > 0 ? (nk + ks - 1) / ks : 1, ks, c};
+        }
+    }
+    return b;
 }
 
 Plan plan_of(const Matmul& a) {
@@ -677,56 +704,75 @@ Plan plan_of(const Matmul& a) {
     auto up = [](int64_t v, int64_t q) { return (v + q - 1) / q * q; };
     if (a.K > 0 && !loadable(a.A, a.lda, al)) p.a_bytes = (size_t)up((int64_t)ar * up(al, 8) * 2, 256);
     if (a.K > 0 && !loadable(a.B, a.ldb, bl)) p.b_bytes = (size_t)up((int64_t)br * up(bl, 8) * 2, 256);
-    const int nk = (a.K + 63) / 64;
+    const int nk = (a.K + 63) / 64, nN = (a.N + 255) / 256, nM = (a.M + 255) / 256;
     p.N4 = (int)up(a.N, 4);
-    p.tile = 0;
-    p.S = 1;
-    p.ksteps = nk > 0 ? nk : 1;
-    double best = 1e30;
-    for (int t = 0; t < 3; ++t) {
-        const int nt = tiles(a.M, a.N, 64 << t);
-        for (int S = 1; S <= 64 && (S == 1 || (nk >= 2 * S && (int64_t)nt * S <= 1024)); ++S) {
-            const int ks = nk > 0 ? (nk + S - 1) / S : 1;
-            const double c = cost_us(t, nt, S, ks, (double)a.M * p.N4);
-            if (c < best) {
-                best = c;
-                p.tile = t;
-                p.ksteps = ks;
-                p.S = nk > 0 ? (nk + ks - 1) / ks : 1;
+    p.parts = 1;
+    p.part[0] = best_part(a.M, a.N, nk, p.N4);
+    // whole rounds of 256-wide tiles as one launch and the remaining rows as another with tiles of its own, where
+    // that is estimated faster (the launch itself 3 us): 36928 x 4096 x 1024 is 580 tiles, 2.3 rounds in the time of 3
+    const int round_rows = nN <= 256 ? 256 / nN : 0;  // tile rows of one round
+    if (round_rows && (256 % nN) * 16 <= 256 && nM > round_rows) {
+        const int rows = nM / round_rows * round_rows * 256;
+        if (rows < a.M) {
+            const Part main{rows, 2, 1, nk > 0 ? nk : 1, cost_us(2, tiles(rows, a.N, 256), 1, nk, 0)};
+            const Part rest = best_part(a.M - rows, a.N, nk, p.N4);
+            if (main.us + rest.us + 3.0 < p.part[0].us) {
+                p.parts = 2;
+                p.part[0] = main;
+                p.part[1] = rest;
             }
         }
     }
-    if (p.S > 1) p.part_bytes = (size_t)p.S * a.M * p.N4 * 4;
+    for (int i = 0; i < p.parts; ++i) {
+        const Part& q = p.part[i];
+        const size_t bytes = q.S > 1 ? (size_t)q.S * q.rows * p.N4 * 4 : 0;
+        if (bytes > p.part_bytes) p.part_bytes = bytes;
+    }
     return p;
 }
 
 template <typename T, bool AK, bool BK>
-void launch_tile(hipStream_t s, const Matmul& a, const Plan& p, float* part) {
-    const int bm = p.tile == 2 ? 256 : p.tile == 1 ? 128 : 64;
-    const dim3 grid(tiles(a.M, a.N, bm), p.S);
-    if (p.tile == 2) matmul256_kernel<T, AK, BK><<<grid, 512, 0, s>>>(a, part, p.N4, p.ksteps);
-    else if (p.tile == 1) matmul_kernel<T, AK, BK, 2, 2, 4, 2><<<grid, 256, 0, s>>>(a, part, p.N4, p.ksteps);
-    else matmul_kernel<T, AK, BK, 4, 1, 1, 3><<<grid, 256, 0, s>>>(a, part, p.N4, p.ksteps);
+void launch_tile(hipStream_t s, const Matmul& a, const Part& p, int N4, float* part) {
+    const dim3 grid(tiles(a.M, a.N, 64 << p.tile), p.S);
+    if (p.tile == 2) matmul256_kernel<T, AK, BK><<<grid, 512, 0, s>>>(a, part, N4, p.kslice);
+    else if (p.tile == 1) matmul_kernel<T, AK, BK, 2, 2, 4, 2><<<grid, 256, 0, s>>>(a, part, N4, p.kslice);
+    else matmul_kernel<T, AK, BK, 4, 1, 1, 3><<<grid, 256, 0, s>>>(a, part, N4, p.kslice);
 }
 
 template <typename T>
-void launch_typed(hipStream_t s, const Matmul& a, const Plan& p, float* part) {
-    if (a.a_k && a.b_k) launch_tile<T, true, true>(s, a, p, part);
-    else if (a.a_k) launch_tile<T, true, false>(s, a, p, part);
-    else if (a.b_k) launch_tile<T, false, true>(s, a, p, part);
-    else launch_tile<T, false, false>(s, a, p, part);
+void launch_part(hipStream_t s, const Matmul& a, const Part& p, int N4, float* part) {
+    if (a.a_k && a.b_k) launch_tile<T, true, true>(s, a, p, N4, part);
+    else if (a.a_k) launch_tile<T, true, false>(s, a, p, N4, part);
+    else if (a.b_k) launch_tile<T, false, true>(s, a, p, N4, part);
+    else launch_tile<T, false, false>(s, a, p, N4, part);
     if (p.S > 1) {
-        const int64_t n = (int64_t)a.M * (p.N4 >> 2);
-        matmul_join_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a.e, part, p.N4, p.S);
+        const int64_t n = (int64_t)a.M * (N4 >> 2);
+        matmul_join_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a.e, part, N4, p.S);
     }
 }
 
-void repack(hipStream_t s, const u16*& p, int64_t& ld, int rows, int len, void* dst) {
+// rows [m0, m0 + rows) of the product
+Matmul rows_of(const Matmul& a, int m0, int rows) {
+    Matmul r = a;
+    r.M = rows;
+    r.A = a.A + (int64_t)m0 * (a.a_k ? a.lda : 1);
+    Epilogue& e = r.e;
+    e.M = rows;
+    e.m_base = a.e.m_base + m0;
+    e.y = (u16*)a.e.y + (int64_t)m0 * a.e.ldy;
+    if (e.res) e.res = (const u16*)a.e.res + (int64_t)m0 * a.e.ldr;
+    if (e.slope) e.slope = a.e.slope + (int64_t)m0 * a.e.N;
+    if (e.lu) e.lu = a.e.lu + (int64_t)m0 * a.e.R;
+    return r;
+}
+
+// rows whose length or stride or base the 16-byte loads cannot take, as rows of the length rounded up to 8
+RepackArgs repack_of(const u16*& p, int64_t& ld, int rows, int len, void* dst) {
     const int cp = (len + 7) / 8 * 8;
-    const int64_t n = (int64_t)rows * (cp / 8);
-    repack_kernel<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(p, ld, rows, len, (u16*)dst, cp);
+    const RepackArgs r{p, ld, rows, len, (u16*)dst, cp};
     p = (const u16*)dst;
     ld = cp;
+    return r;
 }
 
 }  // namespace
@@ -743,21 +789,28 @@ int launch_matmul(hipStream_t s, int dtype, const Matmul& a0, void* ws, size_t w
     const Plan p = plan_of(a);
     if (p.a_bytes + p.b_bytes + p.part_bytes > ws_bytes) return -1;
     unsigned char* w = (unsigned char*)ws;
-    if (p.a_bytes) {
-        repack(s, a.A, a.lda, a.a_k ? a.M : a.K, a.a_k ? a.K : a.M, w);
-        w += p.a_bytes;
+    if (p.a_bytes || p.b_bytes) {
+        RepackArgs r[2]{};
+        if (p.a_bytes) r[0] = repack_of(a.A, a.lda, a.a_k ? a.M : a.K, a.a_k ? a.K : a.M, w);
+        if (p.b_bytes) r[1] = repack_of(a.B, a.ldb, a.b_k ? a.N : a.K, a.b_k ? a.K : a.N, w + p.a_bytes);
+        const int64_t na = ((int64_t)r[0].rows * (r[0].cp / 8) + 255) / 256, nb = ((int64_t)r[1].rows * (r[1].cp / 8) + 255) / 256;
+        repack_kernel<<<(unsigned)(na + nb), 256, 0, s>>>(r[0], r[1], (int)na);
     }
-    if (p.b_bytes) {
-        repack(s, a.B, a.ldb, a.b_k ? a.N : a.K, a.b_k ? a.K : a.N, w);
-        w += p.b_bytes;
-    }
-    float* part = p.S > 1 ? (float*)w : nullptr;
+    float* part = (float*)(w + p.a_bytes + p.b_bytes);
     a.e.vec = ((size_t)a.e.y & 15) == 0 && a.e.ldy % 8 == 0 &&
               (!a.e.res || (((size_t)a.e.res & 15) == 0 && a.e.ldr % 8 == 0)) &&
               (!a.e.slope || (((size_t)a.e.slope & 15) == 0 && a.N % 8 == 0));
+    // y past the L2s' and most of the Infinity Cache's size is not kept there for a later reader anyway: stored past
+    // them it leaves the operand panels (36928 x 1024 x 4096 forward 301 -> 293 us)
     a.e.nt = (int64_t)a.M * a.N * 2 >= (int64_t)64 << 20;
-    if (dtype == 1) launch_typed<BF16>(s, a, p, part);
-    else launch_typed<F16>(s, a, p, part);
+    int m0 = 0;
+    for (int i = 0; i < p.parts; ++i) {
+        const Part& q = p.part[i];
+        const Matmul r = rows_of(a, m0, q.rows);
+        if (dtype == 1) launch_part<BF16>(s, r, q, p.N4, q.S > 1 ? part : nullptr);
+        else launch_part<F16>(s, r, q, p.N4, q.S > 1 ? part : nullptr);
+        m0 += q.rows;
+    }
     return 0;
 }
 

@@ -368,6 +368,27 @@ def test_captured_step_replays(gpu):
     assert torch.equal(seen[1], seen[3]) and not torch.equal(seen[0], seen[1])
 
 
+@pytest.mark.parametrize("p", [0.0, 0.25])
+def test_rounds_and_remaining_rows(gpu, p):
+    """7300 x 2304 is one round of 256-wide tiles (28 rows of 9) and 132 rows more, a launch of their own: masks, residual,
+    slope and the low-rank term go by the whole operand's rows. Row- and column-contiguous x (the wide direction is dx's too)."""
+    m, k, n = 7300, 64, 2304
+    x, w, b, r, dy = rand(m, k), rand(n, k, scale=k ** -0.5, seed=1), rand(n, seed=2), rand(m, n, seed=4), rand(m, n, seed=3)
+    want = R.linear(x, w, b, r, "gelu", mask_of(m, n, p), dy)
+    for name, g in grads(gpu, x, w, b, r, dy, activation="gelu", dropout_p=p, seed=SEED, offset=OFFSET).items():
+        R.check(g, want[name], name)
+    xt = x.to(gpu).t().contiguous().t()
+    R.check(ops.linear(xt, w.to(gpu), b.to(gpu)), R.linear(x, w, b)["y"])
+    # dx of this one is [7300, 2304], with the masked low-rank term
+    x, w, A, B, dy = rand(m, n, seed=5), rand(k, n, scale=n ** -0.5, seed=6), rand(n, 4, scale=n ** -0.5, seed=7), rand(4, k, scale=0.3, seed=8), rand(m, k, seed=9)
+    leaves = [t.to(gpu).requires_grad_() for t in (x, A, B)]
+    y = ops.lora_linear(leaves[0], w.to(gpu), *leaves[1:], scaling=2.0, dropout_p=p, seed=SEED, offset=OFFSET)
+    want = R.lora(x, w, A, B, None, 2.0, mask_of(m, n, p), dy)
+    for name, g in zip(("dx", "dA", "dB"), torch.autograd.grad(y, leaves, dy.to(gpu))):
+        R.check(g, want[name], name)
+    R.check(y, want["y"])
+
+
 def test_long_rows_offsets_past_32_bits(gpu):
     """A [rows, 4096] output of more than 2^32 bytes: the last rows are addressed in 64 bits (checked on slices against
     the same rows computed alone)."""
