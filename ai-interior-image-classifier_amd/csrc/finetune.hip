@@ -103,6 +103,50 @@ __global__ __launch_bounds__(256) void dropout_kernel(DropArgs a) {
     }
 }
 
+// The same for rows that 16-byte accesses cannot address (an odd width, a slice): a wave takes 256 columns of a row, lane l
+// computes the mask of the four columns 4 l .. 4 l + 3, four ballots make it a 256-bit mask in scalar registers, and every
+// access is one element a lane, 64 consecutive ones an instruction (eight scattered elements a lane: 12611 x 2049 fp32 100 us,
+// 2.0 TB/s).
+template <class E>
+__global__ __launch_bounds__(256) void dropout_rows_kernel(DropArgs a) {
+    typedef typename E::store S;
+    const int lane = threadIdx.x & 63;
+    const int c0 = ((int)blockIdx.x * a.tx + (int)(threadIdx.x >> 6) % a.tx) * 256;
+    const int ty = (int)(threadIdx.x >> 6) / a.tx, ny = 4 / a.tx;
+    if (c0 >= a.cols) return;
+    const uint2 off = drop_offset(a.d);
+    for (int64_t m = (int64_t)blockIdx.y * ny + ty; m < a.rows; m += (int64_t)gridDim.y * ny) {
+        unsigned long long keep[4] = {~0ull, ~0ull, ~0ull, ~0ull};
+        if (a.d.on) {
+            const uint4 w = philox4(((unsigned)c0 >> 2) + lane, (unsigned)m, off.x, off.y, a.d.k0, a.d.k1);
+            keep[0] = __ballot(w.x > a.d.drop_max);
+            keep[1] = __ballot(w.y > a.d.drop_max);
+            keep[2] = __ballot(w.z > a.d.drop_max);
+            keep[3] = __ballot(w.w > a.d.drop_max);
+        }
+        const int q = lane & 3;
+        const unsigned long long mine = q & 2 ? (q & 1 ? keep[3] : keep[2]) : (q & 1 ? keep[1] : keep[0]);
+        const S* x = (const S*)a.x + m * a.ldx;
+        const S* r = (const S*)a.res + m * a.ldr;
+        S* y = (S*)a.y + m * a.ldy;
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int c = c0 + 64 * j + lane;
+            v[j] = c < a.cols ? E::to_f32(x[c]) : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int c = c0 + 64 * j + lane;
+            if (c >= a.cols) continue;
+            // column 64 j + lane is word lane & 3 of quad 16 j + lane / 4
+            float o = a.d.on ? ((mine >> (16 * j + (lane >> 2))) & 1 ? v[j] * a.d.scale : 0.f) : v[j];
+            if (a.res) o += E::to_f32(r[c]);
+            y[c] = E::from_f32(o);
+        }
+    }
+}
+
 // ---- dz = dropout(dy) * act'(z), and the column sums of the unrounded dz for the bias gradient ----
 struct DzArgs {
     const void* dy;
@@ -204,89 +248,117 @@ __global__ __launch_bounds__(256) void pad_kernel(PadArgs a, PadArgs b, int bloc
 }
 
 // ---- thin product u[m, r] = alpha sum_k mask(x)[m, k] f[r, k], 32 ranks a launch row ----
-// One workgroup: 16 rows of x, its four waves a quarter of k each, so x is read once, by 16-byte loads straight into the
-// MFMA fragment (lane: row lane & 15). Steps are 64 deep: lane group g takes k 16 g .. 16 g + 15 of it as two fragments
-// (the order of k inside a step is free, f is read in the same one), so the first load touches every whole 128-byte
-// line of the 16 rows (against 64 bytes a row and step: 18464 x 4096 73 -> 42 us). The quarters meet in LDS.
+// One workgroup: RG groups of 16 rows of x, its four waves a quarter of k each, so x is read once, by 16-byte loads straight
+// into the MFMA fragment (lane: row lane & 15). Steps are 64 deep: lane group g takes k 16 g .. 16 g + 15 of it as two
+// fragments (the order of k inside a step is free, f is read in the same one), so a step touches whole 128-byte lines.
+// f's fragments, read from the caches, serve all RG row groups: with one group they were twice x's bytes (18464 x 4096,
+// rank 16: 73 us, 2 TB/s). The quarters meet in LDS.
 struct DownArgs {
     const u16 *x, *f;  // x [M, K] row stride ldx; f [R, K] row stride ldf, rows past r and columns past K (to 64) zero
     u16* u;            // [M, R]
     int64_t ldx, ldf;
-    int M, K, R, vec;
+    int M, K, R, rank, vec;
     float alpha;
     Dropout d;
 };
-template <typename T>
+template <typename T, int RG>
 __global__ __launch_bounds__(256) void lora_down_kernel(DownArgs a) {
     typedef typename T::vec8 vec8;
-    __shared__ float red[3][64][9];
+    __shared__ float red[3][RG][64][9];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int li = lane & 15, g = lane >> 4;
-    const int m = blockIdx.x * 16 + li, r0 = blockIdx.y * 32;
+    const int m0 = blockIdx.x * (16 * RG) + li, r0 = blockIdx.y * 32;
+    const bool two = a.rank > r0 + 16;  // (the second 16 ranks are all padding otherwise)
     const int nk = (a.K + 63) >> 6, k0 = nk * wave / 4, k1 = nk * (wave + 1) / 4;
-    const u16* xr = a.x + (int64_t)min(m, a.M - 1) * a.ldx;
+    const u16* xr[RG];
+#pragma unroll
+    for (int i = 0; i < RG; ++i) xr[i] = a.x + (int64_t)min(m0 + 16 * i, a.M - 1) * a.ldx;  // (rows past M are not stored)
     const u16* f0 = a.f + (int64_t)(r0 + li) * a.ldf;
     const u16* f1 = f0 + 16 * a.ldf;
     const uint2 off = drop_offset(a.d);
-    f32x4 c0 = {0.f, 0.f, 0.f, 0.f}, c1 = c0;
-    auto mask = [&](u16 (&v)[8], int k) {
-        const uint4 p = philox4((unsigned)k >> 2, (unsigned)m, off.x, off.y, a.d.k0, a.d.k1);
-        const uint4 q = philox4(((unsigned)k >> 2) + 1, (unsigned)m, off.x, off.y, a.d.k0, a.d.k1);
-        const unsigned w[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+    f32x4 c0[RG], c1[RG];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = w[j] > a.d.drop_max ? v[j] : (u16)0;
-    };
-    auto step = [&](const uint4& x, int k) {
+    for (int i = 0; i < RG; ++i) c0[i] = c1[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto masked = [&](uint4 x, int m, int k) -> vec8 {
         u16 v[8];
         __builtin_memcpy(v, &x, 16);
-        if (a.d.on) mask(v, k);
-        vec8 xf;
-        __builtin_memcpy(&xf, v, 16);
-        c0 = T::mfma16(*(const vec8*)(f0 + k), xf, c0);  // lane: row m, ranks 4 g .. 4 g + 3
-        c1 = T::mfma16(*(const vec8*)(f1 + k), xf, c1);
+        if (a.d.on) {
+            const uint4 p = philox4((unsigned)k >> 2, (unsigned)m, off.x, off.y, a.d.k0, a.d.k1);
+            const uint4 q = philox4(((unsigned)k >> 2) + 1, (unsigned)m, off.x, off.y, a.d.k0, a.d.k1);
+            const unsigned w[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = w[j] > a.d.drop_max ? v[j] : (u16)0;
+        }
+        vec8 r;
+        __builtin_memcpy(&r, v, 16);
+        return r;
     };
-    // (rows past M repeat the last one and are not stored)
     const int whole = a.vec ? a.K >> 6 : 0;  // steps of 64 whole columns
     int kt = k0;
-#pragma unroll 4
+#pragma unroll 2
     for (; kt < min(k1, whole); ++kt) {
         const int k = kt * 64 + 16 * g;
-        const uint4 x0 = *(const uint4*)(xr + k), x1 = *(const uint4*)(xr + k + 8);
-        step(x0, k);
-        step(x1, k + 8);
+        uint4 x[RG][2];
+#pragma unroll
+        for (int i = 0; i < RG; ++i) {
+            x[i][0] = *(const uint4*)(xr[i] + k);
+            x[i][1] = *(const uint4*)(xr[i] + k + 8);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const vec8 fa = *(const vec8*)(f0 + k + 8 * h);
+            const vec8 fb = two ? *(const vec8*)(f1 + k + 8 * h) : fa;
+#pragma unroll
+            for (int i = 0; i < RG; ++i) {
+                const vec8 xf = masked(x[i][h], m0 + 16 * i, k + 8 * h);
+                c0[i] = T::mfma16(fa, xf, c0[i]);  // lane: row m, ranks 4 g .. 4 g + 3
+                if (two) c1[i] = T::mfma16(fb, xf, c1[i]);
+            }
+        }
     }
     for (; kt < k1; ++kt) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int k = kt * 64 + 16 * g + 8 * h;
-            u16 v[8];
+            const vec8 fa = *(const vec8*)(f0 + k), fb = *(const vec8*)(f1 + k);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = k + j < a.K ? xr[k + j] : (u16)0;
-            uint4 x;
-            __builtin_memcpy(&x, v, 16);
-            step(x, k);
+            for (int i = 0; i < RG; ++i) {
+                u16 v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = k + j < a.K ? xr[i][k + j] : (u16)0;
+                uint4 x;
+                __builtin_memcpy(&x, v, 16);
+                const vec8 xf = masked(x, m0 + 16 * i, k);
+                c0[i] = T::mfma16(fa, xf, c0[i]);
+                c1[i] = T::mfma16(fb, xf, c1[i]);
+            }
         }
     }
     if (wave) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            red[wave - 1][lane][j] = c0[j];
-            red[wave - 1][lane][4 + j] = c1[j];
-        }
+        for (int i = 0; i < RG; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                red[wave - 1][i][lane][j] = c0[i][j];
+                red[wave - 1][i][lane][4 + j] = c1[i][j];
+            }
     }
     __syncthreads();
-    if (wave || m >= a.M) return;
-    for (int w = 0; w < 3; ++w)
+    if (wave) return;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            c0[j] += red[w][lane][j];
-            c1[j] += red[w][lane][4 + j];
-        }
-    u16* u = a.u + (int64_t)m * a.R + r0 + 4 * g;
-    c0 *= a.alpha;
-    c1 *= a.alpha;
-    *(uint2*)u = make_uint2(pack2<T>(c0[0], c0[1]), pack2<T>(c0[2], c0[3]));
-    *(uint2*)(u + 16) = make_uint2(pack2<T>(c1[0], c1[1]), pack2<T>(c1[2], c1[3]));
+    for (int i = 0; i < RG; ++i) {
+        const int m = m0 + 16 * i;
+        if (m >= a.M) continue;
+        for (int w = 0; w < 3; ++w)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                c0[i][j] += red[w][i][lane][j];
+                c1[i][j] += red[w][i][lane][4 + j];
+            }
+        u16* u = a.u + (int64_t)m * a.R + r0 + 4 * g;
+        *(uint2*)u = make_uint2(pack2<T>(c0[i][0] * a.alpha, c0[i][1] * a.alpha), pack2<T>(c0[i][2] * a.alpha, c0[i][3] * a.alpha));
+        *(uint2*)(u + 16) = make_uint2(pack2<T>(c1[i][0] * a.alpha, c1[i][1] * a.alpha), pack2<T>(c1[i][2] * a.alpha, c1[i][3] * a.alpha));
+    }
 }
 
 // ---- thin gradient g[c, r] = sum_m mask(x)[m, c] u[m, r]: 128 columns x 32 ranks a workgroup, slices of rows ----
@@ -509,9 +581,9 @@ Db make_dz(const void* dy, int64_t dy_stride, const int16_t* slope, void* dz, in
     DzArgs& d = b.d;
     b.db = db;
     b.db_f32 = db_f32;
-    // about 2048 workgroups of 256 columns and at least 8 rows (fewer rows a block fill the chip on small products:
+    // about 4096 workgroups of 256 columns and at least 8 rows (fewer rows a block fill the chip on small products:
     // 1237 x 437 21 -> 8 us; fewer blocks shorten the join: 36928 x 4096 23 -> 6 us)
-    const int64_t most = 2048 / ((N + 255) / 256 ? (N + 255) / 256 : 1), need = (M + 7) / 8;
+    const int64_t most = 4096 / ((N + 255) / 256 ? (N + 255) / 256 : 1), need = (M + 7) / 8;
     b.blocks = (int)(need < most ? need : most > 1 ? most : (M ? 1 : 0));
     d.rows = b.blocks ? (int)up((M + b.blocks - 1) / b.blocks, 8) : 8;
     d.dy = dy;
@@ -625,7 +697,7 @@ void launch_pad(hipStream_t s, const PadArgs& a, const PadArgs& b) {
     if (na + nb) pad_kernel<<<(unsigned)(na + nb), 256, 0, s>>>(a, b, (int)na);
 }
 void launch_down(hipStream_t s, bool bf, const void* x, int64_t ldx, const void* f, int64_t ldf, void* u, int64_t M, int64_t K, int64_t R,
-                 float alpha, const Dropout& drop) {
+                 int64_t rank, float alpha, const Dropout& drop) {
     if (!M) return;
     DownArgs d{};
     d.x = (const u16*)x;
@@ -636,12 +708,17 @@ void launch_down(hipStream_t s, bool bf, const void* x, int64_t ldx, const void*
     d.M = (int)M;
     d.K = (int)K;
     d.R = (int)R;
+    d.rank = (int)rank;
     d.vec = aligned16(x) && d.ldx % 8 == 0;
     d.alpha = alpha;
     d.d = drop;
-    const dim3 grid((unsigned)((M + 15) / 16), (unsigned)(R / 32));
-    if (bf) lora_down_kernel<BF16><<<grid, 256, 0, s>>>(d);
-    else lora_down_kernel<F16><<<grid, 256, 0, s>>>(d);
+    // two row groups a workgroup once that still gives every CU one; single groups spread few rows wider
+    const int rg = M >= 8192 ? 2 : 1;
+    const dim3 grid((unsigned)((M + 16 * rg - 1) / (16 * rg)), (unsigned)(R / 32));
+    if (bf && rg == 2) lora_down_kernel<BF16, 2><<<grid, 256, 0, s>>>(d);
+    else if (bf) lora_down_kernel<BF16, 1><<<grid, 256, 0, s>>>(d);
+    else if (rg == 2) lora_down_kernel<F16, 2><<<grid, 256, 0, s>>>(d);
+    else lora_down_kernel<F16, 1><<<grid, 256, 0, s>>>(d);
 }
 int grad_slices(int64_t M, int64_t C, int64_t R) {
     const int64_t wg = ((C + 127) / 128) * (R / 32);
@@ -865,20 +942,27 @@ int clipvit_dropout(void* stream, int dtype, const void* x, int64_t x_stride, co
         d.d = make_dropout(*dropout);
         const int per = dtype == CLIPVIT_F32 ? 4 : 8;
         d.vec = aligned16(x) && aligned16(y) && aligned16(residual) && d.ldx % per == 0 && d.ldy % per == 0 && (!residual || d.ldr % per == 0);
-        // thread groups of 8 columns: the widest row of threads that leaves at most an eighth of them idle
-        const int groups = (int)((cols + 7) / 8);
-        d.tx = 64;
+        // tx threads (waves) cover a row's groups of 8 (256) columns: the widest that leaves at most an eighth of them idle
+        const int per_group = d.vec ? 8 : 256, most = d.vec ? 64 : 4, all = d.vec ? 256 : 4;
+        const int groups = (int)((cols + per_group - 1) / per_group);
+        d.tx = most;
         while (d.tx > 1 && ((groups + d.tx - 1) / d.tx) * (int64_t)d.tx * 8 > (int64_t)groups * 9) d.tx >>= 1;
-        const int ny = 256 / d.tx, gx = (groups + d.tx - 1) / d.tx;
+        const int ny = all / d.tx, gx = (groups + d.tx - 1) / d.tx;
         int64_t gy = (rows + ny - 1) / ny;
         const int64_t cap = (16384 + gx - 1) / gx;
         if (gy > cap) gy = cap;
         if (gy > 65535) gy = 65535;
         const dim3 grid(gx, (unsigned)gy);
         hipStream_t s = (hipStream_t)stream;
-        if (dtype == CLIPVIT_F32) dropout_kernel<F32T><<<grid, 256, 0, s>>>(d);
-        else if (dtype == CLIPVIT_BF16) dropout_kernel<BF16T><<<grid, 256, 0, s>>>(d);
-        else dropout_kernel<F16T><<<grid, 256, 0, s>>>(d);
+        if (d.vec) {
+            if (dtype == CLIPVIT_F32) dropout_kernel<F32T><<<grid, 256, 0, s>>>(d);
+            else if (dtype == CLIPVIT_BF16) dropout_kernel<BF16T><<<grid, 256, 0, s>>>(d);
+            else dropout_kernel<F16T><<<grid, 256, 0, s>>>(d);
+        } else {
+            if (dtype == CLIPVIT_F32) dropout_rows_kernel<F32T><<<grid, 256, 0, s>>>(d);
+            else if (dtype == CLIPVIT_BF16) dropout_rows_kernel<BF16T><<<grid, 256, 0, s>>>(d);
+            else dropout_rows_kernel<F16T><<<grid, 256, 0, s>>>(d);
+        }
         FT_LAUNCHED();
         return CLIPVIT_OK;
     });
@@ -907,7 +991,7 @@ int clipvit_lora_linear(void* stream, const clipvit_lora_args* a, void* workspac
         const Dropout drop = make_dropout(a->dropout);
         launch_pad(s, pad_of(a->a, a->a_stride[1], a->a_stride[0], a->rank, a->K, R, Kp, l.f),
                    pad_of(a->b, a->b_stride[1], a->b_stride[0], a->N, a->rank, a->N, R, l.v));
-        launch_down(s, a->dtype == CLIPVIT_BF16, a->x, a->x_stride, l.f, Kp, a->u, a->M, a->K, R, a->scaling * (drop.on ? drop.scale : 1.f), drop);
+        launch_down(s, a->dtype == CLIPVIT_BF16, a->x, a->x_stride, l.f, Kp, a->u, a->M, a->K, R, a->rank, a->scaling * (drop.on ? drop.scale : 1.f), drop);
         if (launch_matmul(s, a->dtype, l.y, l.mm, l.mm_bytes)) FT_FAIL(CLIPVIT_E_INVALID, std::string("lora_linear: ") + WORKSPACE);
         FT_LAUNCHED();
         return CLIPVIT_OK;
@@ -938,7 +1022,7 @@ int clipvit_lora_linear_grad(void* stream, const clipvit_lora_grad_args* a, void
         if (g.want_du) {
             launch_pad(s, pad_of(a->b, a->b_stride[0], a->b_stride[1], a->rank, a->N, R, Np, g.f),
                        pad_of(a->a, a->a_stride[0], a->a_stride[1], a->K, a->rank, g.want_dx ? a->K : 0, R, g.v));
-            launch_down(s, bf, a->dy, a->dy_stride, g.f, Np, g.du, a->M, a->N, R, a->scaling * (drop.on ? drop.scale : 1.f), none);
+            launch_down(s, bf, a->dy, a->dy_stride, g.f, Np, g.du, a->M, a->N, R, a->rank, a->scaling * (drop.on ? drop.scale : 1.f), none);
             if (g.want_dx && launch_matmul(s, a->dtype, g.dx, g.mm, g.mm_bytes)) FT_FAIL(CLIPVIT_E_INVALID, std::string("lora_linear_grad: ") + WORKSPACE);
             if (a->da) launch_grad(s, bf, a->x, a->x_stride, g.du, a->da, a->rank, 1, a->M, a->K, R, a->rank, drop, g.grad);
         }

@@ -105,6 +105,19 @@ struct Panel {
     }
 };
 
+// k-tile j of a low-rank factor [count, rank] (contiguous rows, rank % 32 == 0), as a row panel from row i0
+template <int R, int NW, class Map>
+__device__ __forceinline__ void stage_low(const u16* low, int rank, int i0, int count, int j, int w, int lane, unsigned char* dst) {
+    const int valid = min(count - i0, 256), r = lane >> 3, chunk = (lane & 7) ^ r;
+    const i32x4_t rs = buf_rsrc(low + (int64_t)i0 * rank, (unsigned)valid * (unsigned)rank * 2);
+#pragma unroll
+    for (int i = 0; i < R / 8 / NW; ++i) {
+        const int piece = w * (R / 8 / NW) + i, row = Map::at(piece * 8 + r);
+        const bool in = row < valid && j * 64 + chunk * 8 < rank;
+        blds16(rs, in ? (unsigned)(row * rank + j * 64 + chunk * 8) * 2 : OOB, 0, dst + piece * 1024);
+    }
+}
+
 // Fragment reads of FR (1, 2 or 4) 16-row fragments x 64 k from position i0 of a panel. Each asm block ends with its own
 // wait (hipcc does not see these reads, and a plain LDS read would make it drain the LDS-DMA loads in flight).
 template <typename T, bool KC, int R, int FR>
@@ -210,44 +223,44 @@ __device__ __forceinline__ void bar() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
+// one 64-deep k-tile of the low-rank term from its fragments; masked, in the accumulators' layout, where a lane's four
+// columns are one counter of the generator (a fragment at a time: the scheduler would otherwise spill)
+template <typename T, int FR, int FB, int J0, int FM>
+__device__ __forceinline__ void low_acc(const Epilogue& e, const uint2& off, const typename T::vec8 (&a)[2][FR], const typename T::vec8 (&b)[2][FB],
+                                        f32x4 (&acc)[FM][4], int i0, int m, int n) {
+    if (!e.low_mask) {
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int i = 0; i < FR; ++i)
+#pragma unroll
+                for (int j = 0; j < FB; ++j) acc[i0 + i][J0 + j] = T::mfma16(b[ks][j], a[ks][i], acc[i0 + i][J0 + j]);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < FR; ++i)
+#pragma unroll
+        for (int j = 0; j < FB; ++j) {
+            f32x4 t = T::mfma16(b[0][j], a[0][i], f32x4{0.f, 0.f, 0.f, 0.f});
+            t = T::mfma16(b[1][j], a[1][i], t);
+            float t0 = t[0], t1 = t[1], t2 = t[2], t3 = t[3];
+            drop4(e.drop, off, e.m_base + m + 16 * i, n + 16 * (J0 + j), 1.0f, t0, t1, t2, t3);
+            acc[i0 + i][J0 + j] += f32x4{t0, t1, t2, t3};
+            __builtin_amdgcn_sched_barrier(0);
+        }
+}
+
 // acc[i][j]: rows mw + 16 i .., columns nw + 16 j .. of C, in the MFMA's layout (lane: row lane & 15, columns
 // 4 (lane >> 4) .. + 3). eb: LDS of this wave's own, 4 KB for each of up to four fragment rows. part != null: the
 // slice's fp32 sums, row stride N4.
 template <typename T, int FM>
 __device__ __forceinline__ void store_tile(const Matmul& a, f32x4 (&acc)[FM][4], int mw, int nw, float* eb, float* part, int N4, int lane) {
-    typedef typename T::vec8 vec8;
     const Epilogue& e = a.e;
     constexpr int H = FM < 4 ? FM : 4;
     const int li = lane & 15, g = lane >> 4, er = lane >> 3, ec = lane & 7;
     const int n = nw + 8 * ec;
     if (mw >= a.M || nw >= (part ? N4 : a.N)) return;
     const uint2 off = e.drop.on ? drop_offset(e.drop) : make_uint2(0, 0);
-    if (!part && e.R > 0) {
-        // rank-R term, in the accumulators' layout: fragments straight from global memory (u and v rows are padded to
-        // 32 columns); its mask is one counter a lane and fragment
-        const u32x4 z = {0u, 0u, 0u, 0u};
-#pragma unroll 1
-        for (int r = 0; r < e.R; r += 32) {
-            vec8 vf[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int c = nw + 16 * j + li;
-                vf[j] = __builtin_bit_cast(vec8, c < a.N ? *(const u32x4*)(e.lv + (int64_t)c * e.R + r + 8 * g) : z);
-            }
-#pragma unroll
-            for (int i = 0; i < FM; ++i) {
-                const int m = mw + 16 * i + li;
-                const vec8 uf = __builtin_bit_cast(vec8, m < a.M ? *(const u32x4*)(e.lu + (int64_t)m * e.R + r + 8 * g) : z);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const f32x4 t = T::mfma16(vf[j], uf, f32x4{0.f, 0.f, 0.f, 0.f});
-                    float t0 = t[0], t1 = t[1], t2 = t[2], t3 = t[3];
-                    if (e.low_mask) drop4(e.drop, off, e.m_base + m, nw + 16 * j + 4 * g, 1.0f, t0, t1, t2, t3);
-                    acc[i][j] += f32x4{t0, t1, t2, t3};
-                }
-            }
-        }
-    }
     auto get = [&](int row, float (&v)[8]) {
         const f32x4 x = *(const f32x4*)(eb + row * 64 + (((2 * ec) ^ (row & 15)) << 2));
         const f32x4 y = *(const f32x4*)(eb + row * 64 + (((2 * ec + 1) ^ (row & 15)) << 2));
@@ -527,6 +540,38 @@ __global__ __launch_bounds__(512, 1) void matmul256_kernel(Matmul a, float* part
         vm_wait<0>();  // no load into LDS outlives the k loop: the epilogue takes the stages over
         bar();
     }
+    if (a.e.R > 0 && blockIdx.y == 0) {
+        // rank-R term, 64 ranks at a time: the factors' rows staged like row panels, whatever the operands are. (Its
+        // fragments straight from global memory cost 14 us a round of tiles; as further k-tiles of the loop above, their
+        // branch slowed the loop by a quarter.)
+        const uint2 off = a.e.drop.on ? drop_offset(a.e.drop) : make_uint2(0, 0);
+        Frags<T, true, 128, 4> la;
+        Frags<T, true, 128, 2> lb;
+        la.init(lds, wm * 64, lane);
+        lb.init(lds + B_OFF, wn * 32, lane);
+        const int m = m0 + wm * 128 + (lane & 15), n = n0 + wn * 64 + 4 * (lane >> 4);
+#pragma unroll 1
+        for (int j = 0; j * 64 < a.e.R; ++j) {
+            if (wm == 0) {
+                stage_low<128, 4, Half<0, 64>>(a.e.lu, a.e.R, m0, a.M, j, wn, lane, smem);
+                stage_low<128, 4, Half<1, 64>>(a.e.lu, a.e.R, m0, a.M, j, wn, lane, smem + HALF);
+            } else {
+                stage_low<128, 4, Half<0, 32>>(a.e.lv, a.e.R, n0, a.N, j, wn, lane, smem + B_OFF);
+                stage_low<128, 4, Half<1, 32>>(a.e.lv, a.e.R, n0, a.N, j, wn, lane, smem + B_OFF + HALF);
+            }
+            vm_wait<0>();
+            bar();
+            lb.read(b0, 0);
+            lb.read(b1, HALF);
+            la.read(af, 0);
+            low_acc<T, 4, 2, 0>(a.e, off, af, b0, acc, 0, m, n);
+            low_acc<T, 4, 2, 2>(a.e, off, af, b1, acc, 0, m, n);
+            la.read(af, HALF);
+            low_acc<T, 4, 2, 0>(a.e, off, af, b0, acc, 4, m + 64, n);
+            low_acc<T, 4, 2, 2>(a.e, off, af, b1, acc, 4, m + 64, n);
+            bar();
+        }
+    }
     store_tile<T, 8>(a, acc, m0 + wm * 128, n0 + wn * 64, (float*)smem + wave * 4096,
                      part ? part + (int64_t)blockIdx.y * a.M * N4 : nullptr, N4, lane);
 }
@@ -595,6 +640,24 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_kernel(Matmul a, float
         vm_wait<0>();  // no load into LDS outlives the k loop: the epilogue takes the stages over
         bar();
     }
+    if (a.e.R > 0 && blockIdx.y == 0) {  // as above
+        const uint2 off = a.e.drop.on ? drop_offset(a.e.drop) : make_uint2(0, 0);
+        Frags<T, true, BM, FM> la;
+        Frags<T, true, BN, 4> lb;
+        la.init(lds, wm * FM * 16, lane);
+        lb.init(lds + A_ST, wn * 64, lane);
+#pragma unroll 1
+        for (int j = 0; j * 64 < a.e.R; ++j) {
+            stage_low<BM, W, Whole>(a.e.lu, a.e.R, m0, a.M, j, wave, lane, smem);
+            stage_low<BN, W, Whole>(a.e.lv, a.e.R, n0, a.N, j, wave, lane, smem + A_ST);
+            vm_wait<0>();
+            bar();
+            lb.read(bf, 0);
+            la.read(af, 0);
+            low_acc<T, FM, 4, 0>(a.e, off, af, bf, acc, 0, m0 + wm * FM * 16 + (lane & 15), n0 + wn * 64 + 4 * (lane >> 4));
+            bar();
+        }
+    }
     store_tile<T, FM>(a, acc, m0 + wm * FM * 16, n0 + wn * 64, (float*)smem + wave * FM * 1024,
                       part ? part + (int64_t)blockIdx.y * a.M * N4 : nullptr, N4, lane);
 }
@@ -612,18 +675,6 @@ __global__ __launch_bounds__(256) void matmul_join_kernel(Epilogue e, const floa
     for (int z = 0; z < S; ++z) s += *(const f32x4*)(p + z * sl);
     float v[4] = {s[0], s[1], s[2], s[3]};
     const uint2 off = e.drop.on ? drop_offset(e.drop) : make_uint2(0, 0);
-    if (e.R > 0) {
-        float t[4] = {0.f, 0.f, 0.f, 0.f};
-        const u16* u = e.lu + (int64_t)m * e.R;
-        for (int j = 0; j < 4; ++j) {
-            if (n + j >= e.N) break;
-            const u16* w = e.lv + (int64_t)(n + j) * e.R;
-            for (int r = 0; r < e.R; ++r) t[j] += T::to_f32(u[r]) * T::to_f32(w[r]);
-        }
-        if (e.low_mask) drop4(e.drop, off, e.m_base + m, n, 1.0f, t[0], t[1], t[2], t[3]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] += t[j];
-    }
     float b[4];
     bias_cols<T, 4>(e, n, b);
     epilogue_cols<T, 4>(e, off, m, n, v, b);
