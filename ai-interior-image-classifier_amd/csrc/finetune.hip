@@ -153,8 +153,9 @@ struct DzArgs {
     const short* slope;  // [M, N] or null
     void* dz;            // [M, lddz] or null
     float* part;         // [gridDim.y][N] column sums of a block's rows, or null
+    void* db;            // the bias gradient itself where one block has all the rows (part null), or null
     int64_t lddy, lddz;
-    int M, N, rows, vec;  // rows of a block
+    int M, N, rows, vec, db_f32;  // rows of a block
     Dropout d;
 };
 template <class E>
@@ -195,7 +196,7 @@ __global__ __launch_bounds__(256) void dz_kernel(DzArgs a) {
             for (int j = 0; j < 8; ++j) s[j] += v[j];
         }
     }
-    if (!a.part) return;
+    if (!a.part && !a.db) return;
 #pragma unroll
     for (int j = 0; j < 8; ++j) sums[ty][tx][j] = s[j];
     __syncthreads();
@@ -205,7 +206,10 @@ __global__ __launch_bounds__(256) void dz_kernel(DzArgs a) {
             float t = 0.f;
 #pragma unroll
             for (int y = 0; y < 8; ++y) t += sums[y][tx][j];
-            if (j < nc) a.part[(int64_t)blockIdx.y * a.N + c + j] = t;
+            if (j >= nc) continue;
+            if (a.part) a.part[(int64_t)blockIdx.y * a.N + c + j] = t;
+            else if (a.db_f32) ((float*)a.db)[c + j] = t;
+            else ((S*)a.db)[c + j] = E::from_f32(t);
         }
     }
 }
@@ -585,6 +589,7 @@ Db make_dz(const void* dy, int64_t dy_stride, const int16_t* slope, void* dz, in
     // 1237 x 437 21 -> 8 us; fewer blocks shorten the join: 36928 x 4096 23 -> 6 us)
     const int64_t most = 4096 / ((N + 255) / 256 ? (N + 255) / 256 : 1), need = (M + 7) / 8;
     b.blocks = (int)(need < most ? need : most > 1 ? most : (M ? 1 : 0));
+    if (db && M && M <= 128) b.blocks = 1;  // few rows: one block writes db, no join launch
     d.rows = b.blocks ? (int)up((M + b.blocks - 1) / b.blocks, 8) : 8;
     d.dy = dy;
     d.slope = slope;
@@ -597,15 +602,17 @@ Db make_dz(const void* dy, int64_t dy_stride, const int16_t* slope, void* dz, in
     d.vec = aligned16(dy) && d.lddy % 8 == 0 && (!dz || (aligned16(dz) && lddz % 8 == 0)) && (!slope || (aligned16(slope) && N % 8 == 0));
     return b;
 }
-size_t dz_part_bytes(const Db& b) { return b.db ? (size_t)b.blocks * b.d.N * 4 : 0; }
+size_t dz_part_bytes(const Db& b) { return b.db && b.blocks > 1 ? (size_t)b.blocks * b.d.N * 4 : 0; }
 void launch_dz(hipStream_t s, bool bf, Db& b, void* part) {
-    b.d.part = b.db ? (float*)part : nullptr;
+    b.d.part = b.db && b.blocks > 1 ? (float*)part : nullptr;
+    b.d.db = b.blocks == 1 ? b.db : nullptr;
+    b.d.db_f32 = b.db_f32;
     if (b.blocks) {
         const dim3 grid((b.d.N + 255) / 256, b.blocks);
         if (bf) dz_kernel<BF16T><<<grid, 256, 0, s>>>(b.d);
         else dz_kernel<F16T><<<grid, 256, 0, s>>>(b.d);
     }
-    if (b.db) {
+    if (b.db && b.blocks != 1) {
         const int g = (b.d.N + 31) / 32;
         if (bf) db_kernel<BF16T><<<g, 256, 0, s>>>(b.d.part, b.blocks, b.d.N, b.db, b.db_f32);
         else db_kernel<F16T><<<g, 256, 0, s>>>(b.d.part, b.blocks, b.d.N, b.db, b.db_f32);

@@ -134,7 +134,7 @@ def test_lora_grad_entry_refuses(kw):
 
 @pytest.mark.parametrize("name, args", [
     ("linear", linear_args(K=17, x_row=17, w_row=17)),  # odd rows: both operands are copied first
-    ("linear_grad", linear_grad_args()), ("lora_linear", lora_args()), ("lora_linear_grad", lora_grad_args())])
+    ("linear_grad", linear_grad_args(M=400)), ("lora_linear", lora_args()), ("lora_linear_grad", lora_grad_args())])
 def test_workspace_rules(name, args):
     L, need = _lib.lib(), ctypes.c_size_t()
     size, call = getattr(L, f"clipvit_{name}_workspace"), getattr(L, f"clipvit_{name}")
