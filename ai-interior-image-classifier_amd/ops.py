@@ -144,6 +144,7 @@ class _On:
 
 
 def _launch(name: str, index: int, args, ws, nbytes: int) -> None:
+    """One C call on the current stream of device `index`."""
     fn = getattr(_lib.lib(), name)
     ptr = ws.data_ptr() if nbytes else None
     if torch.cuda.current_device() == index:
@@ -199,19 +200,18 @@ def _wants_grad(*tensors) -> bool:
 
 
 # ---------------------------------------------------------------- linear
-def _linear_forward(x2, weight, bias, res2, act, drop, save):
-    """(y [M, N], act'(z) or None) of x2 [M, K]."""
-    x2, weight = _panel(x2), _panel(weight)
-    (m, k), n, dt = x2.shape, weight.shape[0], _DT[x2.dtype]
-    (x0, x1), (w0, w1), xp, wp = x2.stride(), weight.stride(), x2.data_ptr(), weight.data_ptr()
+def _linear_forward(x2, w, bias, res2, act, drop, save):
+    """(y [M, N], act'(z) or None, the operands' description) of x2 [M, K], w [N, K] as _panel gives them."""
+    (m, k), n, dt, dev = x2.shape, w.shape[0], _DT[x2.dtype], x2.device
+    (x0, x1), (w0, w1), xp, wp = x2.stride(), w.stride(), x2.data_ptr(), w.data_ptr()
     y = x2.new_empty((m, n))
-    slope = torch.empty((m, n), dtype=torch.int16, device=x2.device) if save and act else None
+    slope = torch.empty((m, n), dtype=torch.int16, device=dev) if save and act else None
     need = _linear_bytes(dt, m, n, k, x0, x1, xp & 15, w0, w1, wp & 15)
-    ws = torch.empty(need, dtype=torch.uint8, device=x2.device) if need else None
-    _launch("clipvit_linear", x2.device.index, _lib.LinearArgs(
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _launch("clipvit_linear", dev.index, _lib.LinearArgs(
         dt, act, dt if bias is None else _DT[bias.dtype], 0, m, n, k, xp, x0, x1, wp, w0, w1, _ptr(bias), _ptr(res2),
         0 if res2 is None else res2.stride(0), y.data_ptr(), n, _ptr(slope), drop), ws, need)
-    return y, slope
+    return y, slope, (dt, m, n, k, x0, x1, w0, w1)
 
 
 class _Linear(torch.autograd.Function):
@@ -219,34 +219,34 @@ class _Linear(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, act, p, seed, offset):
         needs = ctx.needs_input_grad
         drop = _dropout_args(p, seed, offset)
-        y, slope = _linear_forward(_rows(x), weight, bias, None if residual is None else _rows(residual), act, drop,
-                                   needs[0] or needs[1] or needs[2])
+        x2, w = _panel(_rows(x)), _panel(weight)
+        y, slope, ctx.meta = _linear_forward(x2, w, bias, None if residual is None else _rows(residual), act, drop,
+                                             needs[0] or needs[1] or needs[2])
         # (the offset is saved so that autograd notices when it changes before the backward pass)
-        ctx.save_for_backward(x, weight, slope, offset if torch.is_tensor(offset) else None)
-        ctx.drop, ctx.bias_dtype = drop, None if bias is None else bias.dtype
-        return y.view(*x.shape[:-1], weight.shape[0])
+        ctx.save_for_backward(x2, w, slope, offset if torch.is_tensor(offset) else None)
+        ctx.drop, ctx.bias_dtype, ctx.x_shape = drop, None if bias is None else bias.dtype, x.shape
+        return y.view(*x.shape[:-1], w.shape[0])
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weight, slope, _ = ctx.saved_tensors
+        x2, w, slope, _ = ctx.saved_tensors
         nx, nw, nb, nr = ctx.needs_input_grad[:4]
         dx = dw = db = None
         if nx or nw or nb:
-            x2, w, dy2 = _panel(_rows(x)), _panel(weight), _rows_ld(dy)
-            (m, k), n, dt, drop = x2.shape, w.shape[0], _DT[x2.dtype], ctx.drop
-            (x0, x1), (w0, w1), d0 = x2.stride(), w.stride(), dy2.stride(0)
-            xp, wp, dp = x2.data_ptr(), w.data_ptr(), dy2.data_ptr()
+            dy2 = _rows_ld(dy)
+            (dt, m, n, k, x0, x1, w0, w1), drop, dev = ctx.meta, ctx.drop, x2.device
+            d0, xp, wp, dp = dy2.stride(0), x2.data_ptr(), w.data_ptr(), dy2.data_ptr()
             dx = x2.new_empty((m, k)) if nx else None
             dw = x2.new_empty((n, k)) if nw else None
-            db = torch.empty(n, dtype=ctx.bias_dtype, device=x.device) if nb else None
+            db = torch.empty(n, dtype=ctx.bias_dtype, device=dev) if nb else None
             bdt = _DT[ctx.bias_dtype] if nb else dt
             need = _linear_grad_bytes(dt, bdt, m, n, k, d0, dp & 15, x0, x1, xp & 15, w0, w1, wp & 15, slope is not None, nx, nw, nb, drop.p)
-            ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-            _launch("clipvit_linear_grad", x.device.index, _lib.LinearGradArgs(
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+            _launch("clipvit_linear_grad", dev.index, _lib.LinearGradArgs(
                 dt, bdt, m, n, k, dp, d0, xp, x0, x1, wp, w0, w1, _ptr(slope), _ptr(dx), _ptr(dw), _ptr(db), drop), ws, need)
             if nx:
-                dx = dx.view(x.shape)
+                dx = dx.view(ctx.x_shape)
         return dx, dw, db, dy if nr else None, None, None, None, None
 
 
@@ -276,8 +276,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
         bias = bias.contiguous()
     if _wants_grad(x, weight, bias, residual):
         return _Linear.apply(x, weight, bias, residual, act, p, seed, offset)
-    y, _ = _linear_forward(_rows(x), weight, bias, None if residual is None else _rows(residual), act,
-                           _dropout_args(p, seed, offset) if p else _NO_DROPOUT, False)
+    y = _linear_forward(_panel(_rows(x)), _panel(weight), bias, None if residual is None else _rows(residual), act,
+                        _dropout_args(p, seed, offset) if p else _NO_DROPOUT, False)[0]
     return y.view(*x.shape[:-1], n)
 
 
@@ -332,50 +332,49 @@ def dropout(x: torch.Tensor, p: float, *, seed: int, offset=0, residual: torch.T
 
 
 # ---------------------------------------------------------------- LoRA linear
-def _lora_forward(x2, weight, A, B, bias, scaling, drop):
-    """(y [M, N], u [M, rank rounded up to 32]) of x2 [M, K]."""
-    w = _panel(weight)
-    (m, k), n, r, dt = x2.shape, w.shape[0], A.shape[1], _DT[x2.dtype]
+def _lora_forward(x2, w, A, B, bias, scaling, drop):
+    """(y [M, N], u [M, rank rounded up to 32], the operands' description) of x2 [M, K] rows, w [N, K] as _panel gives it."""
+    (m, k), n, r, dt, dev = x2.shape, w.shape[0], A.shape[1], _DT[x2.dtype], x2.device
     x0, (w0, w1), xp, wp = x2.stride(0), w.stride(), x2.data_ptr(), w.data_ptr()
     y, u = x2.new_empty((m, n)), x2.new_empty((m, (r + 31) // 32 * 32))
     need = _lora_bytes(dt, m, n, k, r, x0, xp & 15, w0, w1, wp & 15)
-    ws = torch.empty(need, dtype=torch.uint8, device=x2.device) if need else None
-    _launch("clipvit_lora_linear", x2.device.index, _lib.LoraArgs(
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _launch("clipvit_lora_linear", dev.index, _lib.LoraArgs(
         dt, dt if bias is None else _DT[bias.dtype], m, n, k, r, xp, x0, wp, w0, w1, A.data_ptr(), A.stride(0), A.stride(1),
         B.data_ptr(), B.stride(0), B.stride(1), _ptr(bias), y.data_ptr(), u.data_ptr(), scaling, 0.0, drop), ws, need)
-    return y, u
+    return y, u, (dt, m, n, k, r, x0, w0, w1)
 
 
 class _LoraLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, A, B, bias, scaling, p, seed, offset):
         drop = _dropout_args(p, seed, offset)
-        y, u = _lora_forward(_rows_ld(x), weight, A, B, bias, scaling, drop)
-        ctx.save_for_backward(x, weight, A, B, u, offset if torch.is_tensor(offset) else None)
-        ctx.drop, ctx.scaling, ctx.bias_dtype = drop, scaling, None if bias is None else bias.dtype
-        return y.view(*x.shape[:-1], weight.shape[0])
+        x2, w = _rows_ld(x), _panel(weight)
+        y, u, ctx.meta = _lora_forward(x2, w, A, B, bias, scaling, drop)
+        ctx.save_for_backward(x2, w, A, B, u, offset if torch.is_tensor(offset) else None)
+        ctx.drop, ctx.scaling, ctx.bias_dtype, ctx.x_shape = drop, scaling, None if bias is None else bias.dtype, x.shape
+        return y.view(*x.shape[:-1], w.shape[0])
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weight, A, B, u, _ = ctx.saved_tensors
+        x2, w, A, B, u, _ = ctx.saved_tensors
         nx, nw, nA, nB, nb = ctx.needs_input_grad[:5]
-        x2, w, dy2 = _rows_ld(x), _panel(weight), _rows_ld(dy)
-        (m, k), n, r, dt, drop = x2.shape, w.shape[0], A.shape[1], _DT[x2.dtype], ctx.drop
-        x0, (w0, w1), d0 = x2.stride(0), w.stride(), dy2.stride(0)
-        xp, wp, dp = x2.data_ptr(), w.data_ptr(), dy2.data_ptr()
+        dy2 = _rows_ld(dy)
+        (dt, m, n, k, r, x0, w0, w1), drop, dev = ctx.meta, ctx.drop, x2.device
+        d0, xp, wp, dp = dy2.stride(0), x2.data_ptr(), w.data_ptr(), dy2.data_ptr()
         dx = x2.new_empty((m, k)) if nx else None
         dw = x2.new_empty((n, k)) if nw else None
         dA = x2.new_empty((k, r)) if nA else None
         dB = x2.new_empty((r, n)) if nB else None
-        db = torch.empty(n, dtype=ctx.bias_dtype, device=x.device) if nb else None
+        db = torch.empty(n, dtype=ctx.bias_dtype, device=dev) if nb else None
         bdt = _DT[ctx.bias_dtype] if nb else dt
         need = _lora_grad_bytes(dt, bdt, m, n, k, r, d0, dp & 15, x0, xp & 15, w0, w1, wp & 15, nx, nw, nA, nB, nb, drop.p)
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-        _launch("clipvit_lora_linear_grad", x.device.index, _lib.LoraGradArgs(
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        _launch("clipvit_lora_linear_grad", dev.index, _lib.LoraGradArgs(
             dt, bdt, m, n, k, r, dp, d0, xp, x0, wp, w0, w1, A.data_ptr(), A.stride(0), A.stride(1), B.data_ptr(), B.stride(0),
             B.stride(1), u.data_ptr(), _ptr(dx), _ptr(dw), _ptr(dA), _ptr(dB), _ptr(db), ctx.scaling, 0.0, drop), ws, need)
-        return dx if dx is None else dx.view(x.shape), dw, dA, dB, db, None, None, None, None
+        return dx if dx is None else dx.view(ctx.x_shape), dw, dA, dB, db, None, None, None, None
 
 
 def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_A: torch.Tensor, lora_B: torch.Tensor,
@@ -403,5 +402,5 @@ def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_A: torch.Tensor, lor
         bias = bias.contiguous()
     if _wants_grad(x, weight, lora_A, lora_B, bias):
         return _LoraLinear.apply(x, weight, lora_A, lora_B, bias, float(scaling), p, seed, offset)
-    return _lora_forward(_rows_ld(x), weight, lora_A, lora_B, bias, float(scaling), _dropout_args(p, seed, offset))[0].view(
+    return _lora_forward(_rows_ld(x), _panel(weight), lora_A, lora_B, bias, float(scaling), _dropout_args(p, seed, offset))[0].view(
         *x.shape[:-1], n)
