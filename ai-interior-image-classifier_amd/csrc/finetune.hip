@@ -526,22 +526,23 @@ Dropout make_dropout(const clipvit_dropout_args& d) {
     return r;
 }
 
-// a [rows, cols] view with one unit stride -> (contiguous along columns?, row stride); false: refused
+// a [rows, cols] view with one unit stride -> (contiguous along columns?, row stride); false: refused. A single column has
+// no second k row: any stride does that puts one outside a tile's resource (at most 512 bytes) in 32 bits.
 bool panel_of(int64_t s0, int64_t s1, int64_t rows, int64_t cols, int& contig, int64_t& ld) {
     if (s1 == 1 || cols == 1) {
         contig = 1;
         ld = rows <= 1 ? up(cols, 8) : s0;
         if (cols == 1 && rows > 1 && s0 == 1) {  // one column of consecutive elements
             contig = 0;
-            ld = up(rows, 8);
+            ld = 4096;
             return true;
         }
         return rows <= 1 || (ld >= cols && ld < MATMUL_MAX_LD);
     }
     if (s0 == 1 || rows == 1) {
         contig = 0;
-        ld = cols <= 1 ? up(rows, 8) : s1;
-        return ld >= rows && ld < MATMUL_MAX_LD;
+        ld = cols <= 1 ? 4096 : s1;
+        return cols <= 1 || (ld >= rows && ld < MATMUL_MAX_LD);
     }
     return false;
 }

@@ -20,7 +20,8 @@ name the mask: calls that share both (and the row count) share their masks.
 
 Every call runs on the current stream of the tensors' device and allocates its output and workspace from torch's
 caching allocator. There is no CPU fallback: CPU tensors raise ``ClipVitError``. A backward may be captured
-into a graph through ``torch.autograd.grad`` after the usual warm-up on a side stream.
+into a graph through ``torch.autograd.grad`` after the usual warm-up on a side stream, once no eager autograd graph of
+the same leaves is alive (a capture that finds one raises). Matrices of more than one row hold fewer than 2^22 columns.
 """
 from __future__ import annotations
 
@@ -199,6 +200,27 @@ def _wants_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _differentiable(fn, args, leaves):
+    """fn.apply(*args), with the stream noted at the gradient nodes of the leaves among `leaves`.
+
+    A leaf's gradient node keeps the stream of the graph that it was made for, for as long as one of its graphs lives. A
+    backward pass captured on another stream would draw that stream into the capture, which ends the process, so such
+    a capture is refused here, before anything is recorded."""
+    stream = _stream(args[0].device.index)
+    if torch.cuda.is_current_stream_capturing():
+        for t in leaves:
+            if t is None or not t.requires_grad or not t.is_leaf:
+                continue
+            if torch.autograd.graph.get_gradient_edge(t).node.metadata.get("interior_amd", stream) != stream:
+                raise RuntimeError("a graph capture would differentiate a leaf whose earlier autograd graph, made on another stream, "
+                                   "is still alive: delete that graph's outputs (or run it on the capturing stream) first")
+    y = fn.apply(*args)
+    for node, _ in y.grad_fn.next_functions:  # (after the call: now the new graph holds the nodes)
+        if node is not None:
+            node.metadata.setdefault("interior_amd", stream)
+    return y
+
+
 # ---------------------------------------------------------------- linear
 def _linear_forward(x2, w, bias, res2, act, drop, save):
     """(y [M, N], act'(z) or None, the operands' description) of x2 [M, K], w [N, K] as _panel gives them."""
@@ -275,7 +297,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     if bias is not None and bias.stride(0) != 1:
         bias = bias.contiguous()
     if _wants_grad(x, weight, bias, residual):
-        return _Linear.apply(x, weight, bias, residual, act, p, seed, offset)
+        return _differentiable(_Linear, (x, weight, bias, residual, act, p, seed, offset), (x, weight, bias, residual))
     y = _linear_forward(_panel(_rows(x)), _panel(weight), bias, None if residual is None else _rows(residual), act,
                         _dropout_args(p, seed, offset) if p else _NO_DROPOUT, False)[0]
     return y.view(*x.shape[:-1], n)
@@ -327,7 +349,7 @@ def dropout(x: torch.Tensor, p: float, *, seed: int, offset=0, residual: torch.T
     _check_counter(seed, offset, x)
     _need_device(x, residual)
     if _wants_grad(x, residual):
-        return _Dropout.apply(x, residual, p, seed, offset)
+        return _differentiable(_Dropout, (x, residual, p, seed, offset), (x, residual))
     return _dropout_call(x, residual, _dropout_args(p, seed, offset))
 
 
@@ -401,6 +423,7 @@ def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_A: torch.Tensor, lor
     if bias is not None and bias.stride(0) != 1:
         bias = bias.contiguous()
     if _wants_grad(x, weight, lora_A, lora_B, bias):
-        return _LoraLinear.apply(x, weight, lora_A, lora_B, bias, float(scaling), p, seed, offset)
+        return _differentiable(_LoraLinear, (x, weight, lora_A, lora_B, bias, float(scaling), p, seed, offset),
+                               (x, weight, lora_A, lora_B, bias))
     return _lora_forward(_rows_ld(x), _panel(weight), lora_A, lora_B, bias, float(scaling), _dropout_args(p, seed, offset))[0].view(
         *x.shape[:-1], n)

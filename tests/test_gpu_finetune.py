@@ -368,6 +368,35 @@ def test_captured_step_replays(gpu):
     assert torch.equal(seen[1], seen[3]) and not torch.equal(seen[0], seen[1])
 
 
+def test_capture_beside_a_live_eager_graph_is_refused(gpu):
+    """While an eager graph of the same leaves lives, a captured forward for a backward raises before it records anything;
+    once that graph is gone the capture works."""
+    p, x, dy = mlp_params(gpu), rand(40, 64, seed=7).to(gpu).requires_grad_(), rand(40, 64, seed=8).to(gpu)
+    want = [t.detach().clone() for t in mlp_step(x, p, dy, 3)]
+    eager = ops.dropout(x, 0.5, seed=1)
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            ops.dropout(x, 0.5, seed=1)
+    del eager
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = mlp_step(x, p, dy, 3)
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
+
+
+def test_one_column_of_many_rows(gpu):
+    """K = 1 on 2^26 + 100 rows: the operand is one run of elements, whose length passes what a tile's offsets hold."""
+    m = 2 ** 26 + 100
+    x, w = torch.randn(m, 1, device=gpu).to(BF), torch.tensor([[2.0], [-0.5], [1.0], [4.0], [0.25], [-1.0], [8.0], [0.5]], dtype=BF, device=gpu)
+    y = ops.linear(x, w)
+    assert torch.equal(y, x * w.t())  # powers of two: exact
+
+
 @pytest.mark.parametrize("p", [0.0, 0.25])
 def test_rounds_and_remaining_rows(gpu, p):
     """7300 x 2304 is one round of 256-wide tiles (28 rows of 9) and 132 rows more, a launch of their own: masks, residual,
