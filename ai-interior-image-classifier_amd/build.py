@@ -19,6 +19,7 @@ CSRC = PKG_DIR / "csrc"
 INCLUDE = ROOT / "include"
 BUILD = PKG_DIR / "build"
 LIB = PKG_DIR / "libclipvit_hip.so"
+TORCH_LIB = PKG_DIR / "_ops_torch.so"
 ARCH = "gfx950"
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -71,16 +72,40 @@ def _compile(src: Path) -> tuple[Path, str]:
     return obj, r.stderr
 
 
+def _build_torch_binding() -> None:
+    """_ops_torch.so: the autograd binding of the fine-tuning operators (host C++ against this torch's headers)."""
+    src = CSRC / "ops_torch.cpp"
+    if not _needs(TORCH_LIB, [src, INCLUDE / "clipvit.h", Path(__file__)]):
+        return
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    tmp = TORCH_LIB.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1",
+           "-DUSE_ROCM=1", f"-I{INCLUDE}", "-isystem/opt/rocm/include",
+           *(f"-isystem{d}" for d in include_paths()), f"-isystem{sysconfig.get_paths()['include']}",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", str(src), "-o", str(tmp),
+           f"-L{Path(torch.__file__).parent / 'lib'}", "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-ldl"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed for {src.name}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, TORCH_LIB)
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile and link libclipvit_hip.so; return its path."""
+    """Compile and link libclipvit_hip.so and the torch binding beside it; return the library's path."""
     BUILD.mkdir(exist_ok=True)
     srcs = _sources()
     if force:
         for o in BUILD.glob("*.o"):
             o.unlink()
+        TORCH_LIB.unlink(missing_ok=True)
     jobs = min(len(srcs), int(os.environ.get("MAX_JOBS", "8")), 16)
     with ThreadPoolExecutor(max_workers=max(jobs, 1)) as ex:
+        binding = ex.submit(_build_torch_binding)
         results = list(ex.map(_compile, srcs))
+        binding.result()
     objs = [o for o, _ in results]
     if verbose:
         for o, err in results:

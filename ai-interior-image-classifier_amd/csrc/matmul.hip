@@ -49,7 +49,7 @@ struct Half {
 // One operand's panel of a tile: R rows (KC) or columns, staged by NW waves, NP pieces of 1 KB each.
 template <bool KC, int R, int NW, class Map>
 struct Panel {
-    static constexpr int NP = R / 8 / NW, BYTES = R * 128;
+    static constexpr int NP = R / 8 / NW;
     const unsigned char* base;
     unsigned long long kstep;  // column panel: bytes of 64 k rows
     unsigned range;            // row panel: bytes; column panel: bytes of its last valid row from the first column
@@ -431,6 +431,11 @@ __device__ __forceinline__ void read_step(const Frags<T, AK, 128, 4>& fa, unsign
 //  * B0(T), read in 4 T - 2 and 4 T - 1, by B0(T + 2) in slot 4 T + 1; B1(T), read in 4 T and 4 T + 1, by B1(T + 2) in
 //    slot 4 T + 3: group 1, in its read segments, where it also waits, five slots after the issue.
 // Steps past the last k-tile stage zeros into parts nobody reads (kept, so that the counted waits hold).
+// Bound by the MFMA segments and what a slot adds to their 512 cycles (barrier, waits, staging): at 8192^3 bf16 805 us,
+// 1360 TFLOP/s, for the forward's layouts, 795 us for dx's, 820 us for dw's (a library product of that size: 700 us). With
+// the reads waited for before the barrier and refills a slot earlier it was 874 us; issuing the staging between the
+// MFMAs instead of before them changed nothing (778-794 against 789-791 us on one card). A tile costs 8.5 us besides its
+// k-tiles' 1.4 us each, of which the epilogue is 6 (11 with quick_gelu, whose exponential and reciprocal are quarter rate).
 template <typename T, bool AK, bool BK>
 __global__ __launch_bounds__(512, 1) void matmul256_kernel(Matmul a, float* part, int N4, int kslice) {
     typedef typename T::vec8 vec8;

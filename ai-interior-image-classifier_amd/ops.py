@@ -3,7 +3,8 @@ the unmerged LoRA Linear, each differentiable.
 
 The reference trains its adapters on ``LoRALinear`` modules (main.py:34-59, train_lora.py:62-100), which
 :mod:`lora` only merges; these are that Linear's forward and gradients, in hand-written gfx950 kernels
-(csrc/matmul.hip, csrc/finetune.hip, the ``clipvit_linear`` family of include/clipvit.h):
+(csrc/matmul.hip, csrc/finetune.hip, the ``clipvit_linear`` family of include/clipvit.h) behind native autograd
+nodes (csrc/ops_torch.cpp):
 
 * ``linear(x, weight, bias, residual, activation=, dropout_p=, seed=, offset=)``
   = residual + dropout(act(x weight^T + bias));
@@ -21,23 +22,36 @@ name the mask: calls that share both (and the row count) share their masks.
 Every call runs on the current stream of the tensors' device and allocates its output and workspace from torch's
 caching allocator. There is no CPU fallback: CPU tensors raise ``ClipVitError``. A backward may be captured
 into a graph through ``torch.autograd.grad`` after the usual warm-up on a side stream, once no eager autograd graph of
-the same leaves is alive (a capture that finds one raises). Matrices of more than one row hold fewer than 2^22 columns.
+the same leaves is alive (a capture that finds one raises). They are differentiable once (no ``create_graph``). Matrices of more than one row hold fewer than 2^22 columns.
 """
 from __future__ import annotations
 
 import ctypes
-import functools
-import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
 _DT = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 ACTIVATIONS = {"none": 0, "quick_gelu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4, "relu": 5}
-_byref = ctypes.byref
 _MASK64 = (1 << 64) - 1
+_binding_module = None
+
+
+def _binding():
+    """The native autograd binding (csrc/ops_torch.cpp), given this process's build of the library."""
+    global _binding_module
+    if _binding_module is None:
+        try:
+            from . import _ops_torch as m
+        except ImportError as e:
+            raise _lib.ClipVitError(_lib.E_STATE, f"_ops_torch.so is not built (run __graft_entry__.build()): {e}") from e
+        L = _lib.lib()
+        names = [f"clipvit_{n}{w}" for n in ("linear", "linear_grad", "lora_linear", "lora_linear_grad") for w in ("", "_workspace")]
+        m.set_library({n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in (*names, "clipvit_dropout", "clipvit_last_error")},
+                      _lib.ClipVitError)
+        _binding_module = m
+    return _binding_module
 
 
 # ---------------------------------------------------------------- arguments
@@ -87,191 +101,14 @@ def _check_counter(seed, offset, x: torch.Tensor) -> None:
         raise TypeError(f"offset must be an int or an int64 tensor, got {type(offset).__name__}")
 
 
-def _dropout_args(p: float, seed: int, offset) -> _lib.DropoutArgs:
+def _counter(seed: int, offset):
+    """(seed, offset, offset tensor or None) as 64-bit words."""
     if torch.is_tensor(offset):
-        return _lib.DropoutArgs(p, seed & _MASK64, 0, offset.data_ptr())
-    return _lib.DropoutArgs(p, seed & _MASK64, offset & _MASK64, None)
-
-
-_NO_DROPOUT = _lib.DropoutArgs(0.0, 0, 0, None)
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """[..., n] as [rows, n] with unit column stride and rows that do not overlap (a copy only where the
-    strides are something else)."""
-    if t.dim() != 2:
-        t = t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        t = t.contiguous()
-    return t
-
-
-_MAX_LD = 1 << 22
-
-
-def _rows_ld(t: torch.Tensor) -> torch.Tensor:
-    """_rows with a row stride that the matrix products address (below 2^22, or one row)."""
-    t = _rows(t)
-    return t.contiguous() if t.shape[0] > 1 and t.stride(0) >= _MAX_LD else t
-
-
-def _panel(t: torch.Tensor) -> torch.Tensor:
-    """A matrix operand: one unit stride, rows (or columns) that do not overlap, the other stride below 2^22."""
-    r, c = t.shape
-    s0, s1 = t.stride()
-    if (s1 == 1 or c == 1) and (r <= 1 or c <= s0 < _MAX_LD):
-        return t
-    if (s0 == 1 or r == 1) and (c <= 1 or r <= s1 < _MAX_LD):
-        return t
-    return t.contiguous()
-
-
-def _stream(index: int):
-    """The current stream of a device as the C entry points take it."""
-    return torch._C._cuda_getCurrentRawStream(index)
-
-
-class _On:
-    """The tensors' device as the current one while kernels are launched; entered only where it is not already."""
-
-    def __init__(self, index: int):
-        self.index, self.prev = index, torch.cuda.current_device()
-
-    def __enter__(self):
-        torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        torch.cuda.set_device(self.prev)
-
-
-def _launch(name: str, index: int, args, ws, nbytes: int) -> None:
-    """One C call on the current stream of device `index`."""
-    fn = getattr(_lib.lib(), name)
-    ptr = ws.data_ptr() if nbytes else None
-    if torch.cuda.current_device() == index:
-        rc = fn(_stream(index), _byref(args), ptr, nbytes)
-    else:
-        with _On(index):
-            rc = fn(_stream(index), _byref(args), ptr, nbytes)
-    if rc:
-        _lib.check(rc)
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _bytes(name: str, args) -> int:
-    need = ctypes.c_size_t()
-    _lib.check(getattr(_lib.lib(), name)(_byref(args), _byref(need)))
-    return need.value
-
-
-# Workspace sizes by sizes, strides, alignments and wanted outputs, which is all they depend on (pointers are
-# stand-ins of the same alignment).
-@functools.lru_cache(maxsize=4096)
-def _linear_bytes(dt, m, n, k, x0, x1, xa, w0, w1, wa) -> int:
-    return _bytes("clipvit_linear_workspace", _lib.LinearArgs(
-        dt, 0, dt, 0, m, n, k, 4096 + xa, x0, x1, 4096 + wa, w0, w1, None, None, 0, 4096, n, None, _NO_DROPOUT))
-
-
-@functools.lru_cache(maxsize=4096)
-def _linear_grad_bytes(dt, bdt, m, n, k, d0, da, x0, x1, xa, w0, w1, wa, slope, dx, dw, db, p) -> int:
-    return _bytes("clipvit_linear_grad_workspace", _lib.LinearGradArgs(
-        dt, bdt, m, n, k, 4096 + da, d0, 4096 + xa, x0, x1, 4096 + wa, w0, w1, 4096 if slope else None,
-        4096 if dx else None, 4096 if dw else None, 4096 if db else None, _lib.DropoutArgs(p, 0, 0, None)))
-
-
-@functools.lru_cache(maxsize=4096)
-def _lora_bytes(dt, m, n, k, r, x0, xa, w0, w1, wa) -> int:
-    return _bytes("clipvit_lora_linear_workspace", _lib.LoraArgs(
-        dt, dt, m, n, k, r, 4096 + xa, x0, 4096 + wa, w0, w1, 4096, r, 1, 4096, n, 1, None, 4096, 4096, 1.0, 0.0, _NO_DROPOUT))
-
-
-@functools.lru_cache(maxsize=4096)
-def _lora_grad_bytes(dt, bdt, m, n, k, r, d0, da, x0, xa, w0, w1, wa, dx, dw, dA, dB, db, p) -> int:
-    return _bytes("clipvit_lora_linear_grad_workspace", _lib.LoraGradArgs(
-        dt, bdt, m, n, k, r, 4096 + da, d0, 4096 + xa, x0, 4096 + wa, w0, w1, 4096, r, 1, 4096, n, 1, 4096,
-        4096 if dx else None, 4096 if dw else None, 4096 if dA else None, 4096 if dB else None, 4096 if db else None, 1.0, 0.0,
-        _lib.DropoutArgs(p, 0, 0, None)))
-
-
-def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-def _differentiable(fn, args, leaves):
-    """fn.apply(*args), with the stream noted at the gradient nodes of the leaves among `leaves`.
-
-    A leaf's gradient node keeps the stream of the graph that it was made for, for as long as one of its graphs lives. A
-    backward pass captured on another stream would draw that stream into the capture, which ends the process, so such
-    a capture is refused here, before anything is recorded."""
-    stream = _stream(args[0].device.index)
-    if torch.cuda.is_current_stream_capturing():
-        for t in leaves:
-            if t is None or not t.requires_grad or not t.is_leaf:
-                continue
-            if torch.autograd.graph.get_gradient_edge(t).node.metadata.get("interior_amd", stream) != stream:
-                raise RuntimeError("a graph capture would differentiate a leaf whose earlier autograd graph, made on another stream, "
-                                   "is still alive: delete that graph's outputs (or run it on the capturing stream) first")
-    y = fn.apply(*args)
-    for node, _ in y.grad_fn.next_functions:  # (after the call: now the new graph holds the nodes)
-        if node is not None:
-            node.metadata.setdefault("interior_amd", stream)
-    return y
+        return seed & _MASK64, 0, offset
+    return seed & _MASK64, offset & _MASK64, None
 
 
 # ---------------------------------------------------------------- linear
-def _linear_forward(x2, w, bias, res2, act, drop, save):
-    """(y [M, N], act'(z) or None, the operands' description) of x2 [M, K], w [N, K] as _panel gives them."""
-    (m, k), n, dt, dev = x2.shape, w.shape[0], _DT[x2.dtype], x2.device
-    (x0, x1), (w0, w1), xp, wp = x2.stride(), w.stride(), x2.data_ptr(), w.data_ptr()
-    y = x2.new_empty((m, n))
-    slope = torch.empty((m, n), dtype=torch.int16, device=dev) if save and act else None
-    need = _linear_bytes(dt, m, n, k, x0, x1, xp & 15, w0, w1, wp & 15)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _launch("clipvit_linear", dev.index, _lib.LinearArgs(
-        dt, act, dt if bias is None else _DT[bias.dtype], 0, m, n, k, xp, x0, x1, wp, w0, w1, _ptr(bias), _ptr(res2),
-        0 if res2 is None else res2.stride(0), y.data_ptr(), n, _ptr(slope), drop), ws, need)
-    return y, slope, (dt, m, n, k, x0, x1, w0, w1)
-
-
-class _Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, act, p, seed, offset):
-        needs = ctx.needs_input_grad
-        drop = _dropout_args(p, seed, offset)
-        x2, w = _panel(_rows(x)), _panel(weight)
-        y, slope, ctx.meta = _linear_forward(x2, w, bias, None if residual is None else _rows(residual), act, drop,
-                                             needs[0] or needs[1] or needs[2])
-        # (the offset is saved so that autograd notices when it changes before the backward pass)
-        ctx.save_for_backward(x2, w, slope, offset if torch.is_tensor(offset) else None)
-        ctx.drop, ctx.bias_dtype, ctx.x_shape = drop, None if bias is None else bias.dtype, x.shape
-        return y.view(*x.shape[:-1], w.shape[0])
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x2, w, slope, _ = ctx.saved_tensors
-        nx, nw, nb, nr = ctx.needs_input_grad[:4]
-        dx = dw = db = None
-        if nx or nw or nb:
-            dy2 = _rows_ld(dy)
-            (dt, m, n, k, x0, x1, w0, w1), drop, dev = ctx.meta, ctx.drop, x2.device
-            d0, xp, wp, dp = dy2.stride(0), x2.data_ptr(), w.data_ptr(), dy2.data_ptr()
-            dx = x2.new_empty((m, k)) if nx else None
-            dw = x2.new_empty((n, k)) if nw else None
-            db = torch.empty(n, dtype=ctx.bias_dtype, device=dev) if nb else None
-            bdt = _DT[ctx.bias_dtype] if nb else dt
-            need = _linear_grad_bytes(dt, bdt, m, n, k, d0, dp & 15, x0, x1, xp & 15, w0, w1, wp & 15, slope is not None, nx, nw, nb, drop.p)
-            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-            _launch("clipvit_linear_grad", dev.index, _lib.LinearGradArgs(
-                dt, bdt, m, n, k, dp, d0, xp, x0, x1, wp, w0, w1, _ptr(slope), _ptr(dx), _ptr(dw), _ptr(db), drop), ws, need)
-            if nx:
-                dx = dx.view(ctx.x_shape)
-        return dx, dw, db, dy if nr else None, None, None, None, None
-
-
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
            residual: torch.Tensor | None = None, *, activation: str = "none", dropout_p: float = 0.0,
            seed: int = 0, offset=0) -> torch.Tensor:
@@ -293,48 +130,10 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     p = _check_p(dropout_p)
     _check_counter(seed, offset, x)
     _need_device(x, weight, bias, residual)
-    act = ACTIVATIONS[activation]
-    if bias is not None and bias.stride(0) != 1:
-        bias = bias.contiguous()
-    if _wants_grad(x, weight, bias, residual):
-        return _differentiable(_Linear, (x, weight, bias, residual, act, p, seed, offset), (x, weight, bias, residual))
-    y = _linear_forward(_panel(_rows(x)), _panel(weight), bias, None if residual is None else _rows(residual), act,
-                        _dropout_args(p, seed, offset) if p else _NO_DROPOUT, False)[0]
-    return y.view(*x.shape[:-1], n)
+    return _binding().linear(x, weight, bias, residual, ACTIVATIONS[activation], p, *_counter(seed, offset))
 
 
 # ---------------------------------------------------------------- dropout
-def _dropout_call(x, residual, drop):
-    x2 = _rows(x)
-    res2 = None if residual is None else _rows(residual)
-    y, index = torch.empty(x2.shape, dtype=x.dtype, device=x.device), x.device.index
-    args = (_DT[x.dtype], x2.data_ptr(), x2.stride(0), _ptr(res2), 0 if res2 is None else res2.stride(0), y.data_ptr(), y.stride(0),
-            x2.shape[0], x2.shape[1], _byref(drop))
-    if torch.cuda.current_device() == index:
-        rc = _lib.lib().clipvit_dropout(_stream(index), *args)
-    else:
-        with _On(index):
-            rc = _lib.lib().clipvit_dropout(_stream(index), *args)
-    if rc:
-        _lib.check(rc)
-    return y.view(x.shape)
-
-
-class _Dropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, p, seed, offset):
-        ctx.drop = _dropout_args(p, seed, offset)
-        ctx.save_for_backward(offset if torch.is_tensor(offset) else None)
-        return _dropout_call(x, residual, ctx.drop)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        ctx.saved_tensors  # raises where a tensor offset changed since the forward pass
-        dx = _dropout_call(dy, None, ctx.drop) if ctx.needs_input_grad[0] else None
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
-
-
 def dropout(x: torch.Tensor, p: float, *, seed: int, offset=0, residual: torch.Tensor | None = None) -> torch.Tensor:
     """residual + dropout(x): fp32, bf16 or fp16 of any shape; the last dimension is the mask's column, the others
     together its row. Kept elements are scaled by 1 / (1 - p), dropped ones are exactly 0 (NaN included). The
@@ -348,57 +147,10 @@ def dropout(x: torch.Tensor, p: float, *, seed: int, offset=0, residual: torch.T
     p = _check_p(p)
     _check_counter(seed, offset, x)
     _need_device(x, residual)
-    if _wants_grad(x, residual):
-        return _differentiable(_Dropout, (x, residual, p, seed, offset), (x, residual))
-    return _dropout_call(x, residual, _dropout_args(p, seed, offset))
+    return _binding().dropout(x, residual, p, *_counter(seed, offset))
 
 
 # ---------------------------------------------------------------- LoRA linear
-def _lora_forward(x2, w, A, B, bias, scaling, drop):
-    """(y [M, N], u [M, rank rounded up to 32], the operands' description) of x2 [M, K] rows, w [N, K] as _panel gives it."""
-    (m, k), n, r, dt, dev = x2.shape, w.shape[0], A.shape[1], _DT[x2.dtype], x2.device
-    x0, (w0, w1), xp, wp = x2.stride(0), w.stride(), x2.data_ptr(), w.data_ptr()
-    y, u = x2.new_empty((m, n)), x2.new_empty((m, (r + 31) // 32 * 32))
-    need = _lora_bytes(dt, m, n, k, r, x0, xp & 15, w0, w1, wp & 15)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _launch("clipvit_lora_linear", dev.index, _lib.LoraArgs(
-        dt, dt if bias is None else _DT[bias.dtype], m, n, k, r, xp, x0, wp, w0, w1, A.data_ptr(), A.stride(0), A.stride(1),
-        B.data_ptr(), B.stride(0), B.stride(1), _ptr(bias), y.data_ptr(), u.data_ptr(), scaling, 0.0, drop), ws, need)
-    return y, u, (dt, m, n, k, r, x0, w0, w1)
-
-
-class _LoraLinear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, A, B, bias, scaling, p, seed, offset):
-        drop = _dropout_args(p, seed, offset)
-        x2, w = _rows_ld(x), _panel(weight)
-        y, u, ctx.meta = _lora_forward(x2, w, A, B, bias, scaling, drop)
-        ctx.save_for_backward(x2, w, A, B, u, offset if torch.is_tensor(offset) else None)
-        ctx.drop, ctx.scaling, ctx.bias_dtype, ctx.x_shape = drop, scaling, None if bias is None else bias.dtype, x.shape
-        return y.view(*x.shape[:-1], w.shape[0])
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x2, w, A, B, u, _ = ctx.saved_tensors
-        nx, nw, nA, nB, nb = ctx.needs_input_grad[:5]
-        dy2 = _rows_ld(dy)
-        (dt, m, n, k, r, x0, w0, w1), drop, dev = ctx.meta, ctx.drop, x2.device
-        d0, xp, wp, dp = dy2.stride(0), x2.data_ptr(), w.data_ptr(), dy2.data_ptr()
-        dx = x2.new_empty((m, k)) if nx else None
-        dw = x2.new_empty((n, k)) if nw else None
-        dA = x2.new_empty((k, r)) if nA else None
-        dB = x2.new_empty((r, n)) if nB else None
-        db = torch.empty(n, dtype=ctx.bias_dtype, device=dev) if nb else None
-        bdt = _DT[ctx.bias_dtype] if nb else dt
-        need = _lora_grad_bytes(dt, bdt, m, n, k, r, d0, dp & 15, x0, xp & 15, w0, w1, wp & 15, nx, nw, nA, nB, nb, drop.p)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        _launch("clipvit_lora_linear_grad", dev.index, _lib.LoraGradArgs(
-            dt, bdt, m, n, k, r, dp, d0, xp, x0, wp, w0, w1, A.data_ptr(), A.stride(0), A.stride(1), B.data_ptr(), B.stride(0),
-            B.stride(1), u.data_ptr(), _ptr(dx), _ptr(dw), _ptr(dA), _ptr(dB), _ptr(db), ctx.scaling, 0.0, drop), ws, need)
-        return dx if dx is None else dx.view(ctx.x_shape), dw, dA, dB, db, None, None, None, None
-
-
 def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_A: torch.Tensor, lora_B: torch.Tensor,
                 bias: torch.Tensor | None = None, *, scaling: float = 1.0, dropout_p: float = 0.0, seed: int = 0,
                 offset=0) -> torch.Tensor:
@@ -420,10 +172,4 @@ def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_A: torch.Tensor, lor
     p = _check_p(dropout_p)
     _check_counter(seed, offset, x)
     _need_device(x, weight, lora_A, lora_B, bias)
-    if bias is not None and bias.stride(0) != 1:
-        bias = bias.contiguous()
-    if _wants_grad(x, weight, lora_A, lora_B, bias):
-        return _differentiable(_LoraLinear, (x, weight, lora_A, lora_B, bias, float(scaling), p, seed, offset),
-                               (x, weight, lora_A, lora_B, bias))
-    return _lora_forward(_rows_ld(x), _panel(weight), lora_A, lora_B, bias, float(scaling), _dropout_args(p, seed, offset))[0].view(
-        *x.shape[:-1], n)
+    return _binding().lora_linear(x, weight, lora_A, lora_B, bias, float(scaling), p, *_counter(seed, offset))

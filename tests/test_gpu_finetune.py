@@ -431,3 +431,51 @@ def test_long_rows_offsets_past_32_bits(gpu):
     for a in range(0, m, 53000):
         want += y[a:a + 53000].double().t() @ x[a:a + 53000].double()
     assert (dw.double() - want).norm() <= 2.0 ** -8 * want.norm()
+
+
+def test_graph_is_run_once_unless_retained(gpu):
+    x = rand(40, 24, dtype=BF, seed=1).to(gpu).requires_grad_()
+    w = rand(16, 24, dtype=BF, seed=2).to(gpu).requires_grad_()
+    A, B = (rand(*s, dtype=BF, seed=i).to(gpu).requires_grad_() for i, s in ((3, (24, 4)), (4, (4, 16))))
+    for make, leaves in ((lambda: ops.linear(x, w, activation="gelu", dropout_p=0.2, seed=1), (x, w)),
+                         (lambda: ops.dropout(x, 0.3, seed=1), (x,)),
+                         (lambda: ops.lora_linear(x, w, A, B, scaling=0.5, dropout_p=0.2, seed=1), (x, w, A, B))):
+        y = make()
+        dy = torch.ones_like(y)
+        first = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+        second = torch.autograd.grad(y, leaves, dy)
+        assert all(torch.equal(a, b) for a, b in zip(first, second))
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(y, leaves, dy)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(make(), leaves, dy, create_graph=True)
+
+
+def test_operand_changed_in_place_is_refused_in_backward(gpu):
+    x = rand(3, 5, 24, dtype=HF, seed=1).to(gpu)
+    w = rand(16, 24, dtype=HF, seed=2).to(gpu).requires_grad_()
+    y = ops.linear(x, w)
+    x.mul_(2)  # a view of it is what the node saved
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_two_threads(gpu):
+    import threading
+    x, w = rand(300, 64, dtype=BF, seed=1).to(gpu), rand(128, 64, dtype=BF, seed=2).to(gpu)
+    want = ops.linear(x, w, activation="silu", dropout_p=0.1, seed=5)
+    got = [None] * 4
+
+    def work(i):
+        xs = x.clone().requires_grad_()
+        for _ in range(20):
+            got[i] = ops.linear(xs, w, activation="silu", dropout_p=0.1, seed=5)
+            got[i].backward(torch.ones_like(got[i]))
+        torch.cuda.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(g, want) for g in got)
