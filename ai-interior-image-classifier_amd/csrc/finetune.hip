@@ -2,7 +2,7 @@
 // thin products, and the C entry points of all of them (the matrix product itself is matmul.hip).
 //
 // A Linear with an adapter (main.py:19-59): y = x W^T + b + s (dropout(x) A) B. The reference runs the
-// adapter as a side branch while it trains (train_lora.py) and this library merges it for inference
+// adapter as a side branch while it trains (train_lora.py, without dropout) and this library merges it for inference
 // (clipvit_load_lora); these operators are the unmerged form with its gradients.
 #include <cmath>
 #include <string>
@@ -359,9 +359,15 @@ __global__ __launch_bounds__(256) void lora_down_kernel(DownArgs a) {
                 c0[i][j] += red[w][i][lane][j];
                 c1[i][j] += red[w][i][lane][4 + j];
             }
+        // a padded rank is zero whatever the row holds (the zero factor times an infinity is not)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            c0[i][j] = r0 + 4 * g + j < a.rank ? c0[i][j] * a.alpha : 0.f;
+            c1[i][j] = r0 + 16 + 4 * g + j < a.rank ? c1[i][j] * a.alpha : 0.f;
+        }
         u16* u = a.u + (int64_t)m * a.R + r0 + 4 * g;
-        *(uint2*)u = make_uint2(pack2<T>(c0[i][0] * a.alpha, c0[i][1] * a.alpha), pack2<T>(c0[i][2] * a.alpha, c0[i][3] * a.alpha));
-        *(uint2*)(u + 16) = make_uint2(pack2<T>(c1[i][0] * a.alpha, c1[i][1] * a.alpha), pack2<T>(c1[i][2] * a.alpha, c1[i][3] * a.alpha));
+        *(uint2*)u = make_uint2(pack2<T>(c0[i][0], c0[i][1]), pack2<T>(c0[i][2], c0[i][3]));
+        *(uint2*)(u + 16) = make_uint2(pack2<T>(c1[i][0], c1[i][1]), pack2<T>(c1[i][2], c1[i][3]));
     }
 }
 

@@ -282,6 +282,27 @@ def test_lora_linear(gpu, dtype, p, m, k, n, r):
         assert torch.equal(ops.lora_linear(*leaves, **kw), y)
 
 
+@pytest.mark.parametrize("r,k", [(4, 64), (4, 61), (20, 128)])
+def test_lora_infinity_stays_an_infinity(gpu, r, k):
+    """Positive operands, one infinite element: the row is +inf as in the formula (a padded rank times it would be NaN),
+    the others are untouched, and so is everything where the mask drops the element."""
+    x, w, A, B = (rand(*s, seed=i).abs() + 0.1 for i, s in enumerate(((40, k), (24, k), (k, r), (r, 24))))
+    args = [t.to(gpu) for t in (x, w, A, B)]
+    clean = ops.lora_linear(*args, scaling=2.0)
+    args[0][7, 5] = float("inf")
+    y = ops.lora_linear(*args, scaling=2.0)
+    assert bool((y[7] == float("inf")).all())
+    rows = [i for i in range(40) if i != 7]
+    assert torch.equal(y[rows], clean[rows])
+    args[1][:, 5] = 0  # the base product is NaN there; with p = 1 the adapter's side adds nothing
+    assert bool(ops.lora_linear(*args, scaling=2.0, dropout_p=1.0, seed=1)[7].isnan().all())
+    x2 = x.to(gpu).requires_grad_()
+    dy = torch.ones(40, 24, dtype=BF, device=gpu)
+    dy[3, 2] = float("inf")
+    dx, = torch.autograd.grad(ops.lora_linear(x2, w.to(gpu), *args[2:], scaling=2.0), x2, dy)
+    assert bool((dx[3] == float("inf")).all()) and bool(torch.isfinite(dx[:3]).all()) and bool(torch.isfinite(dx[4:]).all())
+
+
 def test_lora_equals_merge_and_frozen_weight(gpu):
     """B = 0 gives the base Linear bit for bit (the reference's initial state, main.py:27), with a gradient for B."""
     x, w, A = rand(200, 128).to(gpu), rand(96, 128, scale=0.1, seed=1).to(gpu), rand(128, 4, scale=0.02, seed=2).to(gpu).requires_grad_()
