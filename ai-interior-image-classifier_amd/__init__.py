@@ -5,6 +5,7 @@ root registers it). Layout:
     csrc/          hand-written gfx950 HIP kernels + the C ABI (include/clipvit.h)
     _lib.py        ctypes binding (GIL released inside every call)
     engine.py      VisionEngine: one handle = one GPU
+    ops.py         linear, dropout, lora_linear with gradients (csrc/ops_torch.cpp: autograd nodes)
     analyzer.py    the reference's predict / analyze surface (main.py, main_API.py)
     lora.py        comprehensive_lora*.pth format + binding rule, merged at load
     weights.py     OpenAI names, synthetic seeded weights, local checkpoint loader
