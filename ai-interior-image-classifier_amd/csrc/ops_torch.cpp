@@ -118,6 +118,8 @@ void check_capture(const Tensor& first, std::initializer_list<const Tensor*> lea
     }
 }
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
+    for (const Tensor* t : ts)
+        TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), "the fine-tuning operators have no forward-mode derivative");
     if (!at::GradMode::is_enabled()) return false;
     for (const Tensor* t : ts)
         if (t->defined() && t->requires_grad()) return true;
@@ -137,10 +139,12 @@ struct OpNode : Node {
     bool released = false;
 
     // the dropout arguments for the backward pass; `off` keeps their tensor
-    clipvit_dropout_args begin(Tensor& off) {
+    clipvit_dropout_args begin(Tensor& off, const Tensor& dy) {
         TORCH_CHECK(!released, torch::autograd::ERR_BACKWARD_TWICE);
         TORCH_CHECK(!at::GradMode::is_enabled(), "the fine-tuning operators are differentiable once: their backward takes no create_graph");
         off = offset_dev.unpack();
+        TORCH_CHECK(!off.defined() || !dy.defined() || (off.device() == dy.device() && off.scalar_type() == at::kLong && off.numel() == 1),
+                    "a saved tensor came back with another size, type or device than it was saved with");
         clipvit_dropout_args d = drop;
         d.offset_dev = (const int64_t*)ptr(off);
         return d;
@@ -157,6 +161,18 @@ struct OpNode : Node {
     }
     virtual void release_saved() {}
 };
+// A saved tensor as it was saved: a saved-tensor hook may have given back another layout, and must not another size or type.
+Tensor unpacked(const SavedVariable& v, at::IntArrayRef shape, at::ScalarType type, const Tensor& like) {
+    const Tensor t = v.unpack();
+    TORCH_CHECK(t.defined() && t.sizes() == shape && t.scalar_type() == type && t.device() == like.device(),
+                "a saved tensor came back with another size, type or device than it was saved with");
+    return t;
+}
+int64_t rows_in(at::IntArrayRef shape) {
+    int64_t m = 1;
+    for (size_t i = 0; i + 1 < shape.size(); ++i) m *= shape[i];
+    return m;
+}
 template <class N, class... Inputs>
 std::shared_ptr<N> new_node(const Inputs&... inputs) {
     std::shared_ptr<N> node(new N(), torch::autograd::deleteNode);
@@ -201,6 +217,7 @@ LinearOut linear_forward(at::IntArrayRef shape, const Tensor& x2, const Tensor& 
 
 struct LinearNode : OpNode {
     SavedVariable x, w, slope;
+    bool has_slope = false;
     std::vector<int64_t> x_shape;
     at::ScalarType bias_type = at::ScalarType::Undefined;  // (none)
 
@@ -213,16 +230,19 @@ struct LinearNode : OpNode {
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
         Tensor offset_keep;
-        const clipvit_dropout_args drop_args = begin(offset_keep);
-        const Tensor &dy = grads[0], x2 = x.unpack(), w2 = w.unpack(), slope2 = slope.unpack();
+        const clipvit_dropout_args drop_args = begin(offset_keep, grads[0]);
+        const Tensor& dy = grads[0];
         if (!dy.defined()) return variable_list(4);
+        const int64_t m = rows_in(x_shape), k = x_shape.back(), n = dy.size(-1);
+        const at::ScalarType type = dy.scalar_type();
+        const Tensor x2 = panel_of(unpacked(x, {m, k}, type, dy)), w2 = panel_of(unpacked(w, {n, k}, type, dy));
+        const Tensor slope2 = has_slope ? unpacked(slope, {m, n}, at::kShort, dy).contiguous() : Tensor();
         const bool nx = task_should_compute_output(0), nw = task_should_compute_output(1);
         const bool nb = bias_type != at::ScalarType::Undefined && task_should_compute_output(2), nr = task_should_compute_output(3);
         Tensor dx, dw, db;
         if (nx || nw || nb) {
             const On on(x2);
             const Tensor dy2 = rows_of(dy, true);
-            const int64_t m = x2.size(0), k = x2.size(1), n = w2.size(0);
             if (nx) dx = at::empty(x_shape, x2.options());
             if (nw) dw = at::empty({n, k}, x2.options());
             if (nb) db = at::empty({n}, x2.options().dtype(bias_type));
@@ -277,6 +297,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const std::optional<Tensor>
         node->x = SavedVariable(x2, false);
         node->w = SavedVariable(w, false);
         node->slope = SavedVariable(o.slope, false);
+        node->has_slope = o.slope.defined();
         node->x_shape = x.sizes().vec();
         if (bias.defined()) node->bias_type = bias.scalar_type();
         torch::autograd::set_history(o.y, node);
@@ -300,7 +321,7 @@ struct DropoutNode : OpNode {
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
         Tensor offset_keep;
-        const clipvit_dropout_args drop_args = begin(offset_keep);
+        const clipvit_dropout_args drop_args = begin(offset_keep, grads[0]);
         const Tensor& dy = grads[0];
         if (!dy.defined()) return variable_list(2);
         return {task_should_compute_output(0) ? dropout_call(dy, Tensor(), drop_args) : Tensor(), task_should_compute_output(1) ? dy : Tensor()};
@@ -363,6 +384,7 @@ LoraOut lora_forward(at::IntArrayRef shape, const Tensor& x2, const Tensor& w, c
 struct LoraNode : OpNode {
     SavedVariable x, w, a_factor, b_factor, u;
     std::vector<int64_t> x_shape;
+    int64_t rank = 0;
     at::ScalarType bias_type = at::ScalarType::Undefined;  // (none)
     float scaling = 1;
 
@@ -373,12 +395,16 @@ struct LoraNode : OpNode {
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
         Tensor offset_keep;
-        const clipvit_dropout_args drop_args = begin(offset_keep);
-        const Tensor x2 = x.unpack(), w2 = w.unpack(), A = a_factor.unpack(), B = b_factor.unpack(), u2 = u.unpack();
-        if (!grads[0].defined()) return variable_list(5);
+        const clipvit_dropout_args drop_args = begin(offset_keep, grads[0]);
+        const Tensor& dy = grads[0];
+        if (!dy.defined()) return variable_list(5);
+        const int64_t m = rows_in(x_shape), k = x_shape.back(), n = dy.size(-1), r = rank;
+        const at::ScalarType type = dy.scalar_type();
+        const Tensor x2 = rows_of(unpacked(x, {m, k}, type, dy), true), w2 = panel_of(unpacked(w, {n, k}, type, dy));
+        const Tensor A = unpacked(a_factor, {k, r}, type, dy), B = unpacked(b_factor, {r, n}, type, dy);
+        const Tensor u2 = unpacked(u, {m, (r + 31) / 32 * 32}, type, dy).contiguous();
         const On on(x2);
-        const Tensor dy2 = rows_of(grads[0], true);
-        const int64_t m = x2.size(0), k = x2.size(1), n = w2.size(0), r = A.size(1);
+        const Tensor dy2 = rows_of(dy, true);
         const bool nb = bias_type != at::ScalarType::Undefined && task_should_compute_output(4);
         Tensor dx, dw, dA, dB, db;
         if (task_should_compute_output(0)) dx = at::empty(x_shape, x2.options());
@@ -445,6 +471,7 @@ Tensor lora_linear(const Tensor& x, const Tensor& weight, const Tensor& A, const
         node->u = SavedVariable(o.u, false);
         node->x_shape = x.sizes().vec();
         if (bias.defined()) node->bias_type = bias.scalar_type();
+        node->rank = A.size(1);
         node->scaling = (float)scaling;
         torch::autograd::set_history(o.y, node);
     }

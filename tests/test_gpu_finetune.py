@@ -500,3 +500,35 @@ def test_two_threads(gpu):
     for t in threads:
         t.join()
     assert all(torch.equal(g, want) for g in got)
+
+
+def test_forward_mode_is_refused(gpu):
+    import torch.autograd.forward_ad as fwd
+    x, w = rand(4, 8, seed=1).to(gpu), rand(6, 8, seed=2).to(gpu)
+    with fwd.dual_level():
+        d = fwd.make_dual(x, torch.ones_like(x))
+        for call in (lambda: ops.linear(d, w), lambda: ops.dropout(d, 0.5, seed=1), lambda: ops.lora_linear(x, w, d.t()[:, :2], w.t()[:2, :6])):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+
+
+def test_saved_tensor_hooks(gpu):
+    x, w, A, B = (rand(*s, seed=i).to(gpu).requires_grad_() for i, s in enumerate(((40, 24), (16, 24), (24, 4), (4, 16))))
+    dy = rand(40, 16, seed=9).to(gpu)
+
+    def step():
+        y = ops.linear(x, w, activation="silu", dropout_p=0.2, seed=1) + ops.lora_linear(x, w, A, B, scaling=0.5, dropout_p=0.2, seed=2)
+        return torch.autograd.grad(y, (x, w, A, B), dy)
+
+    want = step()
+    with torch.autograd.graph.save_on_cpu():
+        assert all(torch.equal(a, b) for a, b in zip(step(), want))
+    # another layout may change the order of a sum, so the last bit of an output or of du (eps / 2 of a value each, twice)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.t().contiguous(), lambda t: t.t()):
+        for a, b in zip(step(), want):
+            assert float((a - b).float().norm()) <= 2 * torch.finfo(BF).eps * float(b.float().norm())
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t[:1]), pytest.raises(RuntimeError, match="saved tensor came back"):
+        step()
+    offset = torch.ones(1, dtype=torch.int64, device=gpu)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.cpu()), pytest.raises(RuntimeError, match="saved tensor came back"):
+        torch.autograd.grad(ops.dropout(x, 0.5, seed=1, offset=offset), x, rand(40, 24).to(gpu))
