@@ -118,6 +118,17 @@ __device__ __forceinline__ void stage_low(const u16* low, int rank, int i0, int 
     }
 }
 
+// 32 ranks (from 32 j on) of rows i0 .. i0 + 255 of a low-rank factor: 64 bytes a row, its four chunks swizzled by the row
+__device__ __forceinline__ void stage_low32(const u16* low, int rank, int i0, int count, int j, int w, int lane, unsigned char* dst) {
+    const int valid = min(count - i0, 256);
+    const i32x4_t rs = buf_rsrc(low + (int64_t)i0 * rank, (unsigned)valid * (unsigned)rank * 2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int piece = w * 4 + i, row = piece * 16 + (lane >> 2), chunk = (lane & 3) ^ ((row >> 2) & 3);
+        blds16(rs, row < valid ? (unsigned)(row * rank + j * 32 + chunk * 8) * 2 : OOB, 0, dst + piece * 1024);
+    }
+}
+
 // Fragment reads of FR (1, 2 or 4) 16-row fragments x 64 k from position i0 of a panel. Each asm block ends with its own
 // wait (hipcc does not see these reads, and a plain LDS read would make it drain the LDS-DMA loads in flight).
 template <typename T, bool KC, int R, int FR>
@@ -223,14 +234,14 @@ __device__ __forceinline__ void bar() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// one 64-deep k-tile of the low-rank term from its fragments; masked, in the accumulators' layout, where a lane's four
+// KS times 32 ranks of the low-rank term from their fragments; masked, in the accumulators' layout, where a lane's four
 // columns are one counter of the generator (a fragment at a time: the scheduler would otherwise spill)
-template <typename T, int FR, int FB, int J0, int FM>
-__device__ __forceinline__ void low_acc(const Epilogue& e, const uint2& off, const typename T::vec8 (&a)[2][FR], const typename T::vec8 (&b)[2][FB],
+template <typename T, int FR, int FB, int J0, int KS, int FM>
+__device__ __forceinline__ void low_acc(const Epilogue& e, const uint2& off, const typename T::vec8 (&a)[KS][FR], const typename T::vec8 (&b)[KS][FB],
                                         f32x4 (&acc)[FM][4], int i0, int m, int n) {
     if (!e.low_mask) {
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
             for (int i = 0; i < FR; ++i)
 #pragma unroll
@@ -242,7 +253,7 @@ __device__ __forceinline__ void low_acc(const Epilogue& e, const uint2& off, con
 #pragma unroll
         for (int j = 0; j < FB; ++j) {
             f32x4 t = T::mfma16(b[0][j], a[0][i], f32x4{0.f, 0.f, 0.f, 0.f});
-            t = T::mfma16(b[1][j], a[1][i], t);
+            if constexpr (KS == 2) t = T::mfma16(b[1][j], a[1][i], t);
             float t0 = t[0], t1 = t[1], t2 = t[2], t3 = t[3];
             drop4(e.drop, off, e.m_base + m + 16 * i, n + 16 * (J0 + j), 1.0f, t0, t1, t2, t3);
             acc[i0 + i][J0 + j] += f32x4{t0, t1, t2, t3};
@@ -443,8 +454,8 @@ __global__ __launch_bounds__(512, 1) void matmul256_kernel(Matmul a, float* part
     using PA1 = Panel<AK, 128, 4, Half<1, 64>>;
     using PB0 = Panel<BK, 128, 4, Half<0, 32>>;
     using PB1 = Panel<BK, 128, 4, Half<1, 32>>;
-    constexpr int HALF = 16384, ST = 32768, B_OFF = 65536;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[131072];
+    constexpr int HALF = 16384, ST = 32768, B_OFF = 65536, LOW = 131072;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[163840];  // two k-tiles, 32 ranks of the low-rank factors
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave >> 2, wn = wave & 3;
@@ -487,6 +498,12 @@ __global__ __launch_bounds__(512, 1) void matmul256_kernel(Matmul a, float* part
     };
     using H0 = std::integral_constant<int, 0>;
     using H1 = std::integral_constant<int, 1>;
+    const bool low = a.e.R > 0 && blockIdx.y == 0;
+    auto low_stage = [&](int j) {
+        if (wm == 0) stage_low32(a.e.lu, a.e.R, m0, a.M, j, wn, lane, smem + LOW);
+        else stage_low32(a.e.lv, a.e.R, n0, a.N, j, wn, lane, smem + LOW + 16384);
+    };
+    if (low) low_stage(0);  // (the oldest loads: the counted waits below include them)
     if (nk > 0) {
         if (wm == 0) {
             PA0 p0;
@@ -545,36 +562,36 @@ __global__ __launch_bounds__(512, 1) void matmul256_kernel(Matmul a, float* part
         vm_wait<0>();  // no load into LDS outlives the k loop: the epilogue takes the stages over
         bar();
     }
-    if (a.e.R > 0 && blockIdx.y == 0) {
-        // rank-R term, 64 ranks at a time: the factors' rows staged like row panels, whatever the operands are. (Its
-        // fragments straight from global memory cost 14 us a round of tiles; as further k-tiles of the loop above, their
-        // branch slowed the loop by a quarter.)
+    if (low) {
+        // rank-R term, 32 ranks at a time, the first ones staged before the k loop. (All staged after it like k-tiles, 64 a
+        // step: training step of 18464 x 1024 x 4096, rank 16, 492 against 481 us on one card. Fragments straight from global
+        // memory cost 14 us a round of tiles; as further k-tiles of the loop, their branch slowed the loop by a quarter.)
         const uint2 off = a.e.drop.on ? drop_offset(a.e.drop) : make_uint2(0, 0);
-        Frags<T, true, 128, 4> la;
-        Frags<T, true, 128, 2> lb;
-        la.init(lds, wm * 64, lane);
-        lb.init(lds + B_OFF, wn * 32, lane);
-        const int m = m0 + wm * 128 + (lane & 15), n = n0 + wn * 64 + 4 * (lane >> 4);
+        const int li = lane & 15, g = lane >> 4;
+        const unsigned char* pa = smem + LOW + (wm * 128 + li) * 64 + ((g ^ (li >> 2)) << 4);
+        const unsigned char* pb = smem + LOW + 16384 + (wn * 64 + li) * 64 + ((g ^ (li >> 2)) << 4);
+        vm_wait<0>();
+        bar();
 #pragma unroll 1
-        for (int j = 0; j * 64 < a.e.R; ++j) {
-            if (wm == 0) {
-                stage_low<128, 4, Half<0, 64>>(a.e.lu, a.e.R, m0, a.M, j, wn, lane, smem);
-                stage_low<128, 4, Half<1, 64>>(a.e.lu, a.e.R, m0, a.M, j, wn, lane, smem + HALF);
-            } else {
-                stage_low<128, 4, Half<0, 32>>(a.e.lv, a.e.R, n0, a.N, j, wn, lane, smem + B_OFF);
-                stage_low<128, 4, Half<1, 32>>(a.e.lv, a.e.R, n0, a.N, j, wn, lane, smem + B_OFF + HALF);
+        for (int j = 0; j * 32 < a.e.R; ++j) {
+            if (j) {
+                bar();  // every wave has read the ranks before
+                low_stage(j);
+                vm_wait<0>();
+                bar();
             }
-            vm_wait<0>();
-            bar();
-            lb.read(b0, 0);
-            lb.read(b1, HALF);
-            la.read(af, 0);
-            low_acc<T, 4, 2, 0>(a.e, off, af, b0, acc, 0, m, n);
-            low_acc<T, 4, 2, 2>(a.e, off, af, b1, acc, 0, m, n);
-            la.read(af, HALF);
-            low_acc<T, 4, 2, 0>(a.e, off, af, b0, acc, 4, m + 64, n);
-            low_acc<T, 4, 2, 2>(a.e, off, af, b1, acc, 4, m + 64, n);
-            bar();
+            asm volatile("" ::: "memory");
+            vec8 u[1][4], v[1][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[0][i] = *(const vec8*)(pb + i * 1024);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[0][i] = *(const vec8*)(pa + i * 1024);
+            low_acc<T, 4, 4, 0>(a.e, off, u, v, acc, 0, m0 + wm * 128 + li, n0 + wn * 64 + 4 * g);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[0][i] = *(const vec8*)(pa + 4096 + i * 1024);
+            low_acc<T, 4, 4, 0>(a.e, off, u, v, acc, 4, m0 + wm * 128 + 64 + li, n0 + wn * 64 + 4 * g);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
     }
     store_tile<T, 8>(a, acc, m0 + wm * 128, n0 + wn * 64, (float*)smem + wave * 4096,
