@@ -282,6 +282,12 @@ def test_lora_linear(gpu, dtype, p, m, k, n, r):
         assert torch.equal(ops.lora_linear(*leaves, **kw), y)
 
 
+@pytest.mark.parametrize("m, k, n, r, dtype", [(4091, 64, 4088, 33, BF), (4091, 4088, 64, 70, HF), (4091, 4088, 64, 16, BF), (4360, 64, 4096, 96, HF)])
+def test_lora_linear_wide_tiles(gpu, m, k, n, r, dtype):
+    """Output (and dx) of 16 x 16 tiles of 256, ragged, with one to three steps of 32 ranks; 4360 rows are a round and a rest."""
+    test_lora_linear(gpu, dtype, 0.25, m, k, n, r)
+
+
 @pytest.mark.parametrize("r,k", [(4, 64), (4, 61), (20, 128)])
 def test_lora_infinity_stays_an_infinity(gpu, r, k):
     """Positive operands, one infinite element: the row is +inf as in the formula (a padded rank times it would be NaN),
