@@ -1,6 +1,8 @@
 // Shared pieces of the fine-tuning operators (matmul.hip, finetune.hip): the counter-based dropout
 // generator, the activations with their derivatives and the epilogue of a matrix product.
 #pragma once
+#include <type_traits>
+
 #include "common.h"
 
 namespace clipvit {
@@ -66,12 +68,14 @@ __device__ __forceinline__ float act_one(float beta, float z, float& slope) {
         if (SLOPE) slope = s * (1.0f - 0.69314718055994531f * beta * zc * (1.0f - s));
         return z * s;
     } else if constexpr (ACT == ACT_GELU) {
-        // Phi(-|z|) = t (a1 + t (a2 + ..)) e^(-z^2 / 2) / 2, t = 1 / (1 + p |z| / sqrt 2): Abramowitz and Stegun
-        // 7.1.26, off by at most 7.5e-8; it shares the exponential with the derivative (erff and its own exponential:
-        // 70 instructions an element against 30, 4928 x 512 x 2048 with the derivative 52 us against 38)
-        const float az = fabsf(z), t = __builtin_amdgcn_rcpf(1.0f + 0.23164189f * az);
+        // Phi(-|z|) = t P(t) e^(-z^2 / 2), t = 1 / (1 + 0.29 |z|), P of degree 5 fitted for |z| <= 14 (minimax, linear
+        // programme) to 7.1e-8 absolute and 2^-13.5 relative: the tail has to keep its leading digits for bf16, which holds
+        // it. Evaluated in fp32 it is off by at most 2.3e-7 near 0 and 2^-13.4 relative. It shares the exponential with the
+        // derivative (erff and its own exponential: 70 instructions an element against 30, 4928 x 512 x 2048 with the
+        // derivative 52 us against 38).
+        const float az = fabsf(z), t = __builtin_amdgcn_rcpf(1.0f + 0.29f * az);
         const float e = __builtin_amdgcn_exp2f(-0.72134752044448170f * az * az);
-        const float q = t * (0.127414796f + t * (-0.142248368f + t * (0.710706871f + t * (-0.726576014f + t * 0.530702714f)))) * e;
+        const float q = t * (0.116854535f + t * (0.100881662f + t * (0.178990770f + t * (-0.0923373715f + t * (0.284243027f + t * -0.0886325613f))))) * e;
         const float c = z < 0.f ? q : 1.0f - q;
         if (SLOPE) slope = c + 0.39894228040143268f * zc * e;
         return z * c;
@@ -102,15 +106,36 @@ __device__ __forceinline__ void act_cols(int act, float (&v)[C], float (&g)[C]) 
         for (int j = 0; j < C; ++j) v[j] = act_one<SLOPE, ACT_RELU>(0.f, v[j], g[j]);
     }
 }
-// The derivative as the forward saves it: 16-bit fixed point, steps of 2^-14. All of these derivatives
-// lie in (-0.13, 1.13), so the rounding is at most 2^-15 absolute, 16 times below the half step of an fp16
-// value near 1 (2^-12 relative) that dz is rounded to afterwards; the code -32768 stands for NaN.
-__device__ __forceinline__ short slope_encode(float g) {
-    return g != g ? (short)-32768 : (short)__float2int_rn(fminf(fmaxf(g, -1.9f), 1.9f) * 16384.f);
-}
-__device__ __forceinline__ float slope_decode(short q) {
-    return q == -32768 ? __builtin_nanf("") : (float)q * (1.0f / 16384.f);
-}
+// The derivative as the forward saves it: sign and 15 bits of magnitude, all of these derivatives lying in (-0.13, 1.13).
+// From 2^(M - 14) up the magnitude is fixed point in steps of 2^-14; below it is a float of M mantissa bits, whose steps
+// join those: off by at most 2^-15 absolute and 2^-(M + 1) relative. bf16 operands: M = 7, half a bf16 step (2^-8), down to
+// 2^-118; fp16 operands: M = 9, half of 2^-9, down to 2^-33, under what an fp16 dz resolves (2^-24 for |dy| up to 2^8); less
+// is 0. (Fixed point alone loses the derivative of a saturated unit altogether: quick_gelu is 9 % off at z = -6 and 0 past
+// -7.6. A plain 16-bit float is as far off near 1 as dz's own rounding is.) 0x7fff stands for NaN.
+template <typename T>
+struct SlopeCode {
+    static constexpr int M = std::is_same<T, BF16>::value ? 7 : 9, LOW = std::is_same<T, BF16>::value ? -118 : -33;
+    static constexpr unsigned OFF = ((127 + LOW) << M) - 1;          // float bits >> (23 - M) minus this: 1 at 2^LOW
+    static constexpr unsigned JOIN = ((M - 14 - LOW) << M) + 1;      // code of 2^(M - 14)
+    // 512 + magnitude is a float in steps of 2^-14: its bits minus this are the fixed-point part's codes
+    static constexpr unsigned FIXED = 0x44000000u - (JOIN - (1u << M));
+    static_assert(JOIN - (1u << M) + 18678 < 0x7fff, "1.14, more than any magnitude, stays below NaN");
+    static __device__ __forceinline__ short encode(float g) {
+        const unsigned bits = __float_as_uint(g), mag = bits & 0x7fffffffu;
+        const float a = __uint_as_float(mag);
+        const unsigned fixed = __float_as_uint(a + 512.f) - FIXED;
+        const unsigned tail = __builtin_elementwise_sub_sat(mag, (OFF << (23 - M)) - (1u << (22 - M))) >> (23 - M);
+        const unsigned m = min(a < 1.0f / (1 << (14 - M)) ? tail : fixed, 0x7fffu);
+        return (short)(m | (bits >> 16 & 0x8000u));
+    }
+    static __device__ __forceinline__ float decode(short q) {
+        const unsigned m = q & 0x7fff;
+        const float tail = m ? __uint_as_float((m + OFF) << (23 - M)) : 0.f;
+        const float fixed = m == 0x7fff ? __builtin_nanf("") : __uint_as_float(m + FIXED) - 512.f;
+        const float a = m < JOIN ? tail : fixed;
+        return __uint_as_float(__float_as_uint(a) | ((unsigned)q & 0x8000u) << 16);
+    }
+};
 
 // ---- epilogue of C = A B^T ----
 //   z = acc + bias + low-rank term;  y = residual + dropout(act(z));  slope = act'(z)
@@ -157,7 +182,7 @@ __device__ __forceinline__ void epilogue_cols(const Epilogue& e, const uint2& of
             short q[C];
             act_cols<true, C>(e.act, v, gr);
 #pragma unroll
-            for (int j = 0; j < C; ++j) q[j] = slope_encode(gr[j]);
+            for (int j = 0; j < C; ++j) q[j] = SlopeCode<T>::encode(gr[j]);
             short* s = e.slope + (int64_t)m * e.N + n;
             if (whole) {
                 if constexpr (C % 8 == 0) {

@@ -24,11 +24,13 @@ struct F32T {
 };
 struct BF16T {
     typedef u16 store;
+    typedef BF16 half;
     static __device__ __forceinline__ float to_f32(u16 v) { return BF16::to_f32(v); }
     static __device__ __forceinline__ u16 from_f32(float v) { return BF16::from_f32(v); }
 };
 struct F16T {
     typedef u16 store;
+    typedef F16 half;
     static __device__ __forceinline__ float to_f32(u16 v) { return F16::to_f32(v); }
     static __device__ __forceinline__ u16 from_f32(float v) { return F16::from_f32(v); }
 };
@@ -189,7 +191,7 @@ __global__ __launch_bounds__(256) void dz_kernel(DzArgs a) {
                     for (int j = 0; j < 8; ++j) t[j] = j < nc ? q[j] : (short)0;
                 }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] *= slope_decode(t[j]);
+                for (int j = 0; j < 8; ++j) v[j] *= SlopeCode<typename E::half>::decode(t[j]);
             }
             if (a.dz) store_cols<E, 8>((S*)a.dz + m * a.lddz + c, nc, a.vec, v);
 #pragma unroll

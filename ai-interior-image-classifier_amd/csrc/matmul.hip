@@ -326,7 +326,7 @@ __device__ __forceinline__ void store_tile(const Matmul& a, f32x4 (&acc)[FM][4],
                         act_cols<true, 8>(e.act, v, gr);
                         short q[8];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) q[j] = slope_encode(gr[j]);
+                        for (int j = 0; j < 8; ++j) q[j] = SlopeCode<T>::encode(gr[j]);
                         u32x4 w;
                         __builtin_memcpy(&w, q, 16);
                         if (e.nt) __builtin_nontemporal_store(w, (u32x4*)sl);

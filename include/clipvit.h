@@ -272,7 +272,8 @@ typedef enum {
 /* y[m, n] = residual[m, n] + dropout(act(z))[m, n],  z = sum_k x[m, k] w[n, k] + bias[n].
  * x [M, K] and w [N, K] are views with two strides, one of them 1; the other is below 2^22 and at least the row's
  * length. y and residual have unit column stride. slope (or NULL, with an activation): act'(z) as [M, N] contiguous
- * 16-bit fixed point, q / 2^14 (-32768 = NaN), what the gradient takes. Rows of any length, stride and alignment
+ * 16-bit codes, what the gradient of the same dtype takes: off by at most 2^-15 and, relative, 2^-8 (BF16, down to 2^-118)
+ * or 2^-10 (F16, down to 2^-33; less is 0). Rows of any length, stride and alignment
  * are taken; those that 16-byte loads cannot address are copied into the workspace first. y must not overlap an
  * input other than an identical residual. */
 typedef struct {
@@ -301,7 +302,7 @@ int clipvit_linear(void* stream, const clipvit_linear_args* args, void* workspac
 
 /* Gradients of clipvit_linear, each output NULL or wanted: dz = dropout(dy) slope (slope NULL: no activation);
  * dx [M, K] = dz w, dw [N, K] = dz^T x (contiguous, of dtype; dz is rounded to dtype for them when there is a slope
- * or a dropout), db [N] = column sums of the unrounded dz. The residual's gradient is dy itself. dy [M, N] has unit
+ * or a dropout), db [N] = column sums of dz before that rounding. The residual's gradient is dy itself. dy [M, N] has unit
  * column stride. Every sum is taken in a fixed order. */
 typedef struct {
     int dtype;
