@@ -830,7 +830,7 @@ int lora_grad_of(const clipvit_lora_grad_args* a, LoraGrad& g, Arena& ws) {
     if ((g.want_dx && a->N && !a->w) || (g.want_dx && !a->a) || (g.want_du && a->N && !a->b) || ((g.want_dw || a->da) && a->M && a->K && !a->x) ||
         (a->db_factor && a->M && (!a->u || !aligned16(a->u))))
         FT_FAIL(CLIPVIT_E_INVALID, "lora_linear_grad: null or misaligned operand");
-    if (a->M > 1 && ((a->N && (a->dy_stride < a->N || a->dy_stride >= MATMUL_MAX_LD)) || a->x_stride < a->K))
+    if (a->M > 1 && ((a->N && (a->dy_stride < a->N || a->dy_stride >= MATMUL_MAX_LD)) || ((g.want_dw || a->da) && a->x_stride < a->K)))
         FT_FAIL(CLIPVIT_E_INVALID, "lora_linear_grad: row stride");
     const Dropout none{};
     if (g.want_du) {

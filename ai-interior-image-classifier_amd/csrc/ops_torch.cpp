@@ -46,6 +46,9 @@ void check(int rc) {
 
 int type_of(at::ScalarType t) { return t == at::kFloat ? CLIPVIT_F32 : t == at::kBFloat16 ? CLIPVIT_BF16 : CLIPVIT_F16; }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+void set_strides(int64_t (&to)[2], const Tensor& t) {
+    for (int i = 0; i < 2; ++i) to[i] = t.defined() ? t.stride(i) : 0;
+}
 
 constexpr int64_t MAX_LD = 1 << 22;
 
@@ -216,7 +219,7 @@ LinearOut linear_forward(at::IntArrayRef shape, const Tensor& x2, const Tensor& 
 }
 
 struct LinearNode : OpNode {
-    SavedVariable x, w, slope;
+    SavedVariable x, w, slope;  // x where the weight's gradient reads it, w where x's does
     bool has_slope = false;
     std::vector<int64_t> x_shape;
     at::ScalarType bias_type = at::ScalarType::Undefined;  // (none)
@@ -235,19 +238,19 @@ struct LinearNode : OpNode {
         if (!dy.defined()) return variable_list(4);
         const int64_t m = rows_in(x_shape), k = x_shape.back(), n = dy.size(-1);
         const at::ScalarType type = dy.scalar_type();
-        const Tensor x2 = panel_of(unpacked(x, {m, k}, type, dy)), w2 = panel_of(unpacked(w, {n, k}, type, dy));
-        const Tensor slope2 = has_slope ? unpacked(slope, {m, n}, at::kShort, dy).contiguous() : Tensor();
         const bool nx = task_should_compute_output(0), nw = task_should_compute_output(1);
         const bool nb = bias_type != at::ScalarType::Undefined && task_should_compute_output(2), nr = task_should_compute_output(3);
+        const Tensor x2 = nw ? panel_of(unpacked(x, {m, k}, type, dy)) : Tensor(), w2 = nx ? panel_of(unpacked(w, {n, k}, type, dy)) : Tensor();
+        const Tensor slope2 = has_slope && (nx || nw || nb) ? unpacked(slope, {m, n}, at::kShort, dy).contiguous() : Tensor();
         Tensor dx, dw, db;
         if (nx || nw || nb) {
-            const On on(x2);
+            const On on(dy);
             const Tensor dy2 = rows_of(dy, true);
-            if (nx) dx = at::empty(x_shape, x2.options());
-            if (nw) dw = at::empty({n, k}, x2.options());
-            if (nb) db = at::empty({n}, x2.options().dtype(bias_type));
+            if (nx) dx = at::empty(x_shape, dy.options());
+            if (nw) dw = at::empty({n, k}, dy.options());
+            if (nb) db = at::empty({n}, dy.options().dtype(bias_type));
             clipvit_linear_grad_args a{};
-            a.dtype = type_of(x2.scalar_type());
+            a.dtype = type_of(type);
             a.bias_dtype = nb ? type_of(bias_type) : a.dtype;
             a.M = m;
             a.N = n;
@@ -255,17 +258,15 @@ struct LinearNode : OpNode {
             a.dy = ptr(dy2);
             a.dy_stride = dy2.stride(0);
             a.x = ptr(x2);
-            a.x_stride[0] = x2.stride(0);
-            a.x_stride[1] = x2.stride(1);
+            set_strides(a.x_stride, x2);
             a.w = ptr(w2);
-            a.w_stride[0] = w2.stride(0);
-            a.w_stride[1] = w2.stride(1);
+            set_strides(a.w_stride, w2);
             a.slope = (const int16_t*)ptr(slope2);
             a.dx = ptr(dx);
             a.dw = ptr(dw);
             a.db = ptr(db);
             a.dropout = drop_args;
-            const Workspace ws(api.linear_grad_workspace, a, x2);
+            const Workspace ws(api.linear_grad_workspace, a, dy);
             check(api.linear_grad(on.stream, &a, ws.p, ws.bytes));
         }
         return {dx, dw, db, nr ? dy : Tensor()};
@@ -288,14 +289,14 @@ Tensor linear(const Tensor& x, const Tensor& weight, const std::optional<Tensor>
         w = panel_of(weight);
         if (residual.defined()) res2 = rows_of(residual, false);
     }
-    const bool slope = grad && (x.requires_grad() || weight.requires_grad() || (bias.defined() && bias.requires_grad()));
+    const bool product = grad && (x.requires_grad() || weight.requires_grad() || (bias.defined() && bias.requires_grad()));  // (not the residual alone)
     const auto drop = drop_of(p, seed, offset, off);
-    const LinearOut o = linear_forward(shape_with(x, w.size(0)), x2, w, bias, res2, (int)act, drop, slope);
+    const LinearOut o = linear_forward(shape_with(x, w.size(0)), x2, w, bias, res2, (int)act, drop, product);
     if (grad) {
         const auto node = new_node<LinearNode>(x, weight, bias, residual);
-        node->set_dropout(drop, off);
-        node->x = SavedVariable(x2, false);
-        node->w = SavedVariable(w, false);
+        node->set_dropout(drop, product ? off : Tensor());
+        if (weight.requires_grad()) node->x = SavedVariable(x2, false);
+        if (x.requires_grad()) node->w = SavedVariable(w, false);
         node->slope = SavedVariable(o.slope, false);
         node->has_slope = o.slope.defined();
         node->x_shape = x.sizes().vec();
@@ -336,7 +337,7 @@ Tensor dropout(const Tensor& x, const std::optional<Tensor>& residual_, double p
     const Tensor y = dropout_call(x, residual, drop);
     if (grad) {
         const auto node = new_node<DropoutNode>(x, residual);
-        node->set_dropout(drop, off);
+        node->set_dropout(drop, x.requires_grad() ? off : Tensor());
         torch::autograd::set_history(y, node);
     }
     return y;
@@ -382,7 +383,7 @@ LoraOut lora_forward(at::IntArrayRef shape, const Tensor& x2, const Tensor& w, c
 }
 
 struct LoraNode : OpNode {
-    SavedVariable x, w, a_factor, b_factor, u;
+    SavedVariable x, w, a_factor, b_factor, u;  // each where a wanted gradient reads it
     std::vector<int64_t> x_shape;
     int64_t rank = 0;
     at::ScalarType bias_type = at::ScalarType::Undefined;  // (none)
@@ -400,20 +401,21 @@ struct LoraNode : OpNode {
         if (!dy.defined()) return variable_list(5);
         const int64_t m = rows_in(x_shape), k = x_shape.back(), n = dy.size(-1), r = rank;
         const at::ScalarType type = dy.scalar_type();
-        const Tensor x2 = rows_of(unpacked(x, {m, k}, type, dy), true), w2 = panel_of(unpacked(w, {n, k}, type, dy));
-        const Tensor A = unpacked(a_factor, {k, r}, type, dy), B = unpacked(b_factor, {r, n}, type, dy);
-        const Tensor u2 = unpacked(u, {m, (r + 31) / 32 * 32}, type, dy).contiguous();
-        const On on(x2);
+        const bool nx = task_should_compute_output(0), nw = task_should_compute_output(1), nA = task_should_compute_output(2);
+        const bool nB = task_should_compute_output(3), nb = bias_type != at::ScalarType::Undefined && task_should_compute_output(4);
+        const Tensor x2 = nw || nA ? rows_of(unpacked(x, {m, k}, type, dy), true) : Tensor(), w2 = nx ? panel_of(unpacked(w, {n, k}, type, dy)) : Tensor();
+        const Tensor A = nx ? unpacked(a_factor, {k, r}, type, dy) : Tensor(), B = nx || nA ? unpacked(b_factor, {r, n}, type, dy) : Tensor();
+        const Tensor u2 = nB ? unpacked(u, {m, (r + 31) / 32 * 32}, type, dy).contiguous() : Tensor();
+        const On on(dy);
         const Tensor dy2 = rows_of(dy, true);
-        const bool nb = bias_type != at::ScalarType::Undefined && task_should_compute_output(4);
         Tensor dx, dw, dA, dB, db;
-        if (task_should_compute_output(0)) dx = at::empty(x_shape, x2.options());
-        if (task_should_compute_output(1)) dw = at::empty({n, k}, x2.options());
-        if (task_should_compute_output(2)) dA = at::empty({k, r}, x2.options());
-        if (task_should_compute_output(3)) dB = at::empty({r, n}, x2.options());
-        if (nb) db = at::empty({n}, x2.options().dtype(bias_type));
+        if (nx) dx = at::empty(x_shape, dy.options());
+        if (nw) dw = at::empty({n, k}, dy.options());
+        if (nA) dA = at::empty({k, r}, dy.options());
+        if (nB) dB = at::empty({r, n}, dy.options());
+        if (nb) db = at::empty({n}, dy.options().dtype(bias_type));
         clipvit_lora_grad_args a{};
-        a.dtype = type_of(x2.scalar_type());
+        a.dtype = type_of(type);
         a.bias_dtype = nb ? type_of(bias_type) : a.dtype;
         a.M = m;
         a.N = n;
@@ -422,16 +424,13 @@ struct LoraNode : OpNode {
         a.dy = ptr(dy2);
         a.dy_stride = dy2.stride(0);
         a.x = ptr(x2);
-        a.x_stride = x2.stride(0);
+        a.x_stride = x2.defined() ? x2.stride(0) : 0;
         a.w = ptr(w2);
-        a.w_stride[0] = w2.stride(0);
-        a.w_stride[1] = w2.stride(1);
+        set_strides(a.w_stride, w2);
         a.a = ptr(A);
-        a.a_stride[0] = A.stride(0);
-        a.a_stride[1] = A.stride(1);
+        set_strides(a.a_stride, A);
         a.b = ptr(B);
-        a.b_stride[0] = B.stride(0);
-        a.b_stride[1] = B.stride(1);
+        set_strides(a.b_stride, B);
         a.u = ptr(u2);
         a.dx = ptr(dx);
         a.dw = ptr(dw);
@@ -440,7 +439,7 @@ struct LoraNode : OpNode {
         a.dbias = ptr(db);
         a.scaling = scaling;
         a.dropout = drop_args;
-        const Workspace ws(api.lora_grad_workspace, a, x2);
+        const Workspace ws(api.lora_grad_workspace, a, dy);
         check(api.lora_grad(on.stream, &a, ws.p, ws.bytes));
         return {dx, dw, dA, dB, db};
     }
@@ -463,12 +462,13 @@ Tensor lora_linear(const Tensor& x, const Tensor& weight, const Tensor& A, const
     const LoraOut o = lora_forward(shape_with(x, w.size(0)), x2, w, A, B, bias, scaling, drop);
     if (grad) {
         const auto node = new_node<LoraNode>(x, weight, A, B, bias);
-        node->set_dropout(drop, off);
-        node->x = SavedVariable(x2, false);
-        node->w = SavedVariable(w, false);
-        node->a_factor = SavedVariable(A, false);
-        node->b_factor = SavedVariable(B, false);
-        node->u = SavedVariable(o.u, false);
+        const bool gx = x.requires_grad(), gA = A.requires_grad();
+        node->set_dropout(drop, gx || gA ? off : Tensor());  // (dB's mask is in u)
+        if (weight.requires_grad() || gA) node->x = SavedVariable(x2, false);
+        if (gx) node->w = SavedVariable(w, false);
+        if (gx) node->a_factor = SavedVariable(A, false);
+        if (gx || gA) node->b_factor = SavedVariable(B, false);
+        if (B.requires_grad()) node->u = SavedVariable(o.u, false);
         node->x_shape = x.sizes().vec();
         if (bias.defined()) node->bias_type = bias.scalar_type();
         node->rank = A.size(1);

@@ -16,13 +16,15 @@ Matrix operands are bf16 or fp16 (one type per call), accumulated in fp32 and ro
 a gradient that passes an activation or a dropout rounds dz to the operands' type before its products, as
 the MFMA takes it. ``offset`` is an int, or a one-element int64 device tensor that the kernels read when they
 run: under a captured graph, change it between replays and every replay draws its own mask. It must not
-change between a forward and its backward (autograd raises if it does). ``seed`` and ``offset`` together
+change between a forward and a backward that draws the mask again (autograd raises if it does). ``seed`` and ``offset`` together
 name the mask: calls that share both (and the row count) share their masks.
 
 Every call runs on the current stream of the tensors' device and allocates its output and workspace from torch's
 caching allocator. There is no CPU fallback: CPU tensors raise ``ClipVitError``. A backward may be captured
 into a graph through ``torch.autograd.grad`` after the usual warm-up on a side stream, once no eager autograd graph of
-the same leaves is alive (a capture that finds one raises). They are differentiable once (no ``create_graph``). Matrices of more than one row hold fewer than 2^22 columns.
+the same leaves is alive (a capture that finds one raises). They are differentiable once (no ``create_graph``), and
+keep for the backward pass only what the wanted gradients read: a frozen weight's x, or a frozen x's weight, may change
+or be freed after the forward. Matrices of more than one row hold fewer than 2^22 columns.
 """
 from __future__ import annotations
 

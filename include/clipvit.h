@@ -303,7 +303,7 @@ int clipvit_linear(void* stream, const clipvit_linear_args* args, void* workspac
 /* Gradients of clipvit_linear, each output NULL or wanted: dz = dropout(dy) slope (slope NULL: no activation);
  * dx [M, K] = dz w, dw [N, K] = dz^T x (contiguous, of dtype; dz is rounded to dtype for them when there is a slope
  * or a dropout), db [N] = column sums of dz before that rounding. The residual's gradient is dy itself. dy [M, N] has unit
- * column stride. Every sum is taken in a fixed order. */
+ * column stride. An operand that no wanted output reads (x: dw, w: dx) may be NULL. Every sum is taken in a fixed order. */
 typedef struct {
     int dtype;
     int bias_dtype; /* of db: CLIPVIT_F32 or dtype */
@@ -357,7 +357,8 @@ int clipvit_lora_linear(void* stream, const clipvit_lora_args* args, void* works
 
 /* Its gradients, each output NULL or wanted, contiguous: dx [M, K], dw [N, K], da [K, rank], db_factor [rank, N] of
  * dtype and dbias [N]. du = scaling / (1 - p) dy b^T is rounded to dtype; dx = dy w + mask (du a^T), da = (mask x)^T du,
- * db_factor = u^T dy, dw = dy^T x, dbias = column sums of dy, in fixed orders. */
+ * db_factor = u^T dy, dw = dy^T x, dbias = column sums of dy, in fixed orders. An operand that no wanted output reads
+ * (x: dw, da; w and a: dx; b: dx, da; u: db_factor) may be NULL. */
 typedef struct {
     int dtype;
     int bias_dtype;

@@ -1,0 +1,30 @@
+"""What the fine-tuning operators ask of their callers and of the build, without a GPU."""
+import ctypes
+
+import pytest
+
+from interior_amd import _lib
+from test_finetune import linear_grad_args, lora_grad_args
+
+
+@pytest.mark.parametrize("args", [
+    linear_grad_args(dw=None, x=None, x_row=0, x_col=0), linear_grad_args(dx=None, w=None, w_row=0, w_col=0),
+    linear_grad_args(dx=None, dw=None, x=None, w=None, x_row=0, x_col=0, w_row=0, w_col=0)])
+def test_linear_grad_needs_what_its_outputs_read(args):
+    need = ctypes.c_size_t()
+    assert _lib.lib().clipvit_linear_grad_workspace(ctypes.byref(args), ctypes.byref(need)) == 0
+
+
+NO_X, NO_W = dict(x=None, x_stride=0), dict(w=None, w_row=0, w_col=0)
+NO_A, NO_B, NO_U = dict(a=None, a_row=0, a_col=0), dict(b=None, b_row=0, b_col=0), dict(u=None)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(dw=None, da=None, **NO_X),
+    dict(dx=None, **NO_W, **NO_A),
+    dict(dx=None, da=None, **NO_W, **NO_A, **NO_B),
+    dict(db_factor=None, **NO_U),
+    dict(dx=None, dw=None, da=None, db_factor=None, **NO_X, **NO_W, **NO_A, **NO_B, **NO_U)])
+def test_lora_grad_needs_what_its_outputs_read(kw):
+    need = ctypes.c_size_t()
+    assert _lib.lib().clipvit_lora_linear_grad_workspace(ctypes.byref(lora_grad_args(**kw)), ctypes.byref(need)) == 0
