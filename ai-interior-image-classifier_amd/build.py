@@ -86,7 +86,7 @@ def _build_torch_binding() -> None:
            "-DUSE_ROCM=1", f"-I{INCLUDE}", "-isystem/opt/rocm/include",
            *(f"-isystem{d}" for d in include_paths()), f"-isystem{sysconfig.get_paths()['include']}",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", str(src), "-o", str(tmp),
-           f"-L{Path(torch.__file__).parent / 'lib'}", "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-ldl"]
+           f"-L{Path(torch.__file__).parent / 'lib'}", "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed for {src.name}:\n{r.stdout}\n{r.stderr}")

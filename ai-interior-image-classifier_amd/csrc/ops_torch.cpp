@@ -5,7 +5,6 @@
 // because a node written in Python runs under the interpreter on autograd's own thread: a training step of a small Linear
 // took 130 us of host time that way, most of it handing the interpreter over and waking the threads.
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
-#include <dlfcn.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -108,7 +107,9 @@ clipvit_dropout_args drop_of(double p, uint64_t seed, uint64_t offset, const Ten
 void check_capture(const Tensor& first, std::initializer_list<const Tensor*> leaves) {
     int status = 0;
     const auto current = current_stream(first);
-    if (!api.is_capturing || api.is_capturing(current.stream(), &status) || status == 0) return;
+    const int rc = api.is_capturing(current.stream(), &status);
+    TORCH_CHECK(rc == 0, "whether a graph is capturing the current stream could not be asked (HIP error ", rc, "); a backward pass needs to know");
+    if (status == 0) return;
     const c10::Stream stream = current.unwrap();
     for (const Tensor* t : leaves) {
         if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
@@ -478,9 +479,14 @@ Tensor lora_linear(const Tensor& x, const Tensor& weight, const Tensor& A, const
     return o.y;
 }
 
-// the library's entry points by address (whichever build of it the package loaded) and the package's error class
+// the library's entry points by address (whichever build of it the package loaded), the query of the HIP runtime that it is
+// linked to, and the package's error class
 void set_library(const std::map<std::string, uint64_t>& f, py::object error) {
-    auto get = [&](auto& p, const char* name) { p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(f.at(name)); };
+    auto get = [&](auto& p, const char* name) {
+        const auto at = f.find(name);
+        if (at == f.end() || !at->second) throw std::runtime_error(std::string("the library has no ") + name);
+        p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(at->second);
+    };
     get(api.linear, "clipvit_linear");
     get(api.linear_workspace, "clipvit_linear_workspace");
     get(api.linear_grad, "clipvit_linear_grad");
@@ -491,7 +497,7 @@ void set_library(const std::map<std::string, uint64_t>& f, py::object error) {
     get(api.lora_grad_workspace, "clipvit_lora_linear_grad_workspace");
     get(api.dropout, "clipvit_dropout");
     get(api.last_error, "clipvit_last_error");
-    api.is_capturing = reinterpret_cast<int (*)(void*, int*)>(dlsym(RTLD_DEFAULT, "hipStreamIsCapturing"));
+    get(api.is_capturing, "hipStreamIsCapturing");
     error_class = error.release().ptr();
 }
 

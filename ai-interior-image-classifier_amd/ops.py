@@ -48,12 +48,17 @@ def _binding():
             from . import _ops_torch as m
         except ImportError as e:
             raise _lib.ClipVitError(_lib.E_STATE, f"_ops_torch.so is not built (run __graft_entry__.build()): {e}") from e
-        L = _lib.lib()
-        names = [f"clipvit_{n}{w}" for n in ("linear", "linear_grad", "lora_linear", "lora_linear_grad") for w in ("", "_workspace")]
-        m.set_library({n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in (*names, "clipvit_dropout", "clipvit_last_error")},
-                      _lib.ClipVitError)
+        m.set_library(_entry_points(), _lib.ClipVitError)
         _binding_module = m
     return _binding_module
+
+
+def _entry_points() -> dict[str, int]:
+    """Addresses of what the binding calls: the library's entry points and the capture query of the runtime it is linked to."""
+    L = _lib.lib()
+    names = [f"clipvit_{n}{w}" for n in ("linear", "linear_grad", "lora_linear", "lora_linear_grad") for w in ("", "_workspace")]
+    return {n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value
+            for n in (*names, "clipvit_dropout", "clipvit_last_error", "hipStreamIsCapturing")}
 
 
 # ---------------------------------------------------------------- arguments

@@ -3,7 +3,7 @@ import ctypes
 
 import pytest
 
-from interior_amd import _lib
+from interior_amd import _lib, ops
 from test_finetune import linear_grad_args, lora_grad_args
 
 
@@ -28,3 +28,15 @@ NO_A, NO_B, NO_U = dict(a=None, a_row=0, a_col=0), dict(b=None, b_row=0, b_col=0
 def test_lora_grad_needs_what_its_outputs_read(kw):
     need = ctypes.c_size_t()
     assert _lib.lib().clipvit_lora_linear_grad_workspace(ctypes.byref(lora_grad_args(**kw)), ctypes.byref(need)) == 0
+
+
+@pytest.mark.parametrize("name", ["hipStreamIsCapturing", "clipvit_linear", "clipvit_last_error"])
+def test_binding_refuses_a_library_without_an_entry(name):
+    """A missing entry is an error when the binding is set up, not a check that is silently left out later."""
+    m, table = ops._binding(), ops._entry_points()
+    try:
+        for bad in ({k: v for k, v in table.items() if k != name}, table | {name: 0}):
+            with pytest.raises(RuntimeError, match=name):
+                m.set_library(bad, _lib.ClipVitError)
+    finally:
+        m.set_library(table, _lib.ClipVitError)
