@@ -10,6 +10,8 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/extension.h>
 
+#include <unordered_set>
+
 #include "clipvit.h"
 
 namespace py = pybind11;
@@ -103,22 +105,33 @@ clipvit_dropout_args drop_of(double p, uint64_t seed, uint64_t offset, const Ten
 
 // A leaf's gradient node keeps the stream of the graph that it was made for, for as long as one of its graphs lives. A
 // backward pass captured on another stream would draw that stream into the capture, which ends the process, so such a
-// capture is refused before anything is recorded.
-void check_capture(const Tensor& first, std::initializer_list<const Tensor*> leaves) {
+// capture is refused before anything of the call is recorded. The leaves are the operands and those behind them: the search
+// goes through what was computed on the capturing stream (or on none), and stops at a graph made before, which the capture
+// may treat as its input. (A capture happens once: the search costs an eager call nothing.)
+void check_capture(const Tensor& first, std::initializer_list<const Tensor*> operands) {
     int status = 0;
     const auto current = current_stream(first);
     const int rc = api.is_capturing(current.stream(), &status);
     TORCH_CHECK(rc == 0, "whether a graph is capturing the current stream could not be asked (HIP error ", rc, "); a backward pass needs to know");
     if (status == 0) return;
     const c10::Stream stream = current.unwrap();
-    for (const Tensor* t : leaves) {
-        if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
-        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-        if (!node) continue;
+    std::vector<std::shared_ptr<Node>> todo;
+    std::unordered_set<Node*> seen;
+    const auto visit = [&](std::shared_ptr<Node> node) {
+        if (node && seen.insert(node.get()).second) todo.push_back(std::move(node));
+    };
+    for (const Tensor* t : operands)
+        if (t->defined() && t->requires_grad()) visit(t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn());
+    while (!todo.empty()) {
+        const auto node = std::move(todo.back());
+        todo.pop_back();
         const auto made = node->stream();
-        TORCH_CHECK(!made || *made == stream,
+        const bool elsewhere = made && *made != stream;
+        TORCH_CHECK(!elsewhere || node->num_outputs(),
                     "a graph capture would differentiate a leaf whose earlier autograd graph, made on another stream, is still alive: "
                     "delete that graph's outputs (or run it on the capturing stream) first");
+        if (elsewhere) continue;
+        for (const auto& edge : node->next_edges()) visit(edge.function);
     }
 }
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
