@@ -29,7 +29,7 @@ EXPORTS = (
     "clipvit_encode_text", "clipvit_text_destroy", "clipvit_residual_x24_test", "clipvit_set_tuning",
     "clipvit_gemm_log", "clipvit_linear_workspace", "clipvit_linear", "clipvit_linear_grad_workspace",
     "clipvit_linear_grad", "clipvit_dropout", "clipvit_lora_linear_workspace", "clipvit_lora_linear",
-    "clipvit_lora_linear_grad_workspace", "clipvit_lora_linear_grad",
+    "clipvit_lora_linear_grad_workspace", "clipvit_lora_linear_grad", "clipvit_matmul_plan_test", "clipvit_linear_test",
 )
 
 
@@ -96,6 +96,10 @@ class LoraGradArgs(ctypes.Structure):
                        "a_row:q a_col:q b:p b_row:q b_col:q u:p dx:p dw:p da:p db_factor:p dbias:p scaling:f reserved:f dropout:d")
 
 
+class MatmulPart(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int), ("tile", ctypes.c_int), ("slices", ctypes.c_int), ("kslice", ctypes.c_int)]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -143,6 +147,9 @@ def lib() -> ctypes.CDLL:
                                           ctypes.POINTER(ctypes.c_int32), i]),
             "clipvit_dropout": (i, [vp, i, vp, i64, vp, i64, vp, i64, i64, i64, ctypes.POINTER(DropoutArgs)]),
         }
+        parts = ctypes.POINTER(MatmulPart)
+        sig["clipvit_matmul_plan_test"] = (i, [i64, i64, i64, parts, ctypes.POINTER(i)])
+        sig["clipvit_linear_test"] = (i, [vp, ctypes.POINTER(LinearArgs), parts, i, vp, sz, ctypes.POINTER(sz)])
         for name, args in (("linear", LinearArgs), ("linear_grad", LinearGradArgs), ("lora_linear", LoraArgs),
                            ("lora_linear_grad", LoraGradArgs)):
             sig[f"clipvit_{name}_workspace"] = (i, [ctypes.POINTER(args), ctypes.POINTER(sz)])

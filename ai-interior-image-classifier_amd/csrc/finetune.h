@@ -252,10 +252,27 @@ struct Matmul {
     int M, N, K;
     Epilogue e;
 };
-// bytes of device workspace that launch_matmul needs for this shape, strides and alignment
-size_t matmul_workspace(const Matmul& a);
+// One launch: tile (0 = 64 x 64, 1 = 128 x 128, 2 = 256 x 256), slices of k, and its estimated time.
+struct MatmulPart {
+    int rows, tile, S, kslice;
+    double us;
+};
+struct MatmulPlan {
+    size_t a_bytes, b_bytes, part_bytes;
+    int N4, parts;
+    MatmulPart part[2];  // rows [0, part[0].rows), then the rest
+};
+// the launches for this shape, strides and alignment; `chosen`: with these parts' rows, tiles and slices (rows of the first
+// of two a multiple of 256)
+MatmulPlan matmul_plan(const Matmul& a, const MatmulPart* chosen = nullptr, int parts = 0);
+// bytes of device workspace that launch_matmul needs
+size_t matmul_workspace(const MatmulPlan& p);
+inline size_t matmul_workspace(const Matmul& a) { return matmul_workspace(matmul_plan(a)); }
 // 0, or -1 when the workspace is too small
-int launch_matmul(hipStream_t s, int dtype, const Matmul& a, void* ws, size_t ws_bytes);
+int launch_matmul(hipStream_t s, int dtype, const Matmul& a, const MatmulPlan& p, void* ws, size_t ws_bytes);
+inline int launch_matmul(hipStream_t s, int dtype, const Matmul& a, void* ws, size_t ws_bytes) {
+    return launch_matmul(s, dtype, a, matmul_plan(a), ws, ws_bytes);
+}
 
 // largest row stride (elements) the tiles' 32-bit in-tile offsets allow
 constexpr int64_t MATMUL_MAX_LD = 1 << 22;

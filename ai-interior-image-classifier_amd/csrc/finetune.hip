@@ -910,6 +910,49 @@ int clipvit_linear(void* stream, const clipvit_linear_args* a, void* workspace, 
     });
 }
 
+int clipvit_matmul_plan_test(int64_t M, int64_t N, int64_t K, clipvit_matmul_part* parts, int* count) {
+    return guarded([&]() -> int {
+        if (!parts || !count) FT_FAIL(CLIPVIT_E_INVALID, "null argument");
+        if (const int rc = check_sizes("matmul plan", CLIPVIT_F16, CLIPVIT_F16, M, N, K)) return rc;
+        Matmul m{};
+        m.M = (int)M;
+        m.N = (int)N;
+        m.K = (int)K;
+        const MatmulPlan p = matmul_plan(m);
+        *count = p.parts;
+        for (int i = 0; i < p.parts; ++i) parts[i] = clipvit_matmul_part{p.part[i].rows, 64 << p.part[i].tile, p.part[i].S, p.part[i].kslice};
+        return CLIPVIT_OK;
+    });
+}
+
+int clipvit_linear_test(void* stream, const clipvit_linear_args* a, const clipvit_matmul_part* parts, int count, void* workspace, size_t bytes,
+                        size_t* need) {
+    return guarded([&]() -> int {
+        Matmul m;
+        if (const int rc = linear_of(a, m)) return rc;
+        if (!parts || count < 1 || count > 2 || !m.M || !m.N) FT_FAIL(CLIPVIT_E_INVALID, "linear_test: one or two parts of a product");
+        MatmulPart chosen[2];
+        int64_t rows = 0;
+        for (int i = 0; i < count; ++i) {
+            const clipvit_matmul_part& p = parts[i];
+            if (p.rows < 1 || (p.tile != 64 && p.tile != 128 && p.tile != 256) || p.slices < 1 || p.slices > 64 || (i + 1 < count && p.rows % 256))
+                FT_FAIL(CLIPVIT_E_INVALID, "linear_test: rows (the first part's a multiple of 256), tile 64, 128 or 256, 1 to 64 slices");
+            chosen[i] = MatmulPart{p.rows, p.tile >> 7, p.slices, 0, 0};
+            rows += p.rows;
+        }
+        if (rows != m.M) FT_FAIL(CLIPVIT_E_INVALID, "linear_test: the parts' rows are not M");
+        const MatmulPlan p = matmul_plan(m, chosen, count);
+        if (need) {
+            *need = matmul_workspace(p);
+            return CLIPVIT_OK;
+        }
+        if ((bytes && !workspace) || ((size_t)workspace & 255) || launch_matmul((hipStream_t)stream, a->dtype, m, p, workspace, bytes))
+            FT_FAIL(CLIPVIT_E_INVALID, std::string("linear_test: ") + WORKSPACE);
+        FT_LAUNCHED();
+        return CLIPVIT_OK;
+    });
+}
+
 int clipvit_linear_grad_workspace(const clipvit_linear_grad_args* a, size_t* bytes) {
     return guarded([&]() -> int {
         if (!bytes) FT_FAIL(CLIPVIT_E_INVALID, "null argument");

@@ -731,16 +731,7 @@ __global__ __launch_bounds__(256) void repack_kernel(RepackArgs a, RepackArgs b,
 
 bool loadable(const u16* p, int64_t ld, int len) { return ((size_t)p & 15) == 0 && ld % 8 == 0 && len % 8 == 0; }
 
-// One launch: tile (0 = 64 x 64, 1 = 128 x 128, 2 = 256 x 256), slices of k, and its estimated time.
-struct Part {
-    int rows, tile, S, kslice;
-    double us;
-};
-struct Plan {
-    size_t a_bytes, b_bytes, part_bytes;
-    int N4, parts;
-    Part part[2];  // rows [0, part[0].rows), then the rest
-};
+typedef MatmulPart Part;
 
 int tiles(int M, int N, int t) { return ((M + t - 1) / t) * ((N + t - 1) / t); }
 
@@ -770,39 +761,6 @@ Part best_part(int M, int N, int nk, int N4) {
         }
     }
     return b;
-}
-
-Plan plan_of(const Matmul& a) {
-    Plan p{};
-    const int al = a.a_k ? a.K : a.M, ar = a.a_k ? a.M : a.K, bl = a.b_k ? a.K : a.N, br = a.b_k ? a.N : a.K;
-    auto up = [](int64_t v, int64_t q) { return (v + q - 1) / q * q; };
-    if (a.K > 0 && !loadable(a.A, a.lda, al)) p.a_bytes = (size_t)up((int64_t)ar * up(al, 8) * 2, 256);
-    if (a.K > 0 && !loadable(a.B, a.ldb, bl)) p.b_bytes = (size_t)up((int64_t)br * up(bl, 8) * 2, 256);
-    const int nk = (a.K + 63) / 64, nN = (a.N + 255) / 256, nM = (a.M + 255) / 256;
-    p.N4 = (int)up(a.N, 4);
-    p.parts = 1;
-    p.part[0] = best_part(a.M, a.N, nk, p.N4);
-    // whole rounds of 256-wide tiles as one launch and the remaining rows as another with tiles of its own, where
-    // that is estimated faster (the launch itself 3 us): 36928 x 4096 x 1024 is 580 tiles, 2.3 rounds in the time of 3
-    const int round_rows = nN <= 256 ? 256 / nN : 0;  // tile rows of one round
-    if (round_rows && (256 % nN) * 16 <= 256 && nM > round_rows) {
-        const int rows = nM / round_rows * round_rows * 256;
-        if (rows < a.M) {
-            const Part main{rows, 2, 1, nk > 0 ? nk : 1, cost_us(2, tiles(rows, a.N, 256), 1, nk, 0)};
-            const Part rest = best_part(a.M - rows, a.N, nk, p.N4);
-            if (main.us + rest.us + 3.0 < p.part[0].us) {
-                p.parts = 2;
-                p.part[0] = main;
-                p.part[1] = rest;
-            }
-        }
-    }
-    for (int i = 0; i < p.parts; ++i) {
-        const Part& q = p.part[i];
-        const size_t bytes = q.S > 1 ? (size_t)q.S * q.rows * p.N4 * 4 : 0;
-        if (bytes > p.part_bytes) p.part_bytes = bytes;
-    }
-    return p;
 }
 
 template <typename T, bool AK, bool BK>
@@ -851,16 +809,49 @@ RepackArgs repack_of(const u16*& p, int64_t& ld, int rows, int len, void* dst) {
 
 }  // namespace
 
-size_t matmul_workspace(const Matmul& a) {
-    if (a.M <= 0 || a.N <= 0) return 0;
-    const Plan p = plan_of(a);
-    return p.a_bytes + p.b_bytes + p.part_bytes;
+MatmulPlan matmul_plan(const Matmul& a, const MatmulPart* chosen, int parts) {
+    MatmulPlan p{};
+    if (a.M <= 0 || a.N <= 0) return p;
+    const int al = a.a_k ? a.K : a.M, ar = a.a_k ? a.M : a.K, bl = a.b_k ? a.K : a.N, br = a.b_k ? a.N : a.K;
+    auto up = [](int64_t v, int64_t q) { return (v + q - 1) / q * q; };
+    if (a.K > 0 && !loadable(a.A, a.lda, al)) p.a_bytes = (size_t)up((int64_t)ar * up(al, 8) * 2, 256);
+    if (a.K > 0 && !loadable(a.B, a.ldb, bl)) p.b_bytes = (size_t)up((int64_t)br * up(bl, 8) * 2, 256);
+    const int nk = (a.K + 63) / 64, nN = (a.N + 255) / 256, nM = (a.M + 255) / 256;
+    p.N4 = (int)up(a.N, 4);
+    p.parts = chosen ? parts : 1;
+    for (int i = 0; i < parts && chosen; ++i) {
+        const int ks = nk > 0 ? (nk + chosen[i].S - 1) / chosen[i].S : 1;
+        p.part[i] = Part{chosen[i].rows, chosen[i].tile, nk > 0 ? (nk + ks - 1) / ks : 1, ks, 0};
+    }
+    if (!chosen) p.part[0] = best_part(a.M, a.N, nk, p.N4);
+    // whole rounds of 256-wide tiles as one launch and the remaining rows as another with tiles of its own, where
+    // that is estimated faster (the launch itself 3 us): 36928 x 4096 x 1024 is 580 tiles, 2.3 rounds in the time of 3
+    const int round_rows = nN <= 256 ? 256 / nN : 0;  // tile rows of one round
+    if (!chosen && round_rows && (256 % nN) * 16 <= 256 && nM > round_rows) {
+        const int rows = nM / round_rows * round_rows * 256;
+        if (rows < a.M) {
+            const Part main{rows, 2, 1, nk > 0 ? nk : 1, cost_us(2, tiles(rows, a.N, 256), 1, nk, 0)};
+            const Part rest = best_part(a.M - rows, a.N, nk, p.N4);
+            if (main.us + rest.us + 3.0 < p.part[0].us) {
+                p.parts = 2;
+                p.part[0] = main;
+                p.part[1] = rest;
+            }
+        }
+    }
+    for (int i = 0; i < p.parts; ++i) {
+        const Part& q = p.part[i];
+        const size_t bytes = q.S > 1 ? (size_t)q.S * q.rows * p.N4 * 4 : 0;
+        if (bytes > p.part_bytes) p.part_bytes = bytes;
+    }
+    return p;
 }
 
-int launch_matmul(hipStream_t s, int dtype, const Matmul& a0, void* ws, size_t ws_bytes) {
+size_t matmul_workspace(const MatmulPlan& p) { return p.a_bytes + p.b_bytes + p.part_bytes; }
+
+int launch_matmul(hipStream_t s, int dtype, const Matmul& a0, const MatmulPlan& p, void* ws, size_t ws_bytes) {
     if (a0.M <= 0 || a0.N <= 0) return 0;
     Matmul a = a0;
-    const Plan p = plan_of(a);
     if (p.a_bytes + p.b_bytes + p.part_bytes > ws_bytes) return -1;
     unsigned char* w = (unsigned char*)ws;
     if (p.a_bytes || p.b_bytes) {

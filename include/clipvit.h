@@ -426,6 +426,21 @@ int clipvit_gemm_mx8_test(void* stream, const unsigned char* A8_dev, const unsig
                           const float* W_dev, const float* bias_dev, void* C_dev,
                           unsigned char* sC_dev, int M, int N, int K, int epi, int variant);
 
+/* One launch of a fine-tuning operator's matrix product: `rows` rows of C in tiles `tile` wide (64, 128 or 256), k in
+ * `slices` of `kslice` k-tiles of 64 (the last slice may hold fewer). */
+typedef struct {
+    int rows, tile, slices, kslice;
+} clipvit_matmul_part;
+
+/* The launches that a product C [M, N] over K takes by the library's rule: one, or two of which the first has the top rows
+ * (parts holds two). Host only. A Linear's forward is (M, N, K), its dx (M, K, N) and its dw (N, K, M). */
+int clipvit_matmul_plan_test(int64_t M, int64_t N, int64_t K, clipvit_matmul_part* parts, int* count);
+
+/* clipvit_linear with one or two chosen launches instead of the rule's (kslice is not read; more slices than k-tiles become as
+ * many as there are). need non-NULL: only writes the bytes of workspace there and launches nothing. */
+int clipvit_linear_test(void* stream, const clipvit_linear_args* args, const clipvit_matmul_part* parts, int count,
+                        void* workspace, size_t bytes, size_t* need);
+
 /* The 24-bit residual stream format of the 16-bit forward: x fp32 [n] (n % 4 == 0)
  * -> planes [3n bytes: n u16 upper halves, then n bytes of the next 8 mantissa bits, rounded to
  * nearest at bit 8] -> back fp32 [n], by the kernels' own encode / decode functions. */
