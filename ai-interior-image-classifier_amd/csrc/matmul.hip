@@ -798,12 +798,14 @@ Matmul rows_of(const Matmul& a, int m0, int rows) {
     return r;
 }
 
-// rows whose length or stride or base the 16-byte loads cannot take, as rows of the length rounded up to 8
+// rows whose length or stride or base the 16-byte loads cannot take, as rows of the length rounded up to 8. A single row may
+// be longer than a stride that the tiles' 32-bit offsets hold (a multiple of 2^26 elements wraps to row 0): it gets one that
+// puts the k rows after it outside a tile's resource.
 RepackArgs repack_of(const u16*& p, int64_t& ld, int rows, int len, void* dst) {
     const int cp = (len + 7) / 8 * 8;
     const RepackArgs r{p, ld, rows, len, (u16*)dst, cp};
     p = (const u16*)dst;
-    ld = cp;
+    ld = rows > 1 ? cp : 4096;
     return r;
 }
 
