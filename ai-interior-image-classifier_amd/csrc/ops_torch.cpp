@@ -5,9 +5,11 @@
 // because a node written in Python runs under the interpreter on autograd's own thread: a training step of a small Linear
 // took 130 us of host time that way, most of it handing the interpreter over and waking the threads.
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <unordered_set>
@@ -134,7 +136,15 @@ void check_capture(const Tensor& first, std::initializer_list<const Tensor*> ope
         for (const auto& edge : node->next_edges()) visit(edge.function);
     }
 }
+// The library fills the outputs outside torch's dispatcher, so a trace would record their allocation alone and replay
+// uninitialised memory.
+void check_eager() {
+    TORCH_CHECK(!torch::jit::tracer::isTracing() && !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY) &&
+                    !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::FAKE),
+                "the fine-tuning operators cannot be traced (torch.jit.trace, make_fx, fake tensors): call them eagerly or capture a graph");
+}
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
+    check_eager();
     for (const Tensor* t : ts)
         TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), "the fine-tuning operators have no forward-mode derivative");
     if (!at::GradMode::is_enabled()) return false;

@@ -24,7 +24,8 @@ caching allocator. There is no CPU fallback: CPU tensors raise ``ClipVitError``.
 into a graph through ``torch.autograd.grad`` after the usual warm-up on a side stream, once no eager autograd graph of
 the same leaves is alive (a capture that finds one raises). They are differentiable once (no ``create_graph``), and
 keep for the backward pass only what the wanted gradients read: a frozen weight's x, or a frozen x's weight, may change
-or be freed after the forward. Matrices of more than one row hold fewer than 2^22 columns.
+or be freed after the forward. They run eagerly or in a captured graph and refuse to be traced (``torch.jit.trace``,
+``make_fx``). Matrices of more than one row hold fewer than 2^22 columns.
 """
 from __future__ import annotations
 

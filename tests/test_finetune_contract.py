@@ -2,6 +2,7 @@
 import ctypes
 
 import pytest
+import torch
 
 from interior_amd import _lib, ops
 from test_finetune import linear_grad_args, lora_grad_args
@@ -40,3 +41,26 @@ def test_binding_refuses_a_library_without_an_entry(name):
                 m.set_library(bad, _lib.ClipVitError)
     finally:
         m.set_library(table, _lib.ClipVitError)
+
+
+def tracers():
+    from torch._subclasses import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def fake(call, x):
+        with FakeTensorMode(allow_non_fake_inputs=True):
+            call(x)
+
+    return {"jit.trace": lambda call, x: torch.jit.trace(call, x), "make_fx": lambda call, x: make_fx(call)(x),
+            "make_fx symbolic": lambda call, x: make_fx(call, tracing_mode="symbolic")(x), "fake": fake}
+
+
+@pytest.mark.parametrize("how", ["jit.trace", "make_fx", "make_fx symbolic", "fake"])
+def test_binding_refuses_to_be_traced(how):
+    """A trace would record the output's allocation and nothing that fills it. (The binding itself: it asks before it looks
+    at the tensors' device.)"""
+    m, w, A, B = ops._binding(), torch.zeros(5, 8), torch.zeros(8, 2), torch.zeros(2, 5)
+    for call in (lambda x: m.linear(x, w, None, None, 0, 0.0, 0, 0, None), lambda x: m.dropout(x, None, 0.5, 0, 0, None),
+                 lambda x: m.lora_linear(x, w, A, B, None, 1.0, 0.0, 0, 0, None)):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            tracers()[how](call, torch.zeros(4, 8))
