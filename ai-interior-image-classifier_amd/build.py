@@ -8,8 +8,11 @@ when it, a ``csrc/*.h`` header or ``include/clipvit.h`` is newer than its object
 from __future__ import annotations
 
 import os
+import shutil
 import subprocess
 import sys
+import sysconfig
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -72,29 +75,41 @@ def _compile(src: Path) -> tuple[Path, str]:
     return obj, r.stderr
 
 
-def _build_torch_binding() -> None:
-    """_ops_torch.so: the autograd binding of the fine-tuning operators (host C++ against this torch's headers)."""
+def _build_torch_binding() -> str:
+    """_ops_torch.so: the autograd binding of the fine-tuning operators (host C++ against this torch's headers). Returns what
+    it lacks where it cannot be built; an older one is then taken away, since it may not fit the library."""
     src = CSRC / "ops_torch.cpp"
     if not _needs(TORCH_LIB, [src, INCLUDE / "clipvit.h", Path(__file__)]):
-        return
-    import sysconfig
-
-    import torch
-    from torch.utils.cpp_extension import include_paths
+        return ""
+    TORCH_LIB.unlink(missing_ok=True)
+    cxx, python = os.environ.get("CXX", "g++"), Path(sysconfig.get_paths()["include"])
+    try:
+        import torch
+        from torch.utils.cpp_extension import include_paths
+    except ImportError as e:
+        return f"torch ({e})"
+    if not shutil.which(cxx):
+        return f"a C++ compiler ({cxx})"
+    for header, dirs in (("torch/extension.h", include_paths()), ("Python.h", [python])):
+        if not any((Path(d) / header).exists() for d in dirs):
+            return f"the header {header}"
     tmp = TORCH_LIB.with_suffix(".so.tmp")
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1",
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1",
            "-DUSE_ROCM=1", f"-I{INCLUDE}", "-isystem/opt/rocm/include",
-           *(f"-isystem{d}" for d in include_paths()), f"-isystem{sysconfig.get_paths()['include']}",
+           *(f"-isystem{d}" for d in include_paths()), f"-isystem{python}",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", str(src), "-o", str(tmp),
            f"-L{Path(torch.__file__).parent / 'lib'}", "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed for {src.name}:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, TORCH_LIB)
+    return ""
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile and link libclipvit_hip.so and the torch binding beside it; return the library's path."""
+    """Compile and link libclipvit_hip.so, whose C entry points need no torch, and the torch binding beside it; return the
+    library's path. Without what the binding needs the library is built all the same, with a warning: ``interior_amd.ops``
+    raises then."""
     BUILD.mkdir(exist_ok=True)
     srcs = _sources()
     if force:
@@ -105,7 +120,6 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     with ThreadPoolExecutor(max_workers=max(jobs, 1)) as ex:
         binding = ex.submit(_build_torch_binding)
         results = list(ex.map(_compile, srcs))
-        binding.result()
     objs = [o for o, _ in results]
     if verbose:
         for o, err in results:
@@ -118,6 +132,8 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         os.replace(tmp, LIB)
+    if lacks := binding.result():
+        warnings.warn(f"{TORCH_LIB.name} is not built, interior_amd.ops cannot be used: {lacks} is missing", stacklevel=2)
     return LIB
 
 
