@@ -64,7 +64,8 @@ __device__ __forceinline__ unsigned pack2(float lo, float hi) {
 __device__ __forceinline__ float quick_gelu(float x) {
     return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-2.4554669595930157f * x));
 }
-// the same on two values (bit-identical): the multiplies and the add as v_pk_*_f32
+// the same on two values (bit-identical). The units that call it are built without v_pk_*_f32: the pairs are two scalar
+// instructions (as packed ones c_fc takes 3 % less at B/32, see NO_PACKED_F32 in build.py)
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void quick_gelu2(float& a, float& b) {
     const f32x2 y = {a, b};

@@ -249,7 +249,7 @@ __device__ __forceinline__ void p32_body(const GemmArgs& a, int ntiles, unsigned
 #pragma unroll
             for (int f = 0; f < 4; ++f)
 #pragma unroll
-                for (int rr = 0; rr < 4; rr += 2) {  // v_pk_add_f32
+                for (int rr = 0; rr < 4; rr += 2) {
                     const f32x2 s = (f32x2){acc[f][fm][rr], acc[f][fm][rr + 1]} + (f32x2){bv[f][rr], bv[f][rr + 1]};
                     v[4 * f + rr] = s.x;
                     v[4 * f + rr + 1] = s.y;
