@@ -37,7 +37,7 @@ CFLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", f"-I{INCLUDE}"
 # only the GEMMs get it.
 SRC_FLAGS = {"gemm": ["-mllvm", "--amdgpu-sched-strategy=max-memory-clause"]}
 # No v_pk_{add,mul,fma}_f32: the compiler makes them from ordinary float code, and some of their forms
-# have given wrong results on this machine. Same box, in turn: c_fc 0.728 -> 0.752 ms a forward without them and B/32 87.6k ->
+# have given wrong results on this machine. Timed in turn: c_fc 0.728 -> 0.752 ms a forward without them and B/32 87.6k ->
 # 86.7k img/s (its QuickGELU epilogue was packed), L/14@336 2339 -> 2327. norm.hip is still built with them: without, its sums contract
 # differently and the encoder's outputs change in their last bits (every other unit's output is the same bits
 # either way, on B/32, B/16 and L/14@336 in fp16, bf16 and MX-fp8 and on the text tower).
