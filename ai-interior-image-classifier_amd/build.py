@@ -29,20 +29,17 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # --amdgpu-mfma-vgpr-form: MFMA accumulators in VGPRs. Without it the backend put the
 # accumulators of tiles whose occupancy allows > 256 registers (the class-token tail's 2-wave
 # 64x64 tile) in AGPRs and rotated them with v_accvgpr_mov/read/write every k-step.
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32: the compiler makes them from ordinary float code, and some of their forms
+# have given wrong results on this machine. Timed in turn: c_fc 0.728 -> 0.752 ms a forward without them and B/32 87.6k ->
+# 86.7k img/s (its QuickGELU epilogue was packed), L/14@336 2339 -> 2327. No output changes: where the compiler chose which
+# products of a sum to fuse (the LayerNorms' variances, ln_row), the sum is written out.
 CFLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", f"-I{INCLUDE}", f"-I{CSRC}",
-          "-mllvm", "--amdgpu-mfma-vgpr-form", "-Wno-unused-result", "-Wno-unused-value"]
+          "-mllvm", "--amdgpu-mfma-vgpr-form", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wno-unused-result", "-Wno-unused-value"]
 # Per-source flags. gemm.hip: the max-memory-clause machine scheduler (clusters each k-step's
 # staging loads). Same-box A/B of the two builds (profiles/design_r05.md §11): B/32 +0.2 / +0.6 %, B/16
 # +0.5 %, L/14@336 +0.7 / +1.0 % img/s, patch GEMM -7 %; on attention.hip it cost 6 %, so
 # only the GEMMs get it.
 SRC_FLAGS = {"gemm": ["-mllvm", "--amdgpu-sched-strategy=max-memory-clause"]}
-# No v_pk_{add,mul,fma}_f32: the compiler makes them from ordinary float code, and some of their forms
-# have given wrong results on this machine. Timed in turn: c_fc 0.728 -> 0.752 ms a forward without them and B/32 87.6k ->
-# 86.7k img/s (its QuickGELU epilogue was packed), L/14@336 2339 -> 2327. norm.hip is still built with them: without, its sums contract
-# differently and the encoder's outputs change in their last bits (every other unit's output is the same bits
-# either way, on B/32, B/16 and L/14@336 in fp16, bf16 and MX-fp8 and on the text tower).
-NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-PACKED_F32_UNITS = {"norm"}
 # options a unit is built without (none since the r05 one-wave-per-SIMD probes left the build)
 SRC_DROP: dict[str, list[str]] = {}
 
@@ -67,8 +64,6 @@ def _compile(src: Path) -> tuple[Path, str]:
     for f in SRC_DROP.get(src.stem, []):  # a dropped -mllvm option takes its -mllvm with it
         i = flags.index(f)
         del flags[i - 1:i + 1]
-    if src.stem not in PACKED_F32_UNITS:
-        flags += NO_PACKED_F32
     cmd = [HIPCC, *flags, *SRC_FLAGS.get(src.stem, []), "-c", str(src), "-o", str(obj)]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:

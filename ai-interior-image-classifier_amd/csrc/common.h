@@ -65,7 +65,7 @@ __device__ __forceinline__ float quick_gelu(float x) {
     return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-2.4554669595930157f * x));
 }
 // the same on two values (bit-identical). The units that call it are built without v_pk_*_f32: the pairs are two scalar
-// instructions (as packed ones c_fc takes 3 % less at B/32, see NO_PACKED_F32 in build.py)
+// instructions (as packed ones c_fc takes 3 % less at B/32; build.py says why not)
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void quick_gelu2(float& a, float& b) {
     const f32x2 y = {a, b};
@@ -382,19 +382,41 @@ __host__ __device__ inline int grid_for(int nM, int nN, int xn) {
 }
 
 // Row LayerNorm helpers: one wave per row, D = 64 * 4 * V (V float4 per lane).
-template <int V>
+// Squares of a lane's four values, summed in one of three ways that differ in the last bit: the first of each pair fused onto
+// the second's square, the second onto the first's, or not fused. Written out, so that no compiler option chooses.
+enum SquareSum { SQ_FIRST, SQ_SECOND, SQ_PLAIN };
+template <SquareSum S>
+__device__ __forceinline__ float square4(const float4& d) {
+#pragma clang fp contract(off)
+    if constexpr (S == SQ_FIRST) return __builtin_fmaf(d.x, d.x, d.y * d.y) + __builtin_fmaf(d.z, d.z, d.w * d.w);
+    else if constexpr (S == SQ_SECOND) return __builtin_fmaf(d.y, d.y, d.x * d.x) + __builtin_fmaf(d.w, d.w, d.z * d.z);
+    else return (d.x * d.x + d.y * d.y) + (d.z * d.z + d.w * d.w);
+}
+// TAIL: the last float4s of rows of more than 512 in the other two ways, as the encoder's LayerNorms have had them since they
+// were measured against the golden images: that order keeps every output's bits (all of them SQ_FIRST moves two of the images'
+// near-ties and the MX-fp8 features past their bound)
+template <int V, bool TAIL>
+constexpr SquareSum square_sum(int i) {
+    return !TAIL || V < 3 ? SQ_FIRST : i == V - 1 ? SQ_PLAIN : i == V - 2 || V == 3 ? SQ_SECOND : SQ_FIRST;
+}
+template <int V, bool TAIL, int I = 0>
+__device__ __forceinline__ float square_row(const float4 (&v)[V], float q) {
+#pragma clang fp contract(off)
+    if constexpr (I == V) return q;
+    else return square_row<V, TAIL, I + 1>(v, q + square4<square_sum<V, TAIL>(I)>(v[I]));
+}
+template <int V, bool TAIL = false>
 __device__ __forceinline__ void ln_row(float4 (&v)[V], const float* __restrict__ gm,
                                        const float* __restrict__ bt, int lane, float D) {
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) s += (v[i].x + v[i].y) + (v[i].z + v[i].w);
     const float mean = wave_sum(s) / D;
-    float q = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         v[i].x -= mean; v[i].y -= mean; v[i].z -= mean; v[i].w -= mean;
-        q += (v[i].x * v[i].x + v[i].y * v[i].y) + (v[i].z * v[i].z + v[i].w * v[i].w);
     }
+    const float q = square_row<V, TAIL>(v, 0.f);
     const float rstd = rsqrtf(wave_sum(q) / D + 1e-5f);
 #pragma unroll
     for (int i = 0; i < V; ++i) {

@@ -262,7 +262,7 @@ __global__ __launch_bounds__(256) void embed_ln_kernel(float* __restrict__ x, vo
         const float4 a = *(const float4*)(src + c), p = *(const float4*)(pr + c);
         v[i] = make_float4(a.x + p.x, a.y + p.y, a.z + p.z, a.w + p.w);
     }
-    ln_row<V>(v, gp, bp, lane, (float)D);
+    ln_row<V, true>(v, gp, bp, lane, (float)D);
     if constexpr (X24) {  // x16 = the 24-bit residual planes; x keeps the patch rows
 #pragma unroll
         for (int i = 0; i < V; ++i)
@@ -273,7 +273,7 @@ __global__ __launch_bounds__(256) void embed_ln_kernel(float* __restrict__ x, vo
 #pragma unroll
         for (int i = 0; i < V; ++i) *(float4*)(xr + (lane + 64 * i) * 4) = v[i];
     }
-    ln_row<V>(v, g1, b1, lane, (float)D);
+    ln_row<V, !Q8>(v, g1, b1, lane, (float)D);
     if constexpr (Q8) store_row_q8<V>((unsigned char*)h + (size_t)row * D, sq + (size_t)row * (D / 32), v, lane);
     else store_row16<T, V>((u16*)h + (size_t)row * D, v, lane);
 }
@@ -290,8 +290,7 @@ __device__ __forceinline__ void row_stats128(const float4 (&v)[V], float2* __res
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) s += __shfl_xor(s, o, 64);
         const float mean = s * (1.0f / 128.f);
-        const float a = v[i].x - mean, b = v[i].y - mean, c = v[i].z - mean, d = v[i].w - mean;
-        float q = (a * a + b * b) + (c * c + d * d);
+        float q = square4<SQ_FIRST>(make_float4(v[i].x - mean, v[i].y - mean, v[i].z - mean, v[i].w - mean));
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) q += __shfl_xor(q, o, 64);
         if ((lane & 31) == 0) st[2 * i + (lane >> 5)] = make_float2(mean, q);
@@ -322,7 +321,7 @@ __global__ __launch_bounds__(256) void embed_stats_kernel(float* __restrict__ x,
         const float4 a = *(const float4*)(src + c), p = *(const float4*)(pr + c);
         v[i] = make_float4(a.x + p.x, a.y + p.y, a.z + p.z, a.w + p.w);
     }
-    ln_row<V>(v, gp, bp, lane, (float)D);
+    ln_row<V, true>(v, gp, bp, lane, (float)D);
     if (x24) {
 #pragma unroll
         for (int i = 0; i < V; ++i) x24_store(x24, (size_t)rows * D * 2, (size_t)row * D + (lane + 64 * i) * 4, v[i]);
@@ -345,6 +344,7 @@ __global__ __launch_bounds__(256) void lnfold_prep_kernel(const float* __restric
     const int n = blockIdx.x, tid = threadIdx.x;
     float s = 0.f, bb = 0.f;
     for (int k = tid; k < K; k += 256) {
+#pragma clang fp contract(off)  // bb's product is not fused onto its sum
         const float w = W[(size_t)n * K + k], wg = w * gm[k];
         Wg[(size_t)n * K + k] = wg;
         s += T::to_f32(T::from_f32(wg));
@@ -380,7 +380,7 @@ __global__ __launch_bounds__(256) void layernorm_kernel(const float* __restrict_
     float4 v[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) v[i] = *(const float4*)(xr + (lane + 64 * i) * 4);
-    ln_row<V>(v, gm, bt, lane, (float)D);
+    ln_row<V, !Q8>(v, gm, bt, lane, (float)D);
     if constexpr (Q8) store_row_q8<V>((unsigned char*)h + (size_t)row * D, sq + (size_t)row * (D / 32), v, lane);
     else store_row16<T, V>((u16*)h + (size_t)row * D, v, lane);
 }
@@ -462,7 +462,7 @@ __global__ __launch_bounds__(256) void add_layernorm_kernel(void* __restrict__ x
             }
         }
         if constexpr (STORE_X && X16) store_x16<V>(x16 + (size_t)row * D, v[r], lane);
-        ln_row<V>(v[r], gm, bt, lane, (float)D);
+        ln_row<V, !Q8>(v[r], gm, bt, lane, (float)D);
         if constexpr (Q8) store_row_q8<V>((unsigned char*)h + (size_t)row * D, sq + (size_t)row * (D / 32), v[r], lane);
         else if constexpr (BLKH) {
             const int m = (threadIdx.x >> 6) * RPW + r;  // row slot inside the workgroup's rows
@@ -531,7 +531,7 @@ __global__ __launch_bounds__(256) void splitk_resid_ln_kernel(float* __restrict_
         *(float4*)(xr + (lane + 64 * i) * 4) = v[i];
     }
     if constexpr (LN) {
-        ln_row<V>(v, gm, bt, lane, (float)D);
+        ln_row<V, true>(v, gm, bt, lane, (float)D);
         store_row16<T, V>(h + (size_t)row * D, v, lane);
     }
 }

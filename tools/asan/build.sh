@@ -10,7 +10,7 @@ OUT=$ROOT/tools/asan/out
 mkdir -p "$OUT"
 HIPCC=${HIPCC:-/opt/rocm/bin/hipcc}
 SAN="-Xarch_host -fsanitize=address -Xarch_host -fsanitize=undefined -Xarch_host -fno-omit-frame-pointer"
-FLAGS="-O1 -g -std=c++17 -fPIC --offload-arch=gfx950 -I$ROOT/include -I$ROOT/ai-interior-image-classifier_amd/csrc -mllvm --amdgpu-mfma-vgpr-form -Wno-unused-result -Wno-unused-value"
+FLAGS="-O1 -g -std=c++17 -fPIC --offload-arch=gfx950 -I$ROOT/include -I$ROOT/ai-interior-image-classifier_amd/csrc -mllvm --amdgpu-mfma-vgpr-form -Xclang -target-feature -Xclang -packed-fp32-ops -Wno-unused-result -Wno-unused-value"
 objs=""
 for src in "$ROOT"/ai-interior-image-classifier_amd/csrc/*.hip; do
   o=$OUT/$(basename "$src" .hip).o
