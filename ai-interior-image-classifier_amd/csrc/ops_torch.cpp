@@ -165,10 +165,12 @@ struct OpNode : Node {
     SavedVariable offset_dev;
     bool released = false;
 
-    // the dropout arguments for the backward pass; `off` keeps their tensor
-    clipvit_dropout_args begin(Tensor& off, const Tensor& dy) {
+    void begin() const {
         TORCH_CHECK(!released, torch::autograd::ERR_BACKWARD_TWICE);
         TORCH_CHECK(!at::GradMode::is_enabled(), "the fine-tuning operators are differentiable once: their backward takes no create_graph");
+    }
+    // the dropout arguments for a backward pass that draws the mask again; `off` keeps their tensor
+    clipvit_dropout_args mask(Tensor& off, const Tensor& dy) const {
         off = offset_dev.unpack();
         TORCH_CHECK(!off.defined() || !dy.defined() || (off.device() == dy.device() && off.scalar_type() == at::kLong && off.numel() == 1),
                     "a saved tensor came back with another size, type or device than it was saved with");
@@ -178,6 +180,7 @@ struct OpNode : Node {
     }
     void set_dropout(const clipvit_dropout_args& d, const Tensor& off) {
         drop = d;
+        drop.offset_dev = nullptr;  // (the saved tensor's, in mask)
         offset_dev = SavedVariable(off, false);
     }
     void release_variables() override {
@@ -256,8 +259,7 @@ struct LinearNode : OpNode {
     }
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
-        Tensor offset_keep;
-        const clipvit_dropout_args drop_args = begin(offset_keep, grads[0]);
+        begin();
         const Tensor& dy = grads[0];
         if (!dy.defined()) return variable_list(4);
         const int64_t m = rows_in(x_shape), k = x_shape.back(), n = dy.size(-1);
@@ -289,7 +291,8 @@ struct LinearNode : OpNode {
             a.dx = ptr(dx);
             a.dw = ptr(dw);
             a.db = ptr(db);
-            a.dropout = drop_args;
+            Tensor offset_keep;
+            a.dropout = mask(offset_keep, dy);
             const Workspace ws(api.linear_grad_workspace, a, dy);
             check(api.linear_grad(on.stream, &a, ws.p, ws.bytes));
         }
@@ -345,11 +348,12 @@ struct DropoutNode : OpNode {
     std::string name() const override { return "DropoutBackward"; }
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
-        Tensor offset_keep;
-        const clipvit_dropout_args drop_args = begin(offset_keep, grads[0]);
+        begin();
         const Tensor& dy = grads[0];
         if (!dy.defined()) return variable_list(2);
-        return {task_should_compute_output(0) ? dropout_call(dy, Tensor(), drop_args) : Tensor(), task_should_compute_output(1) ? dy : Tensor()};
+        Tensor offset_keep, dx;
+        if (task_should_compute_output(0)) dx = dropout_call(dy, Tensor(), mask(offset_keep, dy));
+        return {dx, task_should_compute_output(1) ? dy : Tensor()};
     }
 };
 
@@ -419,8 +423,7 @@ struct LoraNode : OpNode {
     }
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
-        Tensor offset_keep;
-        const clipvit_dropout_args drop_args = begin(offset_keep, grads[0]);
+        begin();
         const Tensor& dy = grads[0];
         if (!dy.defined()) return variable_list(5);
         const int64_t m = rows_in(x_shape), k = x_shape.back(), n = dy.size(-1), r = rank;
@@ -462,7 +465,9 @@ struct LoraNode : OpNode {
         a.db_factor = ptr(dB);
         a.dbias = ptr(db);
         a.scaling = scaling;
-        a.dropout = drop_args;
+        Tensor offset_keep;
+        a.dropout = drop;
+        if (nx || nA) a.dropout = mask(offset_keep, dy);  // (du's scale is 1 / (1 - p) all the same)
         const Workspace ws(api.lora_grad_workspace, a, dy);
         check(api.lora_grad(on.stream, &a, ws.p, ws.bytes));
         return {dx, dw, dA, dB, db};

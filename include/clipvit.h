@@ -273,7 +273,9 @@ typedef enum {
  * x [M, K] and w [N, K] are views with two strides, one of them 1; the other is below 2^22 and at least the row's
  * length. y and residual have unit column stride. slope (or NULL, with an activation): act'(z) as [M, N] contiguous
  * 16-bit codes, what the gradient of the same dtype takes: off by at most 2^-15 and, relative, 2^-8 (BF16, down to 2^-118)
- * or 2^-10 (F16, down to 2^-33; less is 0). Rows of any length, stride and alignment
+ * or 2^-10 (F16, down to 2^-33; less is 0). A code is a sign bit and a magnitude m of 15 bits, 0x7fff for NaN: with M = 7 and
+ * L = -118 (BF16) or M = 9 and L = -33 (F16), and J = (M - 14 - L) 2^M + 1, it is (m - J + 2^M) 2^-14 from m = J on, 0 for
+ * m = 0, and between them the float of bits (m + (127 + L) 2^M - 1) << (23 - M). Rows of any length, stride and alignment
  * are taken; those that 16-byte loads cannot address are copied into the workspace first. y must not overlap an
  * input other than an identical residual. */
 typedef struct {

@@ -83,3 +83,24 @@ def test_operands_that_no_gradient_reads_may_change(gpu):
     y = ops.linear(t["x"], t["w"], None, r, dropout_p=0.5, seed=1, offset=offset)
     offset += 1
     assert torch.equal(torch.autograd.grad(y, r, dy)[0], dy)
+
+
+@pytest.mark.parametrize("call, draws, others", [
+    (lambda t, off: ops.linear(t["x"], t["w"], t["b"], t["r"], activation="silu", dropout_p=0.5, seed=1, offset=off), "xwb", "r"),
+    (lambda t, off: ops.dropout(t["x"], 0.5, seed=1, offset=off, residual=t["r2"]), "x", ["r2"]),
+    (lambda t, off: ops.lora_linear(t["x"], t["w"], t["A"], t["B"], t["b"], dropout_p=0.5, seed=1, offset=off), "xA", "wBb")])
+def test_changed_offset_stops_only_what_draws_the_mask(gpu, call, draws, others):
+    """A gradient that does not draw the mask again is the same after the offset has changed; one that does is refused."""
+    t, offset = operands(gpu), torch.zeros(1, dtype=torch.int64, device=gpu)
+    t["r2"] = rand(M, K, seed=8).to(gpu)
+    for leaf in t.values():
+        leaf.requires_grad_()
+    y = call(t, offset)
+    dy = rand(*y.shape, seed=9).to(gpu)
+    want = torch.autograd.grad(y, [t[k] for k in others], dy, retain_graph=True)
+    offset += 1
+    got = torch.autograd.grad(y, [t[k] for k in others], dy, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for k in draws:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y, t[k], dy, retain_graph=True)
